@@ -9,7 +9,9 @@ from . import config  # noqa: F401
 from .unit import DualVGRUnit_multiple, param_table  # noqa: F401
 from .head import AnswerHead  # noqa: F401
 from .clip import ClipEncoder  # noqa: F401
-from .inputs import HipLinear, WordFeatures  # noqa: F401
+from .inputs import HipLinear, TokenEmbedding, WordFeatures, embed_tokens  # noqa: F401
+from .attention import CrossAttention, cross_attention  # noqa: F401
+from .losses import distillation_loss  # noqa: F401
 from .store import FeatureStore, VideoQAFlatLoader, write_flat  # noqa: F401
 from .model import DualVGR, init_modules  # noqa: F401
 from .trainer import ClipAdam, TrainStep  # noqa: F401

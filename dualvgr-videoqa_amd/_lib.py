@@ -5,13 +5,16 @@ product entry point that needs it.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
+import weakref
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DVGR_LIB") or os.path.join(_HERE, "libdvgr_hip.so")   # DVGR_LIB: debug builds only
 
 DVGR_F32, DVGR_BF16, DVGR_BF16X3 = 0, 1, 2
+DVGR_ELEM_F32, DVGR_ELEM_BF16, DVGR_ELEM_F16 = 0, 1, 2
 
 # enum dvgr_param_kind
 (P_QA_W1, P_QA_B1, P_QA_W2, P_QA_B2, P_WQ, P_BQ, P_GAT_W, P_GAT_B, P_GAT_A, P_GAT_C,
@@ -22,7 +25,7 @@ DVGR_F32, DVGR_BF16, DVGR_BF16X3 = 0, 1, 2
 
 ERRORS = {-1: "DVGR_E_DIMS (unsupported dimensions)", -2: "DVGR_E_NULL (null pointer)",
           -3: "DVGR_E_WORKSPACE (saved/workspace buffer too small)", -4: "DVGR_E_ALIGN (pointer not 16-byte aligned)",
-          -5: "DVGR_E_KIND (unknown tensor kind)",
+          -5: "DVGR_E_KIND (unknown tensor / element / reduction kind)",
           -6: "DVGR_E_ORDER (rounds 2-3; no longer returned: dvgr_comm_place puts the communication stream on a free pipe)"}
 
 
@@ -51,6 +54,20 @@ class Opts(C.Structure):
                 ("seed", C.c_uint64), ("probe_begin", C.c_void_p), ("probe_end", C.c_void_p),
                 ("layer_done_events", C.POINTER(C.c_void_p)), ("loss", C.POINTER(LossSpec)),
                 ("layer_done_cb", C.c_void_p), ("layer_done_user", C.c_void_p), ("comm", C.c_void_p), ("p1t", C.c_void_p), ("lo8", C.c_void_p)]
+
+
+class AttnView(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("sl", C.c_int64), ("sh", C.c_int64)]
+
+
+class AttnProblem(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "Lq", "Lk", "H", "Hk", "Dh", "elem")] + [("scale", C.c_float)] + \
+               [(n, AttnView) for n in ("q", "k", "v", "o")] + [("lens", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                                                                ("lse", C.c_void_p)]
+
+
+class AttnGrads(C.Structure):
+    _fields_ = [(n, AttnView) for n in ("g_o", "g_q", "g_k", "g_v")]
 
 
 LAYER_DONE_CB = C.CFUNCTYPE(None, C.c_int32, C.c_void_p)
@@ -126,6 +143,15 @@ SYMBOLS += [
     ("dvgr_dbg_launch_count", C.c_longlong, []),
     ("dvgr_dbg_xmap_tags", C.c_int, [C.c_int]),
     ("dvgr_dbg_plan_xcd_blocks", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+]
+
+# include/dvgr_attn.h
+SYMBOLS += [
+    ("dvgr_attn_check", C.c_int, [C.POINTER(AttnProblem)]),
+    ("dvgr_attn_forward_workspace_bytes", C.c_size_t, [C.POINTER(AttnProblem)]),
+    ("dvgr_attn_backward_workspace_bytes", C.c_size_t, [C.POINTER(AttnProblem)]),
+    ("dvgr_attn_forward", C.c_int, [C.POINTER(AttnProblem), C.c_void_p, C.c_size_t, C.c_void_p]),
+    ("dvgr_attn_backward", C.c_int, [C.POINTER(AttnProblem), C.POINTER(AttnGrads), C.c_void_p, C.c_size_t, C.c_void_p]),
 ]
 
 _lib = None
@@ -231,6 +257,56 @@ def check(code: int, what: str):
     if code < 0:
         raise RuntimeError(f"{what} failed: {ERRORS.get(code, code)}")
     raise RuntimeError(f"{what} failed: hipError_t {code}")
+
+
+_ELEMS = {}
+
+
+def elem_code(t, what: str) -> int:
+    """DVGR_ELEM_* of a tensor on a ROCm device; raises for anything else."""
+    if not _ELEMS:
+        import torch
+        _ELEMS.update({torch.float32: DVGR_ELEM_F32, torch.bfloat16: DVGR_ELEM_BF16, torch.float16: DVGR_ELEM_F16})
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs on a ROCm device only (no CPU fallback); got a tensor on {t.device}")
+    code = _ELEMS.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{what} takes fp32, bf16 and fp16 tensors; got {t.dtype}")
+    return code
+
+
+def on(t):
+    """Context in which launches go to the device of `t`, and the raw handle of its current stream there."""
+    import torch
+    dev = t.device
+    if dev.index == torch.cuda.current_device():
+        return _HERE_ALREADY, torch.cuda.current_stream(dev).cuda_stream
+    return torch.cuda.device(dev), torch.cuda.current_stream(dev).cuda_stream
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+_graphs = weakref.WeakKeyDictionary()         # living autograd node of this package -> (stream it was made on, ids of its leaves)
+
+
+def note_graph(ctx, stream, *inputs):
+    """Called in a forward: remembers, while the autograd node lives, which leaves it holds and on which stream it was made."""
+    leaves = tuple([id(t) for t in inputs if t.requires_grad and t.is_leaf])
+    if leaves:
+        _graphs[ctx] = (stream, leaves)
+
+
+def check_capture(ctx, what: str):
+    """Called in a backward: refuses to be captured while another graph of the same leaves, made on another stream, lives.  autograd
+    keeps one accumulation node for a leaf, on the stream where the first living graph made it; a captured backward that ends
+    there would draw that stream into the capture, which ends the process."""
+    import torch
+    mine = _graphs.get(ctx)
+    if mine is None or not torch.cuda.is_current_stream_capturing():
+        return
+    for other, (stream, leaves) in list(_graphs.items()):
+        if stream != mine[0] and not set(leaves).isdisjoint(mine[1]):
+            raise RuntimeError(f"{what}: this backward is being captured while a graph of the same leaves lives that was made on another "
+                               "stream: drop that graph's outputs (or detach them) before the capture")
 
 
 def make_dims(B, N, T, D, Wd, L, G=1, dtype=DVGR_F32) -> Dims:

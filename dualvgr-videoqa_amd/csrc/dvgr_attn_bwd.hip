@@ -1,0 +1,349 @@
+// dvgr_attn_bwd.hip -- include/dvgr_attn.h: attention to an encoder's states, backward.
+//
+//     P = exp2(c q.k - lse)      D = rowsum(dO o O)      dS = P o (dO V^T - D)
+//     dV = P^T dO      dK = scale dS^T Q      dQ = scale dS K
+//
+// Two passes over the scores, neither with atomics: one owns keys and goes over the packed rows (dK, dV; the heads of a group are rows
+// of the same reduction), one owns rows and goes over the keys (dQ).  The scores are computed in both: 7 products instead of 5, for
+// results that do not depend on the schedule.
+#include "dvgr_attn.h"
+
+namespace dvgr {
+namespace attn {
+namespace {
+
+// fp16 has 5 bits of exponent: the score gradients are scaled by the power of two that puts the largest |dO| of the sample's head
+// group into [0.5, 1), so that small upstream gradients do not vanish, and held inside the type's range.
+template <typename T> struct Grad16 { static constexpr bool on = false; };
+template <> struct Grad16<f16_t> { static constexpr bool on = true; };
+__device__ __forceinline__ float grad_scale(uint32_t top) {
+  const int e = (int)(top >> 23);                                   // bits of the largest |dO|
+  return e == 0 || e >= 255 ? 1.f : ldexpf(1.f, 126 - e);
+}
+
+struct BwdArgs {
+  Args f;
+  dvgr_attn_view g_o, g_q, g_k, g_v;
+  float* delta;                     // (B, H, Lq)
+  uint32_t* top;                    // (B, Hk): bits of the largest |dO| (fp16)
+};
+
+__global__ __launch_bounds__(256) void k_attn_clear(uint32_t* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0u;
+}
+
+// D of a packed row: 16 lanes per row
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
+  const Args& A = B.f;
+  const int lane = threadIdx.x & 15;
+  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (i >= (int64_t)A.a.B * A.a.Hk * A.rows) return;
+  const int row = (int)(i % A.rows), hk = (int)(i / A.rows % A.a.Hk), b = (int)(i / A.rows / A.a.Hk);
+  const T* o = (const T*)q_side(A, A.a.o, b, hk).row(row, A.G);
+  const T* g = (const T*)q_side(A, B.g_o, b, hk).row(row, A.G);
+  constexpr int N = Vec16<T>::N;
+  float s = 0.f, top = 0.f;
+  for (int d = lane * N; d < A.a.Dh; d += 16 * N) {
+    float x[N], y[N];
+    load_vec(o + d, x);
+    load_vec(g + d, y);
+#pragma unroll
+    for (int j = 0; j < N; ++j) { s += x[j] * y[j]; top = fmaxf(top, fabsf(y[j])); }
+  }
+#pragma unroll
+  for (int d = 8; d; d >>= 1) { s += __shfl_xor(s, d); top = fmaxf(top, __shfl_xor(top, d)); }
+  if (lane == 0) {
+    B.delta[row_index(A, b, hk, row)] = s;
+    if (Grad16<T>::on) atomicMax(&B.top[b * A.a.Hk + hk], __float_as_uint(top));
+  }
+}
+
+// score gradient as the matrix unit takes it
+template <typename T> __device__ __forceinline__ float grad16(float ds, float sc) {
+  return Grad16<T>::on ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
+}
+
+// ---- dK, dV: KW x 32 keys of one key head, RW x RS x 32 packed rows a turn -------------------------------------------------------
+template <typename T, int DP, int KW, int RW, int RS>
+__global__ __launch_bounds__(kThreads) void k_attn_dkv(BwdArgs B) {
+  const Args& A = B.f;
+  typedef Tile<T, DP> Tl;
+  constexpr int RT = RW * RS * 32, KT = KW * 32, NT = Tl::kNT;
+  extern __shared__ __align__(16) char lds[];
+  char* lq = lds;
+  char* lg = lq + Tl::template bytes<RT>();
+  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytes<RT>());       // [lse, D][RT]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
+  const int ktiles = (A.a.Lk + KT - 1) / KT;
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * ktiles);
+  if (w < 0) return;
+  const int kt = (int)(w % ktiles), hk = (int)(w / ktiles % A.a.Hk), b = (int)(w / ktiles / A.a.Hk);
+  const int n = key_count(A, b), dhb = A.a.Dh * A.es;
+  const int key = kt * KT + kw * 32 + (lane & 31);
+  const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)b * A.a.mask_stride : nullptr;
+  const bool there = key < n && (!mask || mask[key]);
+
+  Frag<T> kf[Tl::kSteps], vf[Tl::kSteps];
+  {
+    const char* kr = k_side(A, A.a.k, b, hk).row(there ? key : 0, 1);
+    const char* vr = k_side(A, A.a.v, b, hk).row(there ? key : 0, 1);
+#pragma unroll
+    for (int s = 0; s < Tl::kSteps; ++s) { kf[s] = Tl::gfrag(kr, s, lane, dhb, there); vf[s] = Tl::gfrag(vr, s, lane, dhb, there); }
+  }
+  f32x16 dk[NT], dv[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) dk[t] = dv[t] = zero16();
+  const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
+  const Side qs = q_side(A, A.a.q, b, hk), gs = q_side(A, B.g_o, b, hk);
+  const int rtiles = kt * KT < n ? (A.rows + RT - 1) / RT : 0;                   // keys behind the sample's: zeros
+
+  Stage<T, DP, RT> sq, sg;
+  float stat = 0.f;
+  const auto fetch = [&](int t) {
+    sq.fetch(qs, A.G, t * RT, A.rows, nullptr, dhb, tid);
+    sg.fetch(gs, A.G, t * RT, A.rows, nullptr, dhb, tid);
+    if (tid < 2 * RT) {
+      const int r = t * RT + tid % RT;
+      const int64_t at = r < A.rows ? row_index(A, b, hk, r) : 0;
+      stat = r < A.rows ? (tid < RT ? A.a.lse[at] : B.delta[at]) : (tid < RT ? INFINITY : 0.f);
+    }
+  };
+  if (rtiles) fetch(0);
+  for (int t = 0; t < rtiles; ++t) {
+    __syncthreads();
+    sq.put(lq, tid);
+    sg.put(lg, tid);
+    if (tid < 2 * RT) lstat[tid] = stat;
+    __syncthreads();
+    if (t + 1 < rtiles) fetch(t + 1);
+#pragma unroll 1
+    for (int i = 0; i < RS; ++i) {
+      const char* tq = lq + (rw * RS + i) * 32 * Tl::kStride;
+      const char* tg = lg + (rw * RS + i) * 32 * Tl::kStride;
+      f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
+#pragma unroll
+      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(tq, st, lane), kf[st], s);
+#pragma unroll
+      for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tg, st, lane), vf[st], dp);
+      const float* ls = lstat + (rw * RS + i) * 32 + (lane >> 5) * 4;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 e = *reinterpret_cast<const float4*>(ls + 8 * g), d = *reinterpret_cast<const float4*>(ls + RT + 8 * g);
+        const float ee[4] = {e.x, e.y, e.z, e.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g + j;
+          const float p = there ? exp2_fast(fmaf(s[r], A.c, -ee[j])) : 0.f;
+          s[r] = p;
+          dp[r] = there ? grad16<T>(p * (dp[r] - dd[j]), sc) : 0.f;
+        }
+      }
+      mma_tr<DP>(dv, tg, s, lane, T());
+      mma_tr<DP>(dk, tq, dp, lane, T());
+    }
+  }
+  if (RW > 1) {                                                     // add the waves that went over other rows, dK then dV
+    float* lo = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      f32x16* acc = x ? dv : dk;
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) lo[((wave * NT + t) * 16 + r) * 64 + lane] = acc[t][r];
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (t % RW != rw) continue;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float a = 0.f;
+#pragma unroll
+          for (int k = 0; k < RW; ++k) a += lo[(((kw * RW + k) * NT + t) * 16 + r) * 64 + lane];
+          acc[t][r] = a;
+        }
+      }
+    }
+  }
+  if (key >= A.a.Lk) return;
+  const float f = A.a.scale / sc;
+  char* gk = const_cast<char*>(k_side(A, B.g_k, b, hk).row(key, 1));
+  char* gv = const_cast<char*>(k_side(A, B.g_v, b, hk).row(key, 1));
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (RW > 1 && t % RW != rw) continue;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * t + 8 * g + (lane >> 5) * 4;
+      if (d >= A.a.Dh) continue;
+      store4<T>(gk + d * sizeof(T), dk[t][4 * g] * f, dk[t][4 * g + 1] * f, dk[t][4 * g + 2] * f, dk[t][4 * g + 3] * f);
+      store4<T>(gv + d * sizeof(T), dv[t][4 * g], dv[t][4 * g + 1], dv[t][4 * g + 2], dv[t][4 * g + 3]);
+    }
+  }
+}
+
+// ---- dQ: QW x 32 packed rows, KW x KS x 32 keys a turn (the forward's arrangement) -----------------------------------------------
+template <typename T, int DP, int QW, int KW, int KS>
+__global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
+  const Args& A = B.f;
+  typedef Tile<T, DP> Tl;
+  constexpr int KT = KW * KS * 32, RT = QW * 32, NT = Tl::kNT;
+  extern __shared__ __align__(16) char lds[];
+  char* lk = lds;
+  char* lv = lds + Tl::template bytes<KT>();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, qw = wave / KW, kw = wave % KW;
+  const int rtiles = (A.rows + RT - 1) / RT;
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles);
+  if (w < 0) return;
+  const int rt = (int)(w % rtiles), hk = (int)(w / rtiles % A.a.Hk), b = (int)(w / rtiles / A.a.Hk);
+  const int n = key_count(A, b), dhb = A.a.Dh * A.es, tn = (n + KT - 1) / KT;
+  const int row = rt * RT + qw * 32 + (lane & 31);
+  const bool live = row < A.rows;
+  const Side ks = k_side(A, A.a.k, b, hk), vs = k_side(A, A.a.v, b, hk);
+  const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)b * A.a.mask_stride : nullptr;
+
+  Frag<T> qf[Tl::kSteps], gf[Tl::kSteps];
+  {
+    const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0, A.G);
+    const char* gr = q_side(A, B.g_o, b, hk).row(live ? row : 0, A.G);
+#pragma unroll
+    for (int s = 0; s < Tl::kSteps; ++s) { qf[s] = Tl::gfrag(qr, s, lane, dhb, live); gf[s] = Tl::gfrag(gr, s, lane, dhb, live); }
+  }
+  const int64_t ri = row_index(A, b, hk, live ? row : 0);
+  const float lse = live ? A.a.lse[ri] : INFINITY, delta = live ? B.delta[ri] : 0.f;
+  const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
+  f32x16 dq[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) dq[t] = zero16();
+
+  Stage<T, DP, KT> sk, sv;
+  bool there = false;
+  const auto fetch = [&](int t) {
+    sk.fetch(ks, 1, t * KT, n, mask, dhb, tid);
+    sv.fetch(vs, 1, t * KT, n, mask, dhb, tid);
+    const int j = t * KT + kw * KS * 32 + lane;
+    there = lane < KS * 32 && j < n && (!mask || mask[j]);
+  };
+  if (tn) fetch(0);
+  for (int t = 0; t < tn; ++t) {
+    __syncthreads();
+    sk.put(lk, tid);
+    sv.put(lv, tid);
+    const unsigned long long bits = __ballot(there);
+    __syncthreads();
+    if (t + 1 < tn) fetch(t + 1);
+    if (!bits) continue;
+#pragma unroll 1
+    for (int i = 0; i < KS; ++i) {
+      const char* tk = lk + (kw * KS + i) * 32 * Tl::kStride;
+      const char* tv = lv + (kw * KS + i) * 32 * Tl::kStride;
+      f32x16 s = zero16(), dp = zero16();                             // rows = keys, column = this lane's packed row
+#pragma unroll
+      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(tk, st, lane), qf[st], s);
+#pragma unroll
+      for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tv, st, lane), gf[st], dp);
+      const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float ds = grad16<T>(exp2_fast(fmaf(s[r], A.c, -lse)) * (dp[r] - delta), sc);
+        s[r] = reg_bit(hb, r) ? ds : 0.f;
+      }
+      mma_tr<DP>(dq, tk, s, lane, T());
+    }
+  }
+  if (KW > 1) {
+    float* lo = reinterpret_cast<float*>(lds);
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) lo[((wave * NT + t) * 16 + r) * 64 + lane] = dq[t][r];
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (t % KW != kw) continue;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) a += lo[(((qw * KW + k) * NT + t) * 16 + r) * 64 + lane];
+        dq[t][r] = a;
+      }
+    }
+  }
+  if (!live) return;
+  const float f = A.a.scale / sc;
+  char* out = const_cast<char*>(q_side(A, B.g_q, b, hk).row(row, A.G));
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (KW > 1 && t % KW != kw) continue;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * t + 8 * g + (lane >> 5) * 4;
+      if (d < A.a.Dh) store4<T>(out + d * sizeof(T), dq[t][4 * g] * f, dq[t][4 * g + 1] * f, dq[t][4 * g + 2] * f, dq[t][4 * g + 3] * f);
+    }
+  }
+}
+
+size_t delta_bytes(const dvgr_attn_problem& a) { return ((size_t)a.B * a.H * a.Lq * sizeof(float) + 255) / 256 * 256; }
+
+template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t work, size_t bytes, const BwdArgs& B, hipStream_t st) {
+  const int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
+  if (e) return e;
+  DVGR_LAUNCH(kern, dim3(xcd_grid(work)), dim3(kThreads), bytes, st, B);
+  return (int)hipGetLastError();
+}
+size_t join_bytes(int waves, int NT) { return waves > 1 ? (size_t)kWaves * NT * 16 * 64 * sizeof(float) : 0; }
+
+template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdArgs& B, hipStream_t st) {
+  typedef Tile<T, DP> Tl;
+  static std::atomic<uint32_t> asked{0};
+  size_t bytes = 2 * Tl::template bytes<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float);
+  if (bytes < join_bytes(RW, Tl::kNT)) bytes = join_bytes(RW, Tl::kNT);
+  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), bytes, B, st);
+}
+template <typename T, int DP, int QW, int KW, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
+  typedef Tile<T, DP> Tl;
+  static std::atomic<uint32_t> asked{0};
+  size_t bytes = 2 * Tl::template bytes<KW * KS * 32>();
+  if (bytes < join_bytes(KW, Tl::kNT)) bytes = join_bytes(KW, Tl::kNT);
+  return launch(k_attn_dq<T, DP, QW, KW, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.rows + QW * 32 - 1) / (QW * 32)), bytes, B, st);
+}
+
+// Few keys (or few rows): the four waves share them and go over different rows (keys).
+template <typename T, int DP> int launch_dp(const BwdArgs& B, hipStream_t st) {
+  constexpr int S = sizeof(T) == 4 ? 1 : 2;                         // a turn of the shared arrangement: 32 rows of fp32, 64 of two bytes
+  if (B.f.a.Lk && B.g_k.p) {
+    const int e = B.f.a.Lk <= 32 ? launch_dkv<T, DP, 1, 4, 1>(B, st) : launch_dkv<T, DP, 4, 1, S>(B, st);
+    if (e) return e;
+  }
+  if (!B.f.rows || !B.g_q.p) return 0;
+  return B.f.rows <= 32 ? launch_dq<T, DP, 1, 4, 1>(B, st) : launch_dq<T, DP, 4, 1, S>(B, st);
+}
+
+template <typename T> int launch_t(const BwdArgs& B, hipStream_t st) {
+  const int64_t rows = (int64_t)B.f.a.B * B.f.a.Hk * B.f.rows, groups = (int64_t)B.f.a.B * B.f.a.Hk;
+  if (Grad16<T>::on) DVGR_LAUNCH(k_attn_clear, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, B.top, groups);
+  if (rows) DVGR_LAUNCH((k_attn_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, B);
+  const int e = (int)hipGetLastError();
+  if (e) return e;
+  if (B.f.a.Dh <= 32) return launch_dp<T, 32>(B, st);
+  if (B.f.a.Dh <= 64) return launch_dp<T, 64>(B, st);
+  if (B.f.a.Dh <= 96) return launch_dp<T, 96>(B, st);
+  return launch_dp<T, 128>(B, st);
+}
+
+}  // namespace
+
+size_t backward_bytes(const dvgr_attn_problem& a) { return delta_bytes(a) + (a.elem == DVGR_ELEM_F16 ? (size_t)a.B * a.Hk * sizeof(uint32_t) : 0); }
+
+int launch_backward(const Args& A, const dvgr_attn_grads& g, void* ws, hipStream_t st) {
+  BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, (float*)ws, (uint32_t*)((char*)ws + delta_bytes(A.a))};
+  return A.a.elem == DVGR_ELEM_F32 ? launch_t<float>(B, st) : A.a.elem == DVGR_ELEM_BF16 ? launch_t<bf16_t>(B, st) : launch_t<f16_t>(B, st);
+}
+
+}  // namespace attn
+}  // namespace dvgr

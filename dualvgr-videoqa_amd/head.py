@@ -48,6 +48,11 @@ HEAD_SYMBOLS = [
                                      C.c_size_t, C.c_void_p, C.c_size_t, C.c_int, C.c_uint64, C.c_void_p]),
     ("dvgr_head_cross_entropy", C.c_int, [C.POINTER(HeadDims), C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p,
                                           C.c_void_p, C.c_void_p]),
+    ("dvgr_distill_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int64]),
+    ("dvgr_distill_forward", C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                       C.c_float, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    ("dvgr_distill_backward", C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                        C.c_float, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
     ("dvgr_head_dbg_keep_mask", C.c_int, [C.c_uint64, C.c_int, C.c_int64, C.c_void_p, C.c_void_p]),
 ]
 _bound = False

@@ -1,19 +1,22 @@
-"""Host side of include/dvgr_inputs.h: the two input-side operators of the reference model
+"""Host side of include/dvgr_inputs.h: the input-side operators
 that are neither an LSTM nor the unit --
 
   * `word_features(table, questions, train)`: tanh(dropout_0.15(embedding(questions))) of
     InputUnitLinguisticDynamic.forward (model/Preprocessing.py:112-113) as one gather kernel, and its backward as one
     scatter-add kernel into the embedding table's gradient;
+  * `embed_tokens(table, tokens, scale, padding_idx)` / `TokenEmbedding`: scale * table[tokens] for fp32, bf16 and fp16 tables of
+    any width, with a gradient that sorts the tokens instead of adding atomically: the same inputs give the same bits;
   * `HipLinear`: DualVGR.visual_motion_input_unit = nn.Linear(vision_dim, module_dim) (model/models.py:46, :74) on the
     unit's contraction engine.  A subclass of nn.Linear: same parameters, state_dict keys and default init.
 
-No CPU fallback: both raise off a ROCm device."""
+No CPU fallback: all raise off a ROCm device."""
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
 
@@ -23,6 +26,11 @@ INPUT_SYMBOLS = [
     ("dvgr_words_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_uint64,
                                       C.c_void_p, C.c_void_p]),
     ("dvgr_words_dbg_keep_mask", C.c_int, [C.c_uint64, C.c_int64, C.c_void_p, C.c_void_p]),
+    ("dvgr_embed_forward", C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_float, C.c_void_p,
+                                     C.c_void_p, C.c_void_p]),
+    ("dvgr_embed_workspace_bytes", C.c_size_t, [C.c_int64, C.c_int64, C.c_int, C.c_int]),
+    ("dvgr_embed_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_int64,
+                                      C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     ("dvgr_linear_forward", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int,
                                       C.c_void_p]),
     ("dvgr_linear_backward", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
@@ -113,6 +121,95 @@ def words_keep_mask(seed: int, shape, device) -> torch.Tensor:
     L_.check(lib.dvgr_words_dbg_keep_mask(int(seed), n, keep.data_ptr(), torch.cuda.current_stream(device).cuda_stream),
              "dvgr_words_dbg_keep_mask")
     return keep.view(*shape)
+
+
+def _embed_forward(table, tokens, elem, scale, bad):
+    lib = load()
+    vocab, wd = table.shape
+    y = torch.empty(*tokens.shape, wd, device=table.device, dtype=table.dtype)
+    here, stream = L_.on(table)
+    with here:
+        L_.check(lib.dvgr_embed_forward(table.data_ptr(), vocab, wd, elem, tokens.data_ptr(), tokens.numel(), scale, y.data_ptr(),
+                                        bad.data_ptr() if bad is not None else None, stream), "dvgr_embed_forward")
+    return y
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, elem, scale, padding, bad):
+        ctx.save_for_backward(tokens)
+        ctx.meta = (table.shape, elem, scale, padding)
+        L_.note_graph(ctx, torch.cuda.current_stream(table.device).cuda_stream, table)
+        return _embed_forward(table.contiguous(), tokens, elem, scale, bad)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        lib = load()
+        L_.check_capture(ctx, "embed_tokens")
+        tokens, = ctx.saved_tensors
+        (vocab, wd), elem, scale, padding = ctx.meta
+        n = tokens.numel()
+        g = g.contiguous()
+        g_table = torch.empty(vocab, wd, device=g.device, dtype=g.dtype)
+        nbytes = lib.dvgr_embed_workspace_bytes(n, vocab, wd, elem)
+        ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
+        here, stream = L_.on(g)
+        with here:
+            L_.check(lib.dvgr_embed_backward(g.data_ptr(), tokens.data_ptr(), n, vocab, wd, elem, scale, padding, g_table.data_ptr(),
+                                             ws.data_ptr(), nbytes, stream), "dvgr_embed_backward")
+        return g_table, None, None, None, None, None
+
+
+def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, padding_idx: int = None,
+                 bad: torch.Tensor = None) -> torch.Tensor:
+    """scale * table[tokens]: `table` (vocab, wd) in fp32, bf16 or fp16, `tokens` integers of any shape -> (*tokens.shape, wd).
+
+    The product is rounded once.  The gradient of the table is dense: the rows of a token are added in fp32 in an order that the
+    tokens alone decide (they are sorted; no atomics) and rounded once; `padding_idx` (negative: from the end, as in
+    torch.nn.Embedding) gets none.  A token outside the table gives a row of zeros, no gradient, and sets `bad` (one int32 on
+    the device) to 1 if it is given."""
+    elem = L_.elem_code(table, "embed_tokens")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise RuntimeError(f"embed_tokens: the table is (vocab, wd), not empty; got {tuple(table.shape)}")
+    if tokens.dtype != torch.int64:
+        if tokens.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+            raise RuntimeError(f"embed_tokens: tokens are integers; got {tokens.dtype}")
+        tokens = tokens.long()
+    if tokens.device != table.device:
+        raise RuntimeError(f"embed_tokens: the tokens are on {tokens.device}, the table is on {table.device}")
+    if bad is not None and (bad.dtype != torch.int32 or bad.numel() != 1 or bad.device != table.device):
+        raise RuntimeError("embed_tokens: `bad` is one int32 on the table's device")
+    padding = -1
+    if padding_idx is not None:
+        padding = int(padding_idx) + (table.shape[0] if padding_idx < 0 else 0)
+        if not 0 <= padding < table.shape[0]:
+            raise RuntimeError(f"embed_tokens: padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
+    tokens = tokens.contiguous()
+    if table.requires_grad and torch.is_grad_enabled():
+        return _Embed.apply(table, tokens, elem, float(scale), padding, bad)
+    return _embed_forward(table.contiguous(), tokens, elem, float(scale), bad)
+
+
+class TokenEmbedding(nn.Embedding):
+    """nn.Embedding(num_embeddings, embedding_dim, padding_idx) on `embed_tokens`: same parameter, state_dict key and default init;
+    rows are multiplied by `scale` (sqrt(embedding_dim) in many language models)."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale: float = 1.0):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx)
+        self.scale = float(scale)
+        self._bad = None
+
+    def forward(self, tokens):
+        if self._bad is None or self._bad.device != self.weight.device:
+            self._bad = torch.zeros(1, device=self.weight.device, dtype=torch.int32)
+        return embed_tokens(self.weight, tokens, self.scale, self.padding_idx, self._bad)
+
+    def check_tokens(self):
+        """Synchronises: raises if any call so far met a token outside the table (torch raises at the lookup itself)."""
+        if self._bad is not None and int(self._bad.item()) != 0:
+            self._bad.zero_()
+            raise IndexError("TokenEmbedding: a token is outside the embedding table")
 
 
 class _Linear(torch.autograd.Function):

@@ -37,11 +37,17 @@ extern "C" {
 #define DVGR_BF16X3 2 /* every fp32 operand split as hi + lo bf16; 3 bf16 MFMAs per product (hi.hi + hi.lo +
                          lo.hi), fp32 accumulate: fp32-grade results (~1e-5 relative) at 3/16 the MFMA cost */
 
+/* Element type of the tensors of the operators that take more than fp32 (dvgr_embed_*, dvgr_distill_*, dvgr_attn_*).  Arithmetic,
+ * softmax statistics and sums are fp32 for all three; a result is rounded to its tensor's type where it is stored. */
+#define DVGR_ELEM_F32 0
+#define DVGR_ELEM_BF16 1
+#define DVGR_ELEM_F16 2
+
 #define DVGR_E_DIMS (-1)      /* unsupported dimension (see dvgr_check_dims)            */
 #define DVGR_E_NULL (-2)      /* a required pointer is NULL                             */
 #define DVGR_E_WORKSPACE (-3) /* saved/workspace buffer too small                       */
 #define DVGR_E_ALIGN (-4)     /* a pointer is not 16-byte aligned                       */
-#define DVGR_E_KIND (-5)      /* unknown parameter / saved-tensor kind                  */
+#define DVGR_E_KIND (-5)      /* unknown parameter / saved-tensor / element / reduction kind */
 #define DVGR_E_ORDER (-6)     /* (rounds 2-3: communicator created after the unit ran; no longer returned -- dvgr_comm_place) */
 
 /* Problem dimensions.  Mirrors the constructor arguments of DualVGRUnit_multiple

@@ -79,6 +79,32 @@ int dvgr_head_backward(const dvgr_head_dims *d, const float *params, const dvgr_
 int dvgr_head_cross_entropy(const dvgr_head_dims *d, int C_valid, const float *logits, const int64_t *target, float scale,
                             float *loss, float *g_logits, void *stream);
 
+/* ---- distillation from a teacher's top logits ------------------------------------------------------------------------------
+ * Per row r of R (R < 2^22): p = softmax over the K entries of values / temperature, q = softmax over the C classes of
+ * logits / temperature,
+ *     loss_r = temperature^2 * sum_k p_k (log p_k - log q[indices_k]).
+ * logits: (R, C) of `elem` (DVGR_ELEM_*), rows `ld` elements apart; values: (R, K) of `elem_values`, indices: (R, K) int64, both
+ * contiguous; 1 <= K <= DVGR_DISTILL_MAX_K.  An entry whose index lies outside [0, C) is not there (lists of differing length);
+ * an entry of value -inf has p = 0; entries of the same class add up.  A row without entries has loss 0 and gradient 0.
+ * loss_rows: (R) fp32.  total: one float, the sum of the rows (DVGR_DISTILL_SUM) or the mean over the rows that have an entry, 0 if
+ * none has (DVGR_DISTILL_MEAN); unused for DVGR_DISTILL_NONE (nullable).
+ * stats: (R + 1, 4) fp32, 16-byte aligned, filled for the backward.  1e-6 <= temperature <= 1e6. */
+#define DVGR_DISTILL_MAX_K 1024
+#define DVGR_DISTILL_NONE 0
+#define DVGR_DISTILL_SUM 1
+#define DVGR_DISTILL_MEAN 2
+size_t dvgr_distill_workspace_bytes(int64_t R, int64_t C);
+int dvgr_distill_forward(const void *logits, int64_t ld, int elem, int64_t R, int64_t C, const void *values, int elem_values,
+                         const int64_t *indices, int K, float temperature, int reduction, float *loss_rows, float *total,
+                         float *stats, void *workspace, size_t workspace_bytes, void *stream);
+
+/* g_logits[r][j] = g_r * temperature * (q_j - sum over entries of class j of p), every one of the R x C elements written.
+ * g_loss_stride 1 (DVGR_DISTILL_NONE): g_r = g_loss[r]; 0: g_r = g_loss[0], divided by the mean's number of rows.  The lists, logits and
+ * `stats` are those of the forward. */
+int dvgr_distill_backward(const void *logits, int64_t ld, int elem, int64_t R, int64_t C, const void *values, int elem_values,
+                          const int64_t *indices, int K, float temperature, const float *stats, const float *g_loss,
+                          int g_loss_stride, void *g_logits, int64_t ld_g, void *stream);
+
 /* test hook: element keep-mask (1 / 0) of dropout site 0 (read-out input), 1 (concatenation), 2 (after BatchNorm) */
 int dvgr_head_dbg_keep_mask(uint64_t seed, int site, int64_t n, float *keep, void *stream);
 

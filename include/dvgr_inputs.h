@@ -34,6 +34,22 @@ int dvgr_words_backward(const float *g_words, const float *words, const int64_t 
 /* Test aid: the 0/1 keep flags of the dropout site for `seed`, n * wd of them in element order. */
 int dvgr_words_dbg_keep_mask(uint64_t seed, int64_t count, float *keep, void *stream);
 
+/* ---- token embedding with scaling, and its gradient by sorted tokens -------------------------------------------------------
+ * Tensors of `elem` (DVGR_ELEM_*), rows of `wd` >= 1 elements, contiguous; any alignment of the element (16-byte aligned rows take
+ * the vector path).  n < 2^26 positions, vocab < 2^31 - 1.
+ *
+ * y[i][:] = scale * table[tokens[i]][:].  A token outside [0, vocab) gives a row of zeros and sets *bad_tokens (int32, device,
+ * nullable) to 1. */
+int dvgr_embed_forward(const void *table, int64_t vocab, int wd, int elem, const int64_t *tokens, int64_t n, float scale, void *y,
+                       int32_t *bad_tokens, void *stream);
+
+/* g_table[v][:] = scale * sum over i with tokens[i] == v of g_y[i][:], added in fp32 in an order that the tokens alone decide and
+ * rounded once: the same inputs give the same bits.  Every row of g_table is written; tokens outside the table and the token
+ * `padding_idx` (-1: none) add nothing.  `workspace` (16-byte aligned): dvgr_embed_workspace_bytes, overwritten. */
+size_t dvgr_embed_workspace_bytes(int64_t n, int64_t vocab, int wd, int elem);
+int dvgr_embed_backward(const void *g_y, const int64_t *tokens, int64_t n, int64_t vocab, int wd, int elem, float scale,
+                        int64_t padding_idx, void *g_table, void *workspace, size_t workspace_bytes, void *stream);
+
 /* y (M x N) = x (M x K) . w^T (w: N x K) + b (N, nullable).  dtype: DVGR_F32 (exact fp32 MFMA) / DVGR_BF16X3 / DVGR_BF16 as
  * in dvgr_dims.dtype; K % 4 == 0, N % 4 == 0. */
 int dvgr_linear_forward(const float *x, const float *w, const float *b, float *y, int M, int N, int K, int dtype,
