@@ -5,16 +5,13 @@ product entry point that needs it.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
-import weakref
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DVGR_LIB") or os.path.join(_HERE, "libdvgr_hip.so")   # DVGR_LIB: debug builds only
 
 DVGR_F32, DVGR_BF16, DVGR_BF16X3 = 0, 1, 2
-DVGR_ELEM_F32, DVGR_ELEM_BF16, DVGR_ELEM_F16 = 0, 1, 2
 
 # enum dvgr_param_kind
 (P_QA_W1, P_QA_B1, P_QA_W2, P_QA_B2, P_WQ, P_BQ, P_GAT_W, P_GAT_B, P_GAT_A, P_GAT_C,
@@ -62,7 +59,7 @@ class AttnView(C.Structure):
 
 class AttnProblem(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "Lq", "Lk", "H", "Hk", "Dh", "elem")] + [("scale", C.c_float)] + \
-               [(n, AttnView) for n in ("q", "k", "v", "o")] + [("lens", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+               [(n, AttnView) for n in ("q", "k", "v", "o")] + [("o_lo", C.c_void_p), ("lens", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
                                                                 ("lse", C.c_void_p)]
 
 
@@ -259,54 +256,32 @@ def check(code: int, what: str):
     raise RuntimeError(f"{what} failed: hipError_t {code}")
 
 
-_ELEMS = {}
+_torch_ops = None
+TORCH_PATH = os.path.join(_HERE, "_dvgr_torch.so")
 
 
-def elem_code(t, what: str) -> int:
-    """DVGR_ELEM_* of a tensor on a ROCm device; raises for anything else."""
-    if not _ELEMS:
-        import torch
-        _ELEMS.update({torch.float32: DVGR_ELEM_F32, torch.bfloat16: DVGR_ELEM_BF16, torch.float16: DVGR_ELEM_F16})
-    if not t.is_cuda:
-        raise RuntimeError(f"{what} runs on a ROCm device only (no CPU fallback); got a tensor on {t.device}")
-    code = _ELEMS.get(t.dtype)
-    if code is None:
-        raise RuntimeError(f"{what} takes fp32, bf16 and fp16 tensors; got {t.dtype}")
-    return code
+def torch_ops():
+    """The autograd nodes of the question-side operators (csrc/dvgr_torch.cpp), bound to the library's entry points (once)."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.machinery
+        import importlib.util
 
+        import torch  # noqa: F401   (its libraries have to be loaded first)
 
-def on(t):
-    """Context in which launches go to the device of `t`, and the raw handle of its current stream there."""
-    import torch
-    dev = t.device
-    if dev.index == torch.cuda.current_device():
-        return _HERE_ALREADY, torch.cuda.current_stream(dev).cuda_stream
-    return torch.cuda.device(dev), torch.cuda.current_stream(dev).cuda_stream
-
-
-_HERE_ALREADY = contextlib.nullcontext()
-_graphs = weakref.WeakKeyDictionary()         # living autograd node of this package -> (stream it was made on, ids of its leaves)
-
-
-def note_graph(ctx, stream, *inputs):
-    """Called in a forward: remembers, while the autograd node lives, which leaves it holds and on which stream it was made."""
-    leaves = tuple([id(t) for t in inputs if t.requires_grad and t.is_leaf])
-    if leaves:
-        _graphs[ctx] = (stream, leaves)
-
-
-def check_capture(ctx, what: str):
-    """Called in a backward: refuses to be captured while another graph of the same leaves, made on another stream, lives.  autograd
-    keeps one accumulation node for a leaf, on the stream where the first living graph made it; a captured backward that ends
-    there would draw that stream into the capture, which ends the process."""
-    import torch
-    mine = _graphs.get(ctx)
-    if mine is None or not torch.cuda.is_current_stream_capturing():
-        return
-    for other, (stream, leaves) in list(_graphs.items()):
-        if stream != mine[0] and not set(leaves).isdisjoint(mine[1]):
-            raise RuntimeError(f"{what}: this backward is being captured while a graph of the same leaves lives that was made on another "
-                               "stream: drop that graph's outputs (or detach them) before the capture")
+        from . import head, inputs
+        lib = load()
+        head.load(), inputs.load()
+        if not os.path.exists(TORCH_PATH):
+            raise RuntimeError(f"{TORCH_PATH} is missing: build it first (make -C dualvgr-videoqa_amd/csrc).  There is no fallback.")
+        spec = importlib.util.spec_from_loader("_dvgr_torch", importlib.machinery.ExtensionFileLoader("_dvgr_torch", TORCH_PATH))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        names = [n for table in (SYMBOLS, head.HEAD_SYMBOLS, inputs.INPUT_SYMBOLS) for n, _, _ in table
+                 if n.startswith(("dvgr_embed_", "dvgr_distill_", "dvgr_attn_"))]
+        mod.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names})
+        _torch_ops = mod
+    return _torch_ops
 
 
 def make_dims(B, N, T, D, Wd, L, G=1, dtype=DVGR_F32) -> Dims:

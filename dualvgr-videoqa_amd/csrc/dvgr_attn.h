@@ -186,6 +186,13 @@ __device__ __forceinline__ int64_t row_index(const Args& A, int b, int hk, int r
   return ((int64_t)b * A.a.H + hk * A.G + (r - l * A.G)) * A.a.Lq + l;
 }
 
+// row of what the output's rounding left (B, Lq, H, Dh), or nullptr
+template <typename T> __device__ __forceinline__ char* lo_row(const Args& A, int b, int hk, int r) {
+  if (sizeof(T) == 4 || !A.a.o_lo) return nullptr;
+  const int l = A.G == 1 ? r : r / A.G;
+  return (char*)A.a.o_lo + (((int64_t)b * A.a.Lq + l) * A.a.H + hk * A.G + (r - l * A.G)) * A.a.Dh * (int64_t)sizeof(T);
+}
+
 // More than 64 KB of LDS has to be asked for once on a device (`asked`: a bit for each).
 inline int allow_lds(const void* kern, size_t bytes, std::atomic<uint32_t>& asked) {
   if (bytes <= 65536) return 0;

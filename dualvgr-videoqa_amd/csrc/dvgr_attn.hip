@@ -152,13 +152,17 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Args A) {
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   char* out = const_cast<char*>(q_side(A, A.a.o, b, hk).row(row, A.G));
+  char* lo = lo_row<T>(A, b, hk, row);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (KW > 1 && t % KW != kw) continue;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * t + 8 * g + h4;
-      if (d < A.a.Dh) store4<T>(out + d * sizeof(T), o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
+      if (d >= A.a.Dh) continue;
+      const float x[4] = {o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv};
+      store4<T>(out + d * sizeof(T), x[0], x[1], x[2], x[3]);
+      if (lo) store4<T>(lo + d * sizeof(T), x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
     }
   }
   // log2 of the row's sum, in units of the scaled scores; +inf for a row without keys: every exp2(s - lse) of the backward is 0
@@ -194,7 +198,12 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A, int RT) {
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* out = (T*)q_side(A, A.a.o, b, hk).row(row, A.G);
-  if (d < A.a.Dh) { out[d] = (T)(o.x * inv); out[d + 1] = (T)(o.y * inv); }
+  T* lo = (T*)lo_row<T>(A, b, hk, row);
+  if (d < A.a.Dh) {
+    o.x *= inv; o.y *= inv;
+    out[d] = (T)o.x; out[d + 1] = (T)o.y;
+    if (lo) { lo[d] = (T)(o.x - (float)(T)o.x); lo[d + 1] = (T)(o.y - (float)(T)o.y); }
+  }
   if (A.a.lse && lane == 0) A.a.lse[row_index(A, b, hk, row)] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
@@ -274,6 +283,7 @@ int check_forward_views(const dvgr_attn_problem& a) {
   if (empty(a)) return 0;
   if (!a.q.p || !a.o.p || (a.Lk && (!a.k.p || !a.v.p))) return DVGR_E_NULL;
   if (!view_ok(a.q, es, a.B, a.Lq, a.H) || !view_ok(a.o, es, a.B, a.Lq, a.H)) return DVGR_E_ALIGN;
+  if (!ptr16(a.o_lo)) return DVGR_E_ALIGN;
   if (a.Lk && (!view_ok(a.k, es, a.B, a.Lk, a.Hk) || !view_ok(a.v, es, a.B, a.Lk, a.Hk))) return DVGR_E_ALIGN;
   return 0;
 }

@@ -43,6 +43,7 @@ __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
   const int row = (int)(i % A.rows), hk = (int)(i / A.rows % A.a.Hk), b = (int)(i / A.rows / A.a.Hk);
   const T* o = (const T*)q_side(A, A.a.o, b, hk).row(row, A.G);
   const T* g = (const T*)q_side(A, B.g_o, b, hk).row(row, A.G);
+  const T* lo = (const T*)lo_row<T>(A, b, hk, row);
   constexpr int N = Vec16<T>::N;
   float s = 0.f, top = 0.f;
   for (int d = lane * N; d < A.a.Dh; d += 16 * N) {
@@ -51,6 +52,11 @@ __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
     load_vec(g + d, y);
 #pragma unroll
     for (int j = 0; j < N; ++j) { s += x[j] * y[j]; top = fmaxf(top, fabsf(y[j])); }
+    if (lo) {
+      load_vec(lo + d, x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += x[j] * y[j];
+    }
   }
 #pragma unroll
   for (int d = 8; d; d >>= 1) { s += __shfl_xor(s, d); top = fmaxf(top, __shfl_xor(top, d)); }

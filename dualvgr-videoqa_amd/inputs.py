@@ -16,7 +16,6 @@ import ctypes as C
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
 
@@ -123,44 +122,6 @@ def words_keep_mask(seed: int, shape, device) -> torch.Tensor:
     return keep.view(*shape)
 
 
-def _embed_forward(table, tokens, elem, scale, bad):
-    lib = load()
-    vocab, wd = table.shape
-    y = torch.empty(*tokens.shape, wd, device=table.device, dtype=table.dtype)
-    here, stream = L_.on(table)
-    with here:
-        L_.check(lib.dvgr_embed_forward(table.data_ptr(), vocab, wd, elem, tokens.data_ptr(), tokens.numel(), scale, y.data_ptr(),
-                                        bad.data_ptr() if bad is not None else None, stream), "dvgr_embed_forward")
-    return y
-
-
-class _Embed(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, tokens, elem, scale, padding, bad):
-        ctx.save_for_backward(tokens)
-        ctx.meta = (table.shape, elem, scale, padding)
-        L_.note_graph(ctx, torch.cuda.current_stream(table.device).cuda_stream, table)
-        return _embed_forward(table.contiguous(), tokens, elem, scale, bad)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        lib = load()
-        L_.check_capture(ctx, "embed_tokens")
-        tokens, = ctx.saved_tensors
-        (vocab, wd), elem, scale, padding = ctx.meta
-        n = tokens.numel()
-        g = g.contiguous()
-        g_table = torch.empty(vocab, wd, device=g.device, dtype=g.dtype)
-        nbytes = lib.dvgr_embed_workspace_bytes(n, vocab, wd, elem)
-        ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8)
-        here, stream = L_.on(g)
-        with here:
-            L_.check(lib.dvgr_embed_backward(g.data_ptr(), tokens.data_ptr(), n, vocab, wd, elem, scale, padding, g_table.data_ptr(),
-                                             ws.data_ptr(), nbytes, stream), "dvgr_embed_backward")
-        return g_table, None, None, None, None, None
-
-
 def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, padding_idx: int = None,
                  bad: torch.Tensor = None) -> torch.Tensor:
     """scale * table[tokens]: `table` (vocab, wd) in fp32, bf16 or fp16, `tokens` integers of any shape -> (*tokens.shape, wd).
@@ -169,26 +130,7 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, 
     tokens alone decide (they are sorted; no atomics) and rounded once; `padding_idx` (negative: from the end, as in
     torch.nn.Embedding) gets none.  A token outside the table gives a row of zeros, no gradient, and sets `bad` (one int32 on
     the device) to 1 if it is given."""
-    elem = L_.elem_code(table, "embed_tokens")
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise RuntimeError(f"embed_tokens: the table is (vocab, wd), not empty; got {tuple(table.shape)}")
-    if tokens.dtype != torch.int64:
-        if tokens.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
-            raise RuntimeError(f"embed_tokens: tokens are integers; got {tokens.dtype}")
-        tokens = tokens.long()
-    if tokens.device != table.device:
-        raise RuntimeError(f"embed_tokens: the tokens are on {tokens.device}, the table is on {table.device}")
-    if bad is not None and (bad.dtype != torch.int32 or bad.numel() != 1 or bad.device != table.device):
-        raise RuntimeError("embed_tokens: `bad` is one int32 on the table's device")
-    padding = -1
-    if padding_idx is not None:
-        padding = int(padding_idx) + (table.shape[0] if padding_idx < 0 else 0)
-        if not 0 <= padding < table.shape[0]:
-            raise RuntimeError(f"embed_tokens: padding_idx {padding_idx} is outside a table of {table.shape[0]} rows")
-    tokens = tokens.contiguous()
-    if table.requires_grad and torch.is_grad_enabled():
-        return _Embed.apply(table, tokens, elem, float(scale), padding, bad)
-    return _embed_forward(table.contiguous(), tokens, elem, float(scale), bad)
+    return L_.torch_ops().embed_tokens(table, tokens, scale, padding_idx, bad)
 
 
 class TokenEmbedding(nn.Embedding):

@@ -14,10 +14,8 @@ import ctypes as C
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
-from . import head as H_
 
 
 def common_loss(emb1: torch.Tensor, emb2: torch.Tensor) -> torch.Tensor:
@@ -109,52 +107,6 @@ REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}            # DVGR_DISTILL_*
 DISTILL_MAX_K = 1024
 
 
-def _distill_forward(logits, values, indices, temperature, reduction):
-    lib = H_.load()
-    R, Cn = logits.shape
-    dev = logits.device
-    rows = torch.empty(R, device=dev, dtype=torch.float32)
-    total = torch.empty((), device=dev, dtype=torch.float32)
-    stats = torch.empty(R + 1, 4, device=dev, dtype=torch.float32)
-    nbytes = lib.dvgr_distill_workspace_bytes(R, Cn)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    here, stream = L_.on(logits)
-    with here:
-        L_.check(lib.dvgr_distill_forward(logits.data_ptr(), logits.stride(0), L_.elem_code(logits, "distillation_loss"), R, Cn, values.data_ptr(),
-                                          L_.elem_code(values, "distillation_loss"), indices.data_ptr(), values.shape[1], temperature, reduction,
-                                          rows.data_ptr(), total.data_ptr(), stats.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
-                                          stream), "dvgr_distill_forward")
-    return rows, total, stats
-
-
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, values, indices, temperature, reduction):
-        rows, total, stats = _distill_forward(logits, values, indices, temperature, reduction)
-        ctx.save_for_backward(logits, values, indices, stats)
-        ctx.meta = (temperature, reduction)
-        L_.note_graph(ctx, torch.cuda.current_stream(logits.device).cuda_stream, logits)
-        return rows if reduction == 0 else total
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        lib = H_.load()
-        L_.check_capture(ctx, "distillation_loss")
-        logits, values, indices, stats = ctx.saved_tensors
-        temperature, reduction = ctx.meta
-        R, Cn = logits.shape
-        g = g.contiguous()
-        g_logits = torch.empty(R, Cn, device=logits.device, dtype=logits.dtype)
-        here, stream = L_.on(logits)
-        with here:
-            L_.check(lib.dvgr_distill_backward(logits.data_ptr(), logits.stride(0), L_.elem_code(logits, "distillation_loss"), R, Cn,
-                                               values.data_ptr(), L_.elem_code(values, "distillation_loss"), indices.data_ptr(), values.shape[1],
-                                               temperature, stats.data_ptr(), g.data_ptr(),
-                                               0 if reduction else 1, g_logits.data_ptr(), Cn, stream), "dvgr_distill_backward")
-        return g_logits, None, None, None, None
-
-
 def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, temperature: float = 1.0,
                       reduction: str = "mean") -> torch.Tensor:
     """T^2 sum_k p_k (log p_k - log q[indices_k]) per row: q = softmax(logits / T) over all classes, p = softmax(values / T) over the
@@ -165,8 +117,6 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     entries of the same class add up.  A row without entries has loss 0 and gradient 0.  reduction: "mean" over the rows that
     have an entry (0 if none has), "sum", or "none" (the rows, shaped logits.shape[:-1]).  The loss is fp32, the gradient has the
     logits' type; 1e-6 <= temperature <= 1e6."""
-    L_.elem_code(logits, "distillation_loss")
-    L_.elem_code(values, "distillation_loss")
     code = REDUCTIONS.get(reduction)
     if code is None:
         raise RuntimeError(f"distillation_loss: reduction is one of {sorted(REDUCTIONS)}; got {reduction!r}")
@@ -176,22 +126,14 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
                            f"{tuple(values.shape)}, {tuple(indices.shape)}")
     if not 1 <= values.shape[-1] <= DISTILL_MAX_K:
         raise RuntimeError(f"distillation_loss: 1 to {DISTILL_MAX_K} entries a row; got {values.shape[-1]}")
-    if indices.dtype != torch.int64:
-        if indices.dtype != torch.int32:
-            raise RuntimeError(f"distillation_loss: indices are int64 or int32; got {indices.dtype}")
-        indices = indices.long()
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"distillation_loss: indices are int64 or int32; got {indices.dtype}")
     if values.device != logits.device or indices.device != logits.device:
-        raise RuntimeError("distillation_loss: logits, values and indices are on one device")
-    if not 1e-6 <= float(temperature) <= 1e6:
+        raise RuntimeError(f"distillation_loss: logits, values and indices are on one device; got {logits.device}, {values.device}, {indices.device}")
+    if not 1e-6 <= temperature <= 1e6:
         raise RuntimeError(f"distillation_loss: 1e-6 <= temperature <= 1e6; got {temperature}")
-    lead, Cn, K = logits.shape[:-1], logits.shape[-1], values.shape[-1]
-    z = logits.reshape(-1, Cn)
-    if z.stride(1) != 1 or z.stride(0) < Cn:
-        z = z.contiguous()
-    values, indices = values.detach().reshape(-1, K).contiguous(), indices.reshape(-1, K).contiguous()
-    if z.requires_grad and torch.is_grad_enabled():
-        out = _Distill.apply(z, values, indices, float(temperature), code)
-    else:
-        rows, total, _ = _distill_forward(z, values, indices, float(temperature), code)
-        out = rows if code == 0 else total
+    if logits.dim() == 2:
+        return L_.torch_ops().distillation_loss(logits, values, indices, temperature, code)
+    lead, K = logits.shape[:-1], values.shape[-1]
+    out = L_.torch_ops().distillation_loss(logits.reshape(-1, logits.shape[-1]), values.reshape(-1, K), indices.reshape(-1, K), temperature, code)
     return out.view(lead) if code == 0 else out

@@ -31,6 +31,8 @@ typedef struct dvgr_attn_problem {
   float scale;             /* > 0                                                                        */
   dvgr_attn_view q, k, v;
   dvgr_attn_view o;        /* written by the forward, read by the backward                               */
+  void *o_lo;              /* bf16 / fp16, (B, Lq, H, Dh) contiguous, or NULL: what o's rounding left, to the type; the forward fills it and
+                              the backward takes rowsum(g_o o) with it, which halves the error of the score gradients' common part */
   const int64_t *lens;     /* (B) number of keys, clamped to [0, Lk], or NULL: Lk                        */
   const uint8_t *mask;     /* (B, Lk) 0 / 1, rows `mask_stride` bytes apart, or NULL                     */
   int64_t mask_stride;

@@ -79,7 +79,7 @@ def problem(**kw):
 
 def test_attention_refusals():
     lib = L.load()
-    assert C.sizeof(L.AttnView) == 32 and C.sizeof(L.AttnProblem) == 32 + 4 * 32 + 4 * 8 and C.sizeof(L.AttnGrads) == 4 * 32
+    assert C.sizeof(L.AttnView) == 32 and C.sizeof(L.AttnProblem) == 32 + 4 * 32 + 5 * 8 and C.sizeof(L.AttnGrads) == 4 * 32
     assert lib.dvgr_attn_check(C.byref(problem())) == 0 and lib.dvgr_attn_check(None) == E_NULL
     for kw in (dict(B=-1), dict(Lq=-1), dict(Lk=-1), dict(H=0), dict(Hk=0), dict(H=5), dict(Dh=0), dict(Dh=12), dict(Dh=136), dict(scale=0.0),
                dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(Lk=1 << 30), dict(Lq=1 << 29), dict(B=1 << 24)):
