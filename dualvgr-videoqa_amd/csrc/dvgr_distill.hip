@@ -61,23 +61,39 @@ __device__ __forceinline__ MaxSum wave_join(MaxSum a, float c) {
   return a;
 }
 
-// The elements [c0, c1) of a row, by threads `tid` of kThreads: 16-byte vectors where the address allows, single elements at the
-// ends (rows of an odd number of classes start at any alignment).
-template <typename T, typename FV, typename FE>
-__device__ __forceinline__ void for_row(const T* row, int64_t c0, int64_t c1, int tid, FV vec, FE one) {
+// The elements [c0, c1) of a row, by threads `tid` of kThreads: kUnroll 16-byte vectors at a time (as many loads in flight), single elements
+// at the ends (rows of an odd number of classes start at any alignment).
+constexpr int kUnroll = 4;
+template <typename T, typename FU, typename FE>
+__device__ __forceinline__ void for_row(const T* row, int64_t c0, int64_t c1, int tid, FU many, FE one) {
   constexpr int N = Vec16<T>::N;
   const int64_t lead = ((16 - ((uintptr_t)(row + c0) & 15)) & 15) / sizeof(T);
   const int64_t a = c0 + lead < c1 ? c0 + lead : c1;
   const int64_t e = a + (c1 - a) / N * N;
   for (int64_t c = c0 + tid; c < a; c += kThreads) one(c);
-  for (int64_t c = a + (int64_t)tid * N; c < e; c += kThreads * N) vec(c);
+  for (int64_t c = a + (int64_t)tid * N; c < e; c += kUnroll * kThreads * N) many(c, e);
   for (int64_t c = e + tid; c < c1; c += kThreads) one(c);
 }
 
 template <typename T>
 __device__ __forceinline__ MaxSum row_part(const T* row, int64_t c0, int64_t c1, float c, float (&sh)[8]) {
   MaxSum s;
-  for_row(row, c0, c1, threadIdx.x, [&](int64_t at) { float f[Vec16<T>::N]; load_vec(row + at, f); s.add(f, c); },
+  constexpr int N = Vec16<T>::N;
+  for_row(row, c0, c1, threadIdx.x, [&](int64_t at, int64_t e) {
+            typename Vec16<T>::type v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+              const int64_t x = at + (int64_t)u * kThreads * N;
+              if (x < e) v[u] = *reinterpret_cast<const typename Vec16<T>::type*>(row + x);
+              else v[u] = (T)-INFINITY;
+            }
+            float f[kUnroll * N];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+              for (int i = 0; i < N; ++i) f[u * N + i] = (float)v[u][i];
+            s.add(f, c);
+          },
           [&](int64_t at) { float f[1] = {(float)row[at]}; s.add(f, c); });
   s = wave_join(s, c);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -95,56 +111,77 @@ __device__ __forceinline__ int entry(const Distill& d, int64_t r, int k, float& 
   return (int)i;
 }
 
-// one wave: the teacher's side of a row and the row's loss
-template <typename T>
-__device__ __forceinline__ void finish_row(const Distill& d, int64_t r, const MaxSum& s, float* loss, RowStats* stats, int lane) {
-  const float c = d.invT * kLog2e, zlog = __log2f(s.l);
-  const T* row = (const T*)d.z + r * d.ldz;
-  MaxSum t;
-  for (int k = lane; k < d.K; k += 64) {
-    float v[1] = {-INFINITY};
-    entry(d, r, k, v[0]);
+// One wave: the teacher's side of a row, up to kHeld entries for each lane.  `fetch` is called before the row is streamed, so that its
+// three dependent loads are in flight meanwhile; longer lists load the rest in `finish`.
+constexpr int kHeld = 4;
+template <typename T> struct Entries {
+  float v[kHeld], z[kHeld];
+  static __device__ __forceinline__ void one(const Distill& d, int64_t r, int k, float& v, float& z) {
+    v = -INFINITY; z = 0.f;
+    const int i = k < d.K ? entry(d, r, k, v) : -1;
+    if (i >= 0) z = (float)((const T*)d.z)[r * d.ldz + i];
+  }
+  __device__ __forceinline__ void fetch(const Distill& d, int64_t r, int lane) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) one(d, r, lane + 64 * i, v[i], z[i]);
+  }
+  __device__ __forceinline__ void finish(const Distill& d, int64_t r, const MaxSum& s, float* loss, RowStats* stats, int lane) const {
+    const float c = d.invT * kLog2e, zlog = __log2f(s.l);
+    MaxSum t;
     t.add(v, c);
-  }
-  t = wave_join(t, c);
-  if (t.l != t.l) t.m = t.l;                                        // a NaN among the values is the row's loss
-  float sum = 0.f;
-  if (t.m != -INFINITY) {
-    const float vlog = __log2f(t.l);
-    for (int k = lane; k < d.K; k += 64) {
-      float v = -INFINITY;
-      const int i = entry(d, r, k, v);
-      if (i < 0 || v == -INFINITY) continue;                        // p = 0 adds nothing, whatever the student says there
-      const float logp = (v - t.m) * c - vlog, logq = ((float)row[i] - s.m) * c - zlog;
-      const float p = exp2_fast(logp);
-      if (p != 0.f) sum += p * (logp - logq);
+    for (int k = lane + 64 * kHeld; k < d.K; k += 64) {
+      float x[1], y;
+      one(d, r, k, x[0], y);
+      t.add(x, c);
     }
-    sum = wave_sum(sum);
-    t.l = vlog;
+    t = wave_join(t, c);
+    if (t.l != t.l) t.m = t.l;                                      // a NaN among the values is the row's loss
+    float sum = 0.f;
+    if (t.m != -INFINITY) {
+      const float vlog = __log2f(t.l);
+      const auto add = [&](float x, float y) {
+        if (x == -INFINITY) return;                                 // p = 0 adds nothing, whatever the student says there
+        const float logp = (x - t.m) * c - vlog, logq = (y - s.m) * c - zlog, p = exp2_fast(logp);
+        if (p != 0.f) sum += p * (logp - logq);
+      };
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) add(v[i], z[i]);
+      for (int k = lane + 64 * kHeld; k < d.K; k += 64) {
+        float x, y;
+        one(d, r, k, x, y);
+        add(x, y);
+      }
+      sum = wave_sum(sum);
+      t.l = vlog;
+    }
+    if (lane == 0) {
+      loss[r] = sum * kLn2 * d.T * d.T;
+      stats[r] = RowStats{s.m, zlog, t.m, t.l};
+    }
   }
-  if (lane == 0) {
-    loss[r] = sum * kLn2 * d.T * d.T;
-    stats[r] = RowStats{s.m, zlog, t.m, t.l};
-  }
-}
+};
 
 // splits == 1: a workgroup per row does everything.  Otherwise (few rows, many classes) it leaves its share's maximum and sum.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_distill_row(Distill d, float* loss, RowStats* stats, float2* part) {
   __shared__ float sh[8];
   const int64_t r = blockIdx.x / d.splits, c0 = (blockIdx.x % d.splits) * d.per, c1 = c0 + d.per < d.C ? c0 + d.per : d.C;
+  Entries<T> e;
+  if (d.splits == 1 && threadIdx.x < 64) e.fetch(d, r, threadIdx.x);
   const MaxSum s = row_part((const T*)d.z + r * d.ldz, c0, c1, d.invT * kLog2e, sh);
   if (d.splits > 1) {
     if (threadIdx.x == 0) part[blockIdx.x] = make_float2(s.m, s.l);
-  } else if (threadIdx.x < 64) finish_row<T>(d, r, s, loss, stats, threadIdx.x);
+  } else if (threadIdx.x < 64) e.finish(d, r, s, loss, stats, threadIdx.x);
 }
 
 template <typename T>
 __global__ __launch_bounds__(64) void k_distill_join(Distill d, const float2* part, float* loss, RowStats* stats) {
   const int64_t r = blockIdx.x;
+  Entries<T> e;
+  e.fetch(d, r, threadIdx.x);
   MaxSum s;
   for (int i = threadIdx.x; i < d.splits; i += 64) s.join(part[r * d.splits + i].x, part[r * d.splits + i].y, d.invT * kLog2e);
-  finish_row<T>(d, r, wave_join(s, d.invT * kLog2e), loss, stats, threadIdx.x);
+  e.finish(d, r, wave_join(s, d.invT * kLog2e), loss, stats, threadIdx.x);
 }
 
 // the sum of the rows' losses (/ number of rows that have an entry); behind the rows' statistics, the factor of a row's gradient
@@ -170,13 +207,13 @@ __global__ __launch_bounds__(1024) void k_distill_total(const float* loss, RowSt
 // SAME: z and its gradient have the same alignment, row by row.  A share is written densely first; the classes the teacher lists
 // are then written again with their p, which needs no atomics: entries of the same class all write the same sum.
 template <typename T, bool SAME>
-__global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowStats* stats, const float* up, int up_stride, T* gz, int64_t ldg) {
+__global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowStats* stats, const float* up, int up_stride, T* __restrict__ gz, int64_t ldg) {
   __shared__ int32_t sh_i[kMaxK];
   __shared__ float sh_p[kMaxK];
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x / d.splits, c0 = (blockIdx.x % d.splits) * d.per, c1 = c0 + d.per < d.C ? c0 + d.per : d.C;
   const RowStats s = stats[r];
-  const T* row = (const T*)d.z + r * d.ldz;
+  const T* __restrict__ row = (const T*)d.z + r * d.ldz;
   T* out = gz + r * ldg;
   const float c = d.invT * kLog2e;
   const bool empty = s.vmax == -INFINITY;
@@ -189,12 +226,19 @@ __global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowSt
     sh_p[k] = i < 0 || empty ? 0.f : exp2_fast((v - s.vmax) * c - s.vlog);
   }
   if (SAME)
-    for_row(row, c0, c1, tid, [&](int64_t at) {
-      float f[Vec16<T>::N];
-      load_vec(row + at, f);
+    for_row(row, c0, c1, tid, [&](int64_t at, int64_t e) {
+      constexpr int N = Vec16<T>::N;
+      float f[kUnroll][N];
 #pragma unroll
-      for (int i = 0; i < Vec16<T>::N; ++i) f[i] = grad(f[i]);
-      store_vec(out + at, f);
+      for (int u = 0; u < kUnroll; ++u)
+        if (at + (int64_t)u * kThreads * N < e) load_vec(row + at + (int64_t)u * kThreads * N, f[u]);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (at + (int64_t)u * kThreads * N >= e) break;
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[u][i] = grad(f[u][i]);
+        store_vec(out + at + (int64_t)u * kThreads * N, f[u]);
+      }
     }, [&](int64_t at) { out[at] = (T)grad((float)row[at]); });
   else
     for (int64_t at = c0 + tid; at < c1; at += kThreads) out[at] = (T)grad((float)row[at]);
@@ -208,10 +252,10 @@ __global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowSt
   }
 }
 
-// A workgroup reads its share of a row with 256 threads x 16 bytes at a time.  Few rows of many classes are split until there are
-// about 1024 workgroups, four for each compute unit, but no share is under 8192 classes.
+// Few rows of many classes are split until there are about 1024 workgroups, four for each compute unit, but no share is under 8192
+// classes; a split of two is not worth the launch that joins it while there are 512 rows.
 int split_of(int64_t R, int64_t C, int64_t& per) {
-  int64_t s = (1024 + R - 1) / R, most = (C + 8191) / 8192;
+  int64_t s = R >= 512 ? 1 : (1024 + R - 1) / R, most = (C + 8191) / 8192;
   s = s < most ? s : most;
   per = ((C + s - 1) / s + 15) / 16 * 16;
   return (int)((C + per - 1) / per);

@@ -3,8 +3,9 @@
 //   y_i = s E[t_i]                                   G[v] = s sum_{i : t_i = v} dy_i   (i ascending)
 //
 // Both are bound by memory: the forward reads and writes n rows, the backward reads n rows and writes the whole table.  The
-// gradient sorts (token, position) pairs by token with a stable radix sort and adds the rows of a token in the order of their
-// positions, in fp32, and rounds once: no float atomics, so the result does not depend on the schedule.
+// gradient brings the positions of a token together, adds their rows in fp32 in an order that the tokens alone decide, and rounds
+// once: no float atomics, so the result does not depend on the schedule.  Two forms: up to kSmall positions one launch in which
+// every workgroup picks the tokens of its own rows of the table; beyond, a stable radix sort of (token, position) pairs.
 #include <hip/hip_runtime.h>
 
 #include "../../include/dvgr.h"
@@ -16,8 +17,8 @@ namespace {
 
 // One wave per token position.  VEC: rows of 16-byte vectors; otherwise single elements, neighbouring lanes on neighbours.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_embed_fwd(const T* table, int64_t vocab, int wd, const int64_t* tokens, int64_t n,
-                                                   float scale, T* y, int32_t* bad) {
+__global__ __launch_bounds__(256) void k_embed_fwd(const T* __restrict__ table, int64_t vocab, int wd, const int64_t* __restrict__ tokens, int64_t n,
+                                                   float scale, T* __restrict__ y, int32_t* bad) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (row >= n) return;
@@ -28,12 +29,19 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const T* table, int64_t vocab
   const T* src = table + (ok ? tok : 0) * (int64_t)wd;
   constexpr int N = Vec16<T>::N;
   if (VEC) {
-    for (int c = lane; c < wd / N; c += 64) {
-      float f[N];
+    const int nv = wd / N;
+    for (int c = lane; c < nv; c += 128) {                          // two loads in flight
+      float f[N], g[N];
+      const bool more = c + 64 < nv;
       load_vec(src + c * N, f);
+      if (more) load_vec(src + (c + 64) * N, g);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = ok ? f[i] * scale : 0.f;
       store_vec(dst + c * N, f);
+      if (!more) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) g[i] = ok ? g[i] * scale : 0.f;
+      store_vec(dst + (c + 64) * N, g);
     }
   } else {
     for (int c = lane; c < wd; c += 64) dst[c] = (T)(ok ? (float)src[c] * scale : 0.f);
@@ -43,13 +51,13 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const T* table, int64_t vocab
 // ---- stable radix sort of (token, position), 8 bits a pass ------------------------------------------------------------------
 // A block owns `tile` consecutive elements.  Pass 0 reads the tokens themselves; a token that has no gradient (outside the table,
 // or the padding token) gets the key `vocab`, which sorts behind every row.
-constexpr int kRadix = 256, kSortThreads = 256;
+constexpr int kRadix = 256, kSortThreads = kRadix, kSortBlocks = 256;
 
 struct SortPass {
   const int64_t* tokens;            // pass 0
   const int32_t *key, *pos;         // later passes
   int32_t *key_out, *pos_out;
-  int32_t* hist;                    // kRadix x blocks: counts, then first places
+  int32_t* hist;                    // blocks x kRadix counts
   int64_t n, vocab, padding;
   int tile, blocks, shift;
 };
@@ -68,39 +76,35 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(SortPass s) {
   const int64_t a = (int64_t)blockIdx.x * s.tile, e = a + s.tile < s.n ? a + s.tile : s.n;
   for (int64_t i = a + tid; i < e; i += kSortThreads) atomicAdd(&cnt[(sort_key(s, i) >> s.shift) & (kRadix - 1)], 1);
   __syncthreads();
-  for (int d = tid; d < kRadix; d += kSortThreads) s.hist[(int64_t)d * s.blocks + blockIdx.x] = cnt[d];
+  for (int d = tid; d < kRadix; d += kSortThreads) s.hist[(int64_t)blockIdx.x * kRadix + d] = cnt[d];
 }
 
-// exclusive prefix sum of kRadix x blocks counts, digit-major: one workgroup, each thread a run of consecutive counts
-__global__ __launch_bounds__(1024) void k_sort_scan(int32_t* hist, int64_t count) {
-  __shared__ int32_t wsum[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t run = (count + 1023) / 1024, a = tid * run, e = a + run < count ? a + run : count;
-  int32_t own = 0;
-  for (int64_t i = a; i < e; ++i) own += hist[i];
-  int32_t inc = own;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int32_t up = __shfl_up(inc, d);
-    if (lane >= d) inc += up;
-  }
-  if (lane == 63) wsum[wave] = inc;
-  __syncthreads();
-  int32_t at = inc - own;
-  for (int w = 0; w < wave; ++w) at += wsum[w];
-  for (int64_t i = a; i < e; ++i) {
-    const int32_t c = hist[i];
-    hist[i] = at;
-    at += c;
-  }
-}
-
-// Stable scatter: rounds of 256 consecutive elements; an element's place is the digit's next free place plus the number of equal
-// digits in front of it in the round (earlier waves' counts, then earlier lanes by ballots).
+// Stable scatter.  Thread d adds up digit d over all blocks (there are at most kSortBlocks) and over those in front of this one; with the
+// digits in front that is the block's first place.  Then rounds of 256 consecutive elements; an element's place is the digit's next
+// free place plus the number of equal digits in front of it in the round (earlier waves' counts, then earlier lanes by ballots).
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortPass s) {
-  __shared__ int32_t next[kRadix], wcnt[4][kRadix];
+  __shared__ int32_t next[kRadix], wcnt[4][kRadix], wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int d = tid; d < kRadix; d += kSortThreads) next[d] = s.hist[(int64_t)d * s.blocks + blockIdx.x];
+  {
+    int32_t all = 0, front = 0;
+#pragma unroll 8
+    for (int b = 0; b < s.blocks; ++b) {
+      const int32_t c = s.hist[b * kRadix + tid];
+      all += c;
+      front += b < (int)blockIdx.x ? c : 0;
+    }
+    int32_t inc = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t up = __shfl_up(inc, d);
+      if (lane >= d) inc += up;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    int32_t at = inc - all + front;
+    for (int w = 0; w < wave; ++w) at += wsum[w];
+    next[tid] = at;
+  }
   const int64_t a = (int64_t)blockIdx.x * s.tile, e = a + s.tile < s.n ? a + s.tile : s.n;
   for (int64_t i0 = a; i0 < e; i0 += kSortThreads) {
     const int64_t i = i0 + tid;
@@ -131,13 +135,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortPass s) {
   }
 }
 
-__global__ __launch_bounds__(256) void k_embed_zero(uint4* g, int64_t n16) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256) g[i] = make_uint4(0, 0, 0, 0);
-}
-template <typename T> __global__ __launch_bounds__(256) void k_embed_zero_elems(T* g, int64_t a, int64_t e) {
-  for (int64_t i = a + (int64_t)blockIdx.x * 256 + threadIdx.x; i < e; i += (int64_t)gridDim.x * 256) g[i] = (T)0.f;
-}
-
 // ---- rows of one token are consecutive now: sum them ------------------------------------------------------------------------
 // One wave owns `kChunk` sorted pairs and 64 lanes x NE elements of the row.  A token whose pairs all lie in the chunk is written at
 // once; one that crosses the chunk's ends leaves fp32 partial sums, head (0) and tail (1), which k_embed_join adds in chunk order.
@@ -148,14 +145,21 @@ template <typename T, bool VEC> struct Cols {
   int c0, wd, lane;
   __device__ Cols(int block, int wd_, int lane_) : c0(block * 64 * N), wd(wd_), lane(lane_) {}
   __device__ __forceinline__ int at(int i) const { return VEC ? c0 + lane * N + i : c0 + i * 64 + lane; }
-  __device__ __forceinline__ void load(const T* row, float (&f)[N]) const {
+  typedef typename Vec16<T>::type Raw;                              // held as loaded: half the registers of floats for two-byte types
+  __device__ __forceinline__ Raw load(const T* row) const {
+    Raw v;
     if (VEC) {
-      if (at(0) < wd) load_vec(row + at(0), f);
-      else for (int i = 0; i < N; ++i) f[i] = 0.f;
+      if (at(0) < wd) return *reinterpret_cast<const Raw*>(row + at(0));
+      v = (T)0.f;
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = at(i) < wd ? (float)row[at(i)] : 0.f;
+      for (int i = 0; i < N; ++i) v[i] = at(i) < wd ? row[at(i)] : (T)0.f;
     }
+    return v;
+  }
+  static __device__ __forceinline__ void add(float (&acc)[N], const Raw& v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += (float)v[i];
   }
   __device__ __forceinline__ void store(T* row, const float (&f)[N]) const {
     if (VEC) {
@@ -166,19 +170,64 @@ template <typename T, bool VEC> struct Cols {
     }
   }
   __device__ __forceinline__ void store_part(float* row, const float (&f)[N]) const {
+    if (VEC) {
+      if (at(0) < wd)
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (at(i) < wd) row[at(i)] = f[i];
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(row + at(i)) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) if (at(i) < wd) row[at(i)] = f[i];
+    }
   }
   __device__ __forceinline__ void add_part(const float* row, float (&f)[N]) const {
+    if (VEC) {
+      if (at(0) < wd)
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (at(i) < wd) f[i] += row[at(i)];
+        for (int i = 0; i < N; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(row + at(i));
+          f[i] += v.x; f[i + 1] += v.y; f[i + 2] += v.z; f[i + 3] += v.w;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) if (at(i) < wd) f[i] += row[at(i)];
+    }
   }
 };
 
+// the rows of the table that no pair names are zero: blocks behind those of the sums look their rows up and clear them
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_embed_sum(const T* g_y, const int32_t* key, const int32_t* pos, int64_t n, int64_t vocab, int wd,
-                                                   int colblocks, float scale, T* g_table, float* part) {
+__device__ __forceinline__ void zero_rows(const int32_t* key, int64_t n, int64_t vocab, int wd, int64_t r0, int rows, T* g_table) {
+  constexpr int N = Vec16<T>::N;
+  __shared__ int sh_there[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid < rows && r0 + tid < vocab) {
+    int64_t a = 0, b = n;                                           // first pair of a token >= r0 + tid
+    while (a < b) {
+      const int64_t m = (a + b) >> 1;
+      if (key[m] < r0 + tid) a = m + 1; else b = m;
+    }
+    sh_there[tid] = a < n && key[a] == r0 + tid;
+  }
+  __syncthreads();
+  float z[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i] = 0.f;
+  for (int r = wave; r < rows && r0 + r < vocab; r += 4) {
+    if (sh_there[r]) continue;
+    T* row = g_table + (r0 + r) * wd;
+    if (VEC) for (int c = lane * N; c < wd; c += 64 * N) store_vec(row + c, z);
+    else for (int c = lane; c < wd; c += 64) row[c] = (T)0.f;
+  }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void k_embed_sum(const T* __restrict__ g_y, const int32_t* key, const int32_t* pos, int64_t n, int64_t vocab, int wd,
+                                                   int colblocks, float scale, T* __restrict__ g_table, float* part, int sum_blocks, int zero_per) {
   constexpr int N = Vec16<T>::N, U = 8;
+  if ((int)blockIdx.x >= sum_blocks) {
+    zero_rows<T, VEC>(key, n, vocab, wd, (int64_t)((int)blockIdx.x - sum_blocks) * zero_per, zero_per, g_table);
+    return;
+  }
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int64_t chunk = unit / colblocks, a = chunk * kChunk;
@@ -196,11 +245,11 @@ __global__ __launch_bounds__(256) void k_embed_sum(const T* g_y, const int32_t* 
   if (cur >= vocab) return;
   bool open_left = cur == left;
   for (int j0 = 0; j0 < m; j0 += U) {
-    float f[U][N];
+    typename Cols<T, VEC>::Raw f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {                                   // (padding pairs of a short chunk read a row that exists: position 0)
       const int32_t p = __builtin_amdgcn_readlane(mypos, (j0 + u) & 63);
-      cols.load(g_y + (int64_t)p * wd, f[u]);
+      f[u] = cols.load(g_y + (int64_t)p * wd);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -218,8 +267,7 @@ __global__ __launch_bounds__(256) void k_embed_sum(const T* g_y, const int32_t* 
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += f[u][i];
+      cols.add(acc, f[u]);
     }
   }
   if (open_left) cols.store_part(part + (2 * chunk) * wd, acc);     // a token that fills the chunk and came in from the left: head
@@ -231,63 +279,198 @@ __global__ __launch_bounds__(256) void k_embed_sum(const T* g_y, const int32_t* 
   }
 }
 
-// Tokens that cross chunks: the workgroup of the chunk where the token starts adds its tail and the following heads.  kJoinWaves waves
-// take consecutive, equal shares of the heads (a frequent token has thousands) and are added in order.
-constexpr int kJoinWaves = 8;
+// Tokens that cross chunks: the chunk where a token starts adds its tail and the heads that follow.  A wave looks at one chunk's end and
+// adds up to kAlone heads by itself; a frequent token has hundreds, which the workgroup's waves share, consecutive equal parts each,
+// added in order.
+constexpr int kJoinWaves = 16, kAlone = 8;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* key, int64_t n, int64_t vocab, int wd, int colblocks, float scale,
                                                                 T* g_table, const float* part) {
   constexpr int N = Vec16<T>::N;
   __shared__ float sh[kJoinWaves][64 * N];
-  __shared__ int32_t sh_end;
+  __shared__ int32_t sh_long[kJoinWaves], sh_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t chunk = blockIdx.x / colblocks, a = chunk * kChunk, b = a + kChunk;      // b < n: the launch leaves the last chunk out
-  const int32_t k = key[b - 1];
-  if (k >= vocab || key[b] != k) return;                            // nothing crosses this chunk's end,
-  if (a > 0 && key[a - 1] == k) return;                             // or it started further left
-  const int64_t chunks = (n + kChunk - 1) / kChunk;
-  int64_t end = chunk + 1;                                          // the first chunk behind `chunk` that does not start with k
-  for (;; ) {
-    if (tid == 0) sh_end = 64 * kJoinWaves;
-    __syncthreads();
-    const int64_t c = end + tid;
-    if (c >= chunks || key[c * kChunk] != k) atomicMin(&sh_end, tid);
-    __syncthreads();
-    const int got = sh_end;
-    end += got;
-    __syncthreads();
-    if (got < 64 * kJoinWaves) break;
-  }
+  const int64_t chunks = (n + kChunk - 1) / kChunk, first = (int64_t)(blockIdx.x / colblocks) * kJoinWaves, mine = first + wave;
   const Cols<T, VEC> cols((int)(blockIdx.x % colblocks), wd, lane);
-  const int64_t heads = end - (chunk + 1), share = (heads + kJoinWaves - 1) / kJoinWaves;
-  const int64_t h0 = chunk + 1 + wave * share, h1 = h0 + share < end ? h0 + share : end;
+  // heads of the token that starts in chunk c and leaves it, up to 64; 0: there is none
+  const auto heads_of = [&](int64_t c) {
+    const int64_t b = (c + 1) * kChunk;                             // c + 1 is a chunk: b < n
+    const int32_t k = key[b - 1];
+    if (k >= vocab || key[b] != k || (c > 0 && key[c * kChunk - 1] == k)) return 0;
+    const unsigned long long other = __ballot(c + 1 + lane >= chunks || key[(c + 1 + lane) * kChunk] != k);
+    return other ? __ffsll(other) - 1 : 64;
+  };
   float acc[N];
+  int heads = mine + 1 < chunks ? heads_of(mine) : 0;
+  if (lane == 0) sh_long[wave] = heads > kAlone;
+  if (heads > 0 && heads <= kAlone) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (wave == 0) cols.add_part(part + (2 * chunk + 1) * wd, acc);
-#pragma unroll 4
-  for (int64_t h = h0; h < h1; ++h) cols.add_part(part + (2 * h) * wd, acc);
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    cols.add_part(part + (2 * mine + 1) * wd, acc);
+#pragma unroll 2
+    for (int h = 1; h <= heads; ++h) cols.add_part(part + 2 * (mine + h) * wd, acc);
 #pragma unroll
-  for (int i = 0; i < N; ++i) sh[wave][i * 64 + lane] = acc[i];
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float t = acc[i];
-    for (int w = 1; w < kJoinWaves; ++w) t += sh[w][i * 64 + lane];
-    acc[i] = t * scale;
+    for (int i = 0; i < N; ++i) acc[i] *= scale;
+    cols.store(g_table + (int64_t)key[(mine + 1) * kChunk] * wd, acc);
   }
-  cols.store(g_table + (int64_t)k * wd, acc);
+  __syncthreads();
+  for (int w = 0; w < kJoinWaves; ++w) {
+    if (!sh_long[w]) continue;                                      // (uniform over the workgroup)
+    const int64_t c = first + w;
+    const int32_t k = key[(c + 1) * kChunk];
+    int64_t a = c + 1;                                              // first chunk behind c that does not start with k
+    for (int got = 64 * kJoinWaves; got == 64 * kJoinWaves; a += got) {
+      if (tid == 0) sh_end = 64 * kJoinWaves;
+      __syncthreads();
+      if (a + tid >= chunks || key[(a + tid) * kChunk] != k) atomicMin(&sh_end, tid);
+      __syncthreads();
+      got = sh_end;
+      __syncthreads();
+    }
+    const int64_t share = (a - (c + 1) + kJoinWaves - 1) / kJoinWaves;
+    const int64_t h0 = c + 1 + wave * share, h1 = h0 + share < a ? h0 + share : a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    if (wave == 0) cols.add_part(part + (2 * c + 1) * wd, acc);
+#pragma unroll 4
+    for (int64_t h = h0; h < h1; ++h) cols.add_part(part + (2 * h) * wd, acc);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sh[wave][i * 64 + lane] = acc[i];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float x = acc[i];
+        for (int v = 1; v < kJoinWaves; ++v) x += sh[v][i * 64 + lane];
+        acc[i] = x * scale;
+      }
+      cols.store(g_table + (int64_t)k * wd, acc);
+    }
+    __syncthreads();
+  }
 }
 
+// ---- few positions: one launch ----------------------------------------------------------------------------------------------
+// Workgroup w of kSmallGroups owns the rows w, w + kSmallGroups, ... (the frequent tokens of a vocabulary are neighbours).  It reads all the tokens (they fit the L2 many times over) and keeps the positions of its own
+// in their order.  A wave takes a row and adds its positions one after the other; a row of more than kAloneRow positions is shared by the
+// workgroup's waves, consecutive equal parts each, added in order.
+constexpr int kSmall = 4096, kSmallWaves = 16, kSmallThreads = 64 * kSmallWaves, kSmallRows = 256, kAloneRow = 16, kSmallGroups = 512;
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kSmallThreads) void k_embed_small(const T* __restrict__ g_y, const int64_t* __restrict__ tokens, int n, int64_t vocab, int wd,
+                                                               int colblocks, float scale, int64_t padding, T* __restrict__ g_table) {
+  constexpr int N = Vec16<T>::N, U = 4;
+  __shared__ uint16_t pos[kSmall], sel[kSmall], row[kSmall];
+  __shared__ int32_t cnt[kSmallRows], wcnt[kSmallWaves];
+  __shared__ float sh[kSmallWaves][64 * N];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rows = (int)((vocab - blockIdx.x + kSmallGroups - 1) / kSmallGroups);
+  const auto row_at = [&](int r) { return g_table + ((int64_t)r * kSmallGroups + blockIdx.x) * wd; };
+  if (tid < kSmallRows) cnt[tid] = 0;
+  __syncthreads();
+  // puts the elements that are `mine` behind the `have` that are there, in the threads' order; how many there are then
+  const auto compact = [&](int have, bool mine, auto put) {
+    const unsigned long long b = __ballot(mine);
+    if (lane == 0) wcnt[wave] = __popcll(b);
+    __syncthreads();
+    int at = have + __popcll(b & ((1ull << lane) - 1ull)), all = have;
+    for (int w = 0; w < kSmallWaves; ++w) {
+      at += w < wave ? wcnt[w] : 0;
+      all += wcnt[w];
+    }
+    if (mine) put(at);
+    __syncthreads();
+    return all;
+  };
+  int m = 0;
+  for (int i0 = 0; i0 < n; i0 += kSmallThreads) {
+    const int i = i0 + tid;
+    const int64_t t = i < n ? tokens[i] : -1;
+    const bool mine = t >= 0 && t < vocab && t % kSmallGroups == blockIdx.x && t != padding;
+    if (mine) atomicAdd(&cnt[t / kSmallGroups], 1);
+    m = compact(m, mine, [&](int at) { pos[at] = (uint16_t)i; row[at] = (uint16_t)(t / kSmallGroups); });
+  }
+  float acc[N];
+  for (int r = wave; r < rows; r += kSmallWaves) {
+    if (cnt[r] > kAloneRow) continue;
+    for (int cb = 0; cb < colblocks; ++cb) {
+      const Cols<T, VEC> cols(cb, wd, lane);
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      for (int j0 = 0, left = cnt[r]; left; j0 += 64) {             // ends: the list holds cnt[r] of row r
+        unsigned long long b = __ballot(j0 + lane < m && row[(j0 + lane) & (kSmall - 1)] == r);
+        left -= __popcll(b);
+        while (b) {
+          typename Cols<T, VEC>::Raw f[U];
+          int have = 0;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (!b) break;
+            f[u] = cols.load(g_y + (int64_t)pos[j0 + __ffsll(b) - 1] * wd);
+            b &= b - 1;
+            ++have;
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (u < have) cols.add(acc, f[u]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] *= scale;
+      cols.store(row_at(r), acc);
+    }
+  }
+  for (int r = 0; r < rows; ++r) {
+    const int k = cnt[r];
+    if (k <= kAloneRow) continue;                                   // (uniform over the workgroup)
+    int have = 0;
+    for (int j0 = 0; j0 < m; j0 += kSmallThreads) {
+      const int j = j0 + tid;
+      have = compact(have, j < m && row[j & (kSmall - 1)] == r, [&](int at) { sel[at] = pos[j]; });
+    }
+    const int share = (k + kSmallWaves - 1) / kSmallWaves, a = wave * share, b = a + share < k ? a + share : k;
+    for (int cb = 0; cb < colblocks; ++cb) {
+      const Cols<T, VEC> cols(cb, wd, lane);
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      for (int j = a; j < b; j += U) {
+        typename Cols<T, VEC>::Raw f[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) f[u] = cols.load(g_y + (int64_t)sel[j + u < b ? j + u : j] * wd);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (j + u < b) cols.add(acc, f[u]);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) sh[wave][i * 64 + lane] = acc[i];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          float x = acc[i];
+          for (int w = 1; w < kSmallWaves; ++w) x += sh[w][i * 64 + lane];
+          acc[i] = x * scale;
+        }
+        cols.store(row_at(r), acc);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// One launch for up to kSmall positions while a workgroup's rows fit its counters.
 struct EmbedPlan {
+  bool small;
   int tile, blocks, passes, colblocks;
   int64_t chunks;
   size_t key[2], pos[2], hist, part, total;       // byte offsets
 };
 EmbedPlan embed_plan(int64_t n, int64_t vocab, int wd, int elem) {
   EmbedPlan p{};
-  p.tile = n <= (1 << 18) ? 1024 : 4096;
+  p.small = n <= kSmall && vocab <= (int64_t)kSmallGroups * kSmallRows;
+  if (p.small) return p;
+  const int64_t tile = (n + kSortBlocks - 1) / kSortBlocks;          // at most kSortBlocks blocks, 1024 pairs each at least
+  p.tile = (int)(tile < 1024 ? 1024 : (tile + kSortThreads - 1) / kSortThreads * kSortThreads);
   p.blocks = (int)((n + p.tile - 1) / p.tile);
   for (int64_t v = vocab; v; v >>= 8) ++p.passes;                   // keys are 0 .. vocab
   p.colblocks = (wd + 64 * (16 / elem_size(elem)) - 1) / (64 * (16 / elem_size(elem)));
@@ -303,7 +486,7 @@ EmbedPlan embed_plan(int64_t n, int64_t vocab, int wd, int elem) {
 
 int embed_check(int64_t n, int64_t vocab, int wd, int elem) {
   if (!elem_size(elem)) return DVGR_E_KIND;
-  if (vocab < 1 || vocab >= (1ll << 31) - 1 || wd < 1 || n < 0 || n >= (1ll << 26)) return DVGR_E_DIMS;
+  if (vocab < 1 || vocab >= (1ll << 31) - 1 || wd < 1 || wd >= (1 << 30) || n < 0 || n >= (1ll << 26)) return DVGR_E_DIMS;
   if (n / kChunk * (wd / 256 + 1) >= (1ll << 23)) return DVGR_E_DIMS;            // a launch holds at most 2^32 threads
   return 0;
 }
@@ -320,47 +503,47 @@ int embed_forward(const T* table, int64_t vocab, int wd, const int64_t* tokens, 
 template <typename T, bool VEC>
 int embed_sum(const T* g_y, const int32_t* key, const int32_t* pos, int64_t n, int64_t vocab, int wd, const EmbedPlan& p, float scale,
               T* g_table, float* part, hipStream_t st) {
-  const int64_t units = p.chunks * p.colblocks;
-  DVGR_LAUNCH((k_embed_sum<T, VEC>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, g_y, key, pos, n, vocab, wd, p.colblocks, scale,
-              g_table, part);
+  const int64_t row_bytes = (int64_t)wd * sizeof(T), sum_blocks = (p.chunks * p.colblocks + 3) / 4;
+  const int zero_per = row_bytes >= 32768 ? 1 : row_bytes <= 128 ? 256 : (int)(32768 / row_bytes);
+  DVGR_LAUNCH((k_embed_sum<T, VEC>), dim3((unsigned)(sum_blocks + (vocab + zero_per - 1) / zero_per)), dim3(256), 0, st, g_y, key, pos, n, vocab, wd,
+              p.colblocks, scale, g_table, part, (int)sum_blocks, zero_per);
   int e = (int)hipGetLastError();
   if (e || p.chunks < 2) return e;
-  DVGR_LAUNCH((k_embed_join<T, VEC>), dim3((unsigned)((p.chunks - 1) * p.colblocks)), dim3(64 * kJoinWaves), 0, st, key, n, vocab, wd, p.colblocks,
-              scale, g_table, part);
+  DVGR_LAUNCH((k_embed_join<T, VEC>), dim3((unsigned)((p.chunks - 1 + kJoinWaves - 1) / kJoinWaves * p.colblocks)), dim3(64 * kJoinWaves), 0, st, key, n,
+              vocab, wd, p.colblocks, scale, g_table, part);
+  return (int)hipGetLastError();
+}
+
+template <typename T, bool VEC>
+int embed_small(const T* g_y, const int64_t* tokens, int n, int64_t vocab, int wd, float scale, int64_t padding, T* g_table, hipStream_t st) {
+  const int colblocks = (wd + 64 * Vec16<T>::N - 1) / (64 * Vec16<T>::N);
+  DVGR_LAUNCH((k_embed_small<T, VEC>), dim3((unsigned)(vocab < kSmallGroups ? vocab : kSmallGroups)), dim3(kSmallThreads), 0, st, g_y, tokens, n, vocab, wd, colblocks, scale,
+              padding, g_table);
   return (int)hipGetLastError();
 }
 
 template <typename T>
 int embed_backward(const T* g_y, const int64_t* tokens, int64_t n, int64_t vocab, int wd, float scale, int64_t padding, T* g_table,
                    char* ws, const EmbedPlan& p, hipStream_t st) {
-  const int64_t total = vocab * wd, n16 = ptr16(g_table) ? total * (int64_t)sizeof(T) / 16 : 0;
-  if (n16) {
-    const int64_t blocks = (n16 + 255) / 256;
-    DVGR_LAUNCH(k_embed_zero, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, reinterpret_cast<uint4*>(g_table), n16);
-  }
-  const int64_t done = n16 * 16 / (int64_t)sizeof(T);
-  if (done < total) {                                               // the last elements, or a table that is not 16-byte aligned
-    const int64_t blocks = (total - done + 255) / 256;
-    DVGR_LAUNCH((k_embed_zero_elems<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, g_table, done, total);
-  }
-  if (n == 0) return (int)hipGetLastError();
+  const bool vec = wd % Vec16<T>::N == 0 && ptr16(g_y) && ptr16(g_table);
+  if (p.small)
+    return vec ? embed_small<T, true>(g_y, tokens, (int)n, vocab, wd, scale, padding, g_table, st)
+               : embed_small<T, false>(g_y, tokens, (int)n, vocab, wd, scale, padding, g_table, st);
   SortPass s{};
   s.n = n; s.vocab = vocab; s.padding = padding; s.tile = p.tile; s.blocks = p.blocks;
   s.hist = reinterpret_cast<int32_t*>(ws + p.hist);
   int at = 0;
-  for (int i = 0; i < p.passes; ++i, at ^= 1) {
+  for (int i = 0; n && i < p.passes; ++i, at ^= 1) {
     s.tokens = i ? nullptr : tokens;
     s.key = reinterpret_cast<int32_t*>(ws + p.key[at]); s.pos = reinterpret_cast<int32_t*>(ws + p.pos[at]);
     s.key_out = reinterpret_cast<int32_t*>(ws + p.key[at ^ 1]); s.pos_out = reinterpret_cast<int32_t*>(ws + p.pos[at ^ 1]);
     s.shift = 8 * i;
     DVGR_LAUNCH(k_sort_count, dim3(p.blocks), dim3(kSortThreads), 0, st, s);
-    DVGR_LAUNCH(k_sort_scan, dim3(1), dim3(1024), 0, st, s.hist, (int64_t)kRadix * p.blocks);
     DVGR_LAUNCH(k_sort_scatter, dim3(p.blocks), dim3(kSortThreads), 0, st, s);
   }
   const int32_t* key = reinterpret_cast<const int32_t*>(ws + p.key[at]);
   const int32_t* pos = reinterpret_cast<const int32_t*>(ws + p.pos[at]);
   float* part = reinterpret_cast<float*>(ws + p.part);
-  const bool vec = wd % Vec16<T>::N == 0 && ptr16(g_y) && ptr16(g_table);
   return vec ? embed_sum<T, true>(g_y, key, pos, n, vocab, wd, p, scale, g_table, part, st)
              : embed_sum<T, false>(g_y, key, pos, n, vocab, wd, p, scale, g_table, part, st);
 }
@@ -387,15 +570,15 @@ int dvgr_embed_forward(const void* table, int64_t vocab, int wd, int elem, const
 }
 
 size_t dvgr_embed_workspace_bytes(int64_t n, int64_t vocab, int wd, int elem) {
-  return embed_check(n, vocab, wd, elem) || n == 0 ? 0 : embed_plan(n, vocab, wd, elem).total;
+  return embed_check(n, vocab, wd, elem) ? 0 : embed_plan(n, vocab, wd, elem).total;
 }
 
 int dvgr_embed_backward(const void* g_y, const int64_t* tokens, int64_t n, int64_t vocab, int wd, int elem, float scale, int64_t padding_idx,
                         void* g_table, void* workspace, size_t workspace_bytes, void* stream) {
   const int e = embed_check(n, vocab, wd, elem);
   if (e) return e;
-  if (!g_table || (n && (!g_y || !tokens || !workspace))) return DVGR_E_NULL;
-  const EmbedPlan p = n ? embed_plan(n, vocab, wd, elem) : EmbedPlan{};
+  const EmbedPlan p = embed_plan(n, vocab, wd, elem);
+  if (!g_table || (n && (!g_y || !tokens)) || (p.total && !workspace)) return DVGR_E_NULL;
   if (workspace_bytes < p.total) return DVGR_E_WORKSPACE;
   if (!ptr16(workspace)) return DVGR_E_ALIGN;
   hipStream_t st = (hipStream_t)stream;

@@ -26,14 +26,14 @@ def test_embedding_refusals():
     assert f(A, 10, 8, 0, None, 4, 1.0, A, None, None) == E_NULL
     assert f(A, 10, 8, 0, A, 4, 1.0, None, None, None) == E_NULL
     assert f(None, 10, 8, 0, None, 0, 1.0, None, None, None) == 0                     # nothing to do
-    need = ws(100, 10, 8, 0)
-    assert need > 0 and ws(0, 10, 8, 0) == 0 and ws(-1, 10, 8, 0) == 0 and ws(100, 10, 8, 9) == 0
-    assert b(A, A, 100, 10, 8, 0, 1.0, -1, None, A, need, None) == E_NULL
-    assert b(None, A, 100, 10, 8, 0, 1.0, -1, A, A, need, None) == E_NULL
-    assert b(A, A, 100, 10, 8, 0, 1.0, -1, A, None, need, None) == E_NULL
-    assert b(A, A, 100, 10, 8, 0, 1.0, -1, A, A, need - 1, None) == E_WORKSPACE
-    assert b(A, A, 100, 10, 8, 0, 1.0, -1, A, A + 8, need, None) == E_ALIGN
-    assert b(A, A, 100, 10, 8, 7, 1.0, -1, A, A, need, None) == E_KIND
+    need = ws(9000, 10, 8, 0)
+    assert need > 0 and ws(100, 10, 8, 0) == 0 and ws(0, 10, 8, 0) == 0 and ws(-1, 10, 8, 0) == 0 and ws(100, 10, 8, 9) == 0
+    assert b(A, A, 9000, 10, 8, 0, 1.0, -1, None, A, need, None) == E_NULL
+    assert b(None, A, 9000, 10, 8, 0, 1.0, -1, A, A, need, None) == E_NULL
+    assert b(A, A, 9000, 10, 8, 0, 1.0, -1, A, None, need, None) == E_NULL
+    assert b(A, A, 9000, 10, 8, 0, 1.0, -1, A, A, need - 1, None) == E_WORKSPACE
+    assert b(A, A, 9000, 10, 8, 0, 1.0, -1, A, A + 8, need, None) == E_ALIGN
+    assert b(A, A, 9000, 10, 8, 7, 1.0, -1, A, A, need, None) == E_KIND
 
 
 def test_distillation_refusals():
