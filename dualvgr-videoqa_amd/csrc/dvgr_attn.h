@@ -35,7 +35,7 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256, kWaves = 4;          // of the kernels for many rows
 
 // One head's side of a tensor: row r of the packed rows (query l, head g of the group, r = l * G + g) or key r (G = 1).
 struct Side {

@@ -3,10 +3,10 @@
 //     P = exp2(c q.k - lse)      D = rowsum(dO o O)      dS = P o (dO V^T - D)
 //     dV = P^T dO      dK = scale dS^T Q      dQ = scale dS K
 //
-// Two passes over the scores, neither with atomics: one owns keys and goes over the packed rows (dK, dV; the heads of a group are rows
-// of the same reduction), one owns rows and goes over the keys (dQ).  The scores are computed in both: 7 products instead of 5, for
-// results that do not depend on the schedule.
-#include "dvgr_attn.h"
+// Many rows: two passes over the scores, neither with atomics: one owns keys and goes over the packed rows (dK, dV; the heads of a
+// group are rows of the same reduction), one owns rows and goes over the keys (dQ).  The scores are computed in both: 7 products
+// instead of 5, for results that do not depend on the schedule.  Up to 32 rows: one pass over the keys does it all.
+#include "dvgr_attn_few.h"
 
 namespace dvgr {
 namespace attn {
@@ -71,9 +71,24 @@ template <typename T> __device__ __forceinline__ float grad16(float ds, float sc
   return Grad16<T>::on ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
 }
 
+template <typename T, int NT> __device__ __forceinline__ void write_dq(const BwdArgs& B, int b, int hk, int row, const f32x16 (&dq)[NT], float f, int first,
+                                                                       int step, int lane) {
+  char* out = const_cast<char*>(q_side(B.f, B.g_q, b, hk).row(row, B.f.G));
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t % step != first) continue;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * t + 8 * g + (lane >> 5) * 4;
+      if (d < B.f.a.Dh) store4<T>(out + d * sizeof(T), dq[t][4 * g] * f, dq[t][4 * g + 1] * f, dq[t][4 * g + 2] * f, dq[t][4 * g + 3] * f);
+    }
+  }
+}
+
 // ---- dK, dV: KW x 32 keys of one key head, RW x RS x 32 packed rows a turn -------------------------------------------------------
+// (The accumulators are 2 DP / 32 x 16 registers; up to 96 two waves of a SIMD hold theirs, at 128 one.)
 template <typename T, int DP, int KW, int RW, int RS>
-__global__ __launch_bounds__(kThreads) void k_attn_dkv(BwdArgs B) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 2 : 1)) void k_attn_dkv(BwdArgs B) {
   const Args& A = B.f;
   typedef Tile<T, DP> Tl;
   constexpr int RT = RW * RS * 32, KT = KW * 32, NT = Tl::kNT;
@@ -191,22 +206,22 @@ __global__ __launch_bounds__(kThreads) void k_attn_dkv(BwdArgs B) {
   }
 }
 
-// ---- dQ: QW x 32 packed rows, KW x KS x 32 keys a turn (the forward's arrangement) -----------------------------------------------
-template <typename T, int DP, int QW, int KW, int KS>
+// ---- dQ: 4 x 32 packed rows, KS x 32 keys a turn (the forward's arrangement) ---------------------------------------------------
+template <typename T, int DP, int KS>
 __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   const Args& A = B.f;
   typedef Tile<T, DP> Tl;
-  constexpr int KT = KW * KS * 32, RT = QW * 32, NT = Tl::kNT;
+  constexpr int KT = KS * 32, RT = kWaves * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   char* lk = lds;
   char* lv = lds + Tl::template bytes<KT>();
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, qw = wave / KW, kw = wave % KW;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rtiles = (A.rows + RT - 1) / RT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles);
   if (w < 0) return;
   const int rt = (int)(w % rtiles), hk = (int)(w / rtiles % A.a.Hk), b = (int)(w / rtiles / A.a.Hk);
   const int n = key_count(A, b), dhb = A.a.Dh * A.es, tn = (n + KT - 1) / KT;
-  const int row = rt * RT + qw * 32 + (lane & 31);
+  const int row = rt * RT + wave * 32 + (lane & 31);
   const bool live = row < A.rows;
   const Side ks = k_side(A, A.a.k, b, hk), vs = k_side(A, A.a.v, b, hk);
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)b * A.a.mask_stride : nullptr;
@@ -230,8 +245,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   const auto fetch = [&](int t) {
     sk.fetch(ks, 1, t * KT, n, mask, dhb, tid);
     sv.fetch(vs, 1, t * KT, n, mask, dhb, tid);
-    const int j = t * KT + kw * KS * 32 + lane;
-    there = lane < KS * 32 && j < n && (!mask || mask[j]);
+    const int j = t * KT + lane;
+    there = lane < KT && j < n && (!mask || mask[j]);
   };
   if (tn) fetch(0);
   for (int t = 0; t < tn; ++t) {
@@ -241,12 +256,12 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
     const unsigned long long bits = __ballot(there);
     __syncthreads();
     if (t + 1 < tn) fetch(t + 1);
-    if (!bits) continue;
 #pragma unroll 1
     for (int i = 0; i < KS; ++i) {
-      const char* tk = lk + (kw * KS + i) * 32 * Tl::kStride;
-      const char* tv = lv + (kw * KS + i) * 32 * Tl::kStride;
-      f32x16 s = zero16(), dp = zero16();                             // rows = keys, column = this lane's packed row
+      if (!(uint32_t)(bits >> (32 * i))) continue;                  // (uniform over the wave)
+      const char* tk = lk + i * 32 * Tl::kStride;
+      const char* tv = lv + i * 32 * Tl::kStride;
+      f32x16 s = zero16(), dp = zero16();                           // rows = keys, column = this lane's packed row
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(tk, st, lane), qf[st], s);
 #pragma unroll
@@ -260,46 +275,225 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
       mma_tr<DP>(dq, tk, s, lane, T());
     }
   }
+  if (live) write_dq<T>(B, b, hk, row, dq, A.a.scale / sc, 0, 1, lane);
+}
+
+// ---- up to 32 rows: KW waves over different keys, everything in one pass ---------------------------------------------------------
+// The rows' queries and upstream gradients lie in LDS for all waves, with their log-sums and D (computed here: all rows of the head
+// group are in the tile, and so is the largest |dO|).  A wave's 32 keys meet all rows at once, so their dK and dV are final and
+// leave at once; dQ is added up over the keys.  Its product needs the score gradients transposed: through LDS, 4 KB a wave.
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void k_attn_few_bwd(BwdArgs B) {
+  const Args& A = B.f;
+  typedef Tile<T, DP> Tl;
+  constexpr int NT = Tl::kNT, kScr = 36;           // floats of a scratch row: 16-byte aligned, spread over the banks
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, kw = tid >> 6, col = lane & 31, h4 = (lane >> 5) * 4;
+  char* lq = lds;
+  char* lg = lq + Tl::template bytes<32>();
+  float* stat = reinterpret_cast<float*>(lg + Tl::template bytes<32>());        // [lse, D][32], largest |dO|
+  char* own = reinterpret_cast<char*>(stat + 68) + kw * (Tl::template bytes<32>() + 32 * kScr * 4);
+  char* lk = own;
+  float* scr = reinterpret_cast<float*>(own + Tl::template bytes<32>());
+  const FewWork f = few_work<KW>(A, kw);
+  if (!f.any) return;
+  const int dhb = A.a.Dh * A.es;
+  const Side ks = k_side(A, A.a.k, f.b, f.hk), vs = k_side(A, A.a.v, f.b, f.hk);
+  const Side qs = q_side(A, A.a.q, f.b, f.hk), gs = q_side(A, B.g_o, f.b, f.hk);
+  const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)f.b * A.a.mask_stride : nullptr;
+
+  WaveStage<T, DP> sk;
+  Frag<T> vf[Tl::kSteps];
+  bool there = false;
+  const auto fetch_v = [&](int t) {
+    const int key = t * 32 + col;
+    const char* vr = vs.row(key < f.n ? key : 0, 1);
+#pragma unroll
+    for (int s = 0; s < Tl::kSteps; ++s) vf[s] = Tl::gfrag(vr, s, lane, dhb, key < f.n);
+    there = key < f.n && (!mask || mask[key]);
+  };
+  if (f.t0 < f.t1) {
+    sk.fetch(ks, 1, f.t0 * 32, f.n, dhb, lane);
+    fetch_v(f.t0);
+  }
+  {                                                                 // the rows
+    constexpr int per = 2 * KW;                                     // threads of a row
+    const int r = tid / per, sub = tid % per;
+    const bool live = r < A.rows;
+    const char* qr = qs.row(live ? r : 0, A.G);
+    const char* gr = gs.row(live ? r : 0, A.G);
+    const char* orow = q_side(A, A.a.o, f.b, f.hk).row(live ? r : 0, A.G);
+    const char* lo = lo_row<T>(A, f.b, f.hk, live ? r : 0);
+    float d = 0.f, top = 0.f;
+    for (int c = sub * 16; c < Tl::kRowBytes; c += per * 16) {
+      uint4 q = make_uint4(0, 0, 0, 0), g = q;
+      if (live && c < dhb) {
+        q = *reinterpret_cast<const uint4*>(qr + c);
+        g = *reinterpret_cast<const uint4*>(gr + c);
+        float x[Vec16<T>::N], y[Vec16<T>::N], z[Vec16<T>::N];
+        load_vec(reinterpret_cast<const T*>(orow + c), x);
+        load_vec(reinterpret_cast<const T*>(gr + c), y);
+        if (lo) load_vec(reinterpret_cast<const T*>(lo + c), z);
+#pragma unroll
+        for (int i = 0; i < Vec16<T>::N; ++i) {
+          d += (lo ? x[i] + z[i] : x[i]) * y[i];
+          top = fmaxf(top, fabsf(y[i]));
+        }
+      }
+      *reinterpret_cast<uint4*>(lq + r * Tl::kStride + c) = q;
+      *reinterpret_cast<uint4*>(lg + r * Tl::kStride + c) = g;
+    }
+#pragma unroll
+    for (int o = 1; o < per; o <<= 1) { d += __shfl_xor(d, o); top = fmaxf(top, __shfl_xor(top, o)); }
+    if (sub == 0) {
+      stat[r] = live ? A.a.lse[row_index(A, f.b, f.hk, r)] : INFINITY;
+      stat[32 + r] = d;
+    }
+    if (Grad16<T>::on) {
+      if (tid == 0) stat[64] = 0.f;
+      __syncthreads();
+      if (sub == 0) atomicMax(reinterpret_cast<int*>(stat + 64), __float_as_int(top));       // (not negative: ordered as integers)
+    }
+  }
+  __syncthreads();
+  const float sc = Grad16<T>::on ? grad_scale(__float_as_uint(stat[64])) : 1.f, fac = A.a.scale / sc;
+  f32x16 dq[NT], acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) dq[t] = zero16();
+  const auto out_row = [&](const dvgr_attn_view& v, int key) { return const_cast<char*>(k_side(A, v, f.b, f.hk).row(key, 1)); };
+  const auto leave = [&](const dvgr_attn_view& v, int key, float x) {
+    if (key >= A.a.Lk) return;
+    char* out = out_row(v, key);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * t + 8 * g + h4;
+        if (d < A.a.Dh) store4<T>(out + d * sizeof(T), acc[t][4 * g] * x, acc[t][4 * g + 1] * x, acc[t][4 * g + 2] * x, acc[t][4 * g + 3] * x);
+      }
+  };
+  int t = f.t0;
+  for (; t < f.t1; t += KW) {
+    const uint32_t bits = (uint32_t)__ballot(there);
+    const bool here = there;
+    wave_order();
+    sk.put(lk, bits, lane);
+    wave_order();
+    f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
+#pragma unroll
+    for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(lg, st, lane), vf[st], dp);
+    if (t + KW < f.t1) {
+      sk.fetch(ks, 1, (t + KW) * 32, f.n, dhb, lane);
+      fetch_v(t + KW);
+    }
+#pragma unroll
+    for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lq, st, lane), Tl::frag(lk, st, lane), s);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 e = *reinterpret_cast<const float4*>(stat + 8 * g + h4), d = *reinterpret_cast<const float4*>(stat + 32 + 8 * g + h4);
+      const float ee[4] = {e.x, e.y, e.z, e.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * g + j;
+        const float p = here ? exp2_fast(fmaf(s[r], A.c, -ee[j])) : 0.f;
+        s[r] = p;
+        dp[r] = here ? grad16<T>(p * (dp[r] - dd[j]), sc) : 0.f;
+        scr[(8 * g + h4 + j) * kScr + col] = dp[r];
+      }
+    }
+    wave_order();
+    if (B.g_k.p) {
+      const int key = t * 32 + col;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) acc[u] = zero16();
+      mma_tr<DP>(acc, lg, s, lane, T());
+      leave(B.g_v, key, 1.f);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) acc[u] = zero16();
+      mma_tr<DP>(acc, lq, dp, lane, T());
+      leave(B.g_k, key, fac);
+    }
+    if (B.g_q.p) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {                                 // rows = keys, column = this lane's packed row
+        const float4 x = *reinterpret_cast<const float4*>(scr + col * kScr + 8 * g + h4);
+        s[4 * g] = x.x; s[4 * g + 1] = x.y; s[4 * g + 2] = x.z; s[4 * g + 3] = x.w;
+      }
+      mma_tr<DP>(dq, lk, s, lane, T());
+    }
+  }
+  if (B.g_k.p) {                                                    // keys behind the sample's last tile
+    const int tiles = (A.a.Lk + 31) / 32, per = A.tiles_per_split * KW, t2 = (f.split + 1) * per < tiles ? (f.split + 1) * per : tiles;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[u] = zero16();
+    for (; t < t2; t += KW) { leave(B.g_v, t * 32 + col, 1.f); leave(B.g_k, t * 32 + col, 1.f); }
+  }
+  if (!B.g_q.p) return;
   if (KW > 1) {
     float* lo = reinterpret_cast<float*>(lds);
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) lo[((wave * NT + t) * 16 + r) * 64 + lane] = dq[t][r];
+      for (int r = 0; r < 16; ++r) lo[((kw * NT + u) * 16 + r) * 64 + lane] = dq[u][r];
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t % KW != kw) continue;
+    for (int u = 0; u < NT; ++u) {
+      if (u % KW != kw) continue;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float a = 0.f;
 #pragma unroll
-        for (int k = 0; k < KW; ++k) a += lo[(((qw * KW + k) * NT + t) * 16 + r) * 64 + lane];
-        dq[t][r] = a;
+        for (int k = 0; k < KW; ++k) a += lo[((k * NT + u) * 16 + r) * 64 + lane];
+        dq[u][r] = a;
       }
     }
   }
-  if (!live) return;
-  const float f = A.a.scale / sc;
-  char* out = const_cast<char*>(q_side(A, B.g_q, b, hk).row(row, A.G));
+  if (col >= A.rows) return;
+  if (A.splits == 1) { write_dq<T>(B, f.b, f.hk, col, dq, fac, kw, KW, lane); return; }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (KW > 1 && t % KW != kw) continue;
+  for (int u = 0; u < NT; ++u) {
+    if (u % KW != kw) continue;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int d = 32 * t + 8 * g + (lane >> 5) * 4;
-      if (d < A.a.Dh) store4<T>(out + d * sizeof(T), dq[t][4 * g] * f, dq[t][4 * g + 1] * f, dq[t][4 * g + 2] * f, dq[t][4 * g + 3] * f);
+      const int d = 32 * u + 8 * g + h4;
+      if (d < A.a.Dh)
+        *reinterpret_cast<float4*>(A.part_o + (f.w * A.rows + col) * A.a.Dh + d) =
+            make_float4(dq[u][4 * g] * fac, dq[u][4 * g + 1] * fac, dq[u][4 * g + 2] * fac, dq[u][4 * g + 3] * fac);
     }
   }
 }
 
+// dQ from the shares of the keys: a workgroup per packed row, its waves take every fourth share, added in the waves' order
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dq_join(BwdArgs B) {
+  const Args& A = B.f;
+  __shared__ float sh[4][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = 2 * lane;
+  const int row = (int)(blockIdx.x % A.rows), hk = (int)(blockIdx.x / A.rows % A.a.Hk), b = (int)(blockIdx.x / A.rows / A.a.Hk);
+  const float* at = A.part_o + (((int64_t)b * A.a.Hk + hk) * A.splits * A.rows + row) * A.a.Dh + d;
+  float x = 0.f, y = 0.f;
+  if (d < A.a.Dh)
+#pragma unroll 8
+    for (int s = wave; s < A.splits; s += 4) {
+      const float2 p = *reinterpret_cast<const float2*>(at + (int64_t)s * A.rows * A.a.Dh);
+      x += p.x; y += p.y;
+    }
+  sh[wave][d] = x; sh[wave][d + 1] = y;
+  __syncthreads();
+  if (wave || d >= A.a.Dh) return;
+  T* out = (T*)const_cast<char*>(q_side(A, B.g_q, b, hk).row(row, A.G));
+  out[d] = (T)(sh[0][d] + sh[1][d] + sh[2][d] + sh[3][d]);
+  out[d + 1] = (T)(sh[0][d + 1] + sh[1][d + 1] + sh[2][d + 1] + sh[3][d + 1]);
+}
+
 size_t delta_bytes(const dvgr_attn_problem& a) { return ((size_t)a.B * a.H * a.Lq * sizeof(float) + 255) / 256 * 256; }
 
-template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t work, size_t bytes, const BwdArgs& B, hipStream_t st) {
+template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t work, int threads, size_t bytes, const BwdArgs& B,
+                                hipStream_t st) {
   const int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
   if (e) return e;
-  DVGR_LAUNCH(kern, dim3(xcd_grid(work)), dim3(kThreads), bytes, st, B);
+  DVGR_LAUNCH(kern, dim3(xcd_grid(work)), dim3(threads), bytes, st, B);
   return (int)hipGetLastError();
 }
 size_t join_bytes(int waves, int NT) { return waves > 1 ? (size_t)kWaves * NT * 16 * 64 * sizeof(float) : 0; }
@@ -309,46 +503,76 @@ template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdAr
   static std::atomic<uint32_t> asked{0};
   size_t bytes = 2 * Tl::template bytes<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float);
   if (bytes < join_bytes(RW, Tl::kNT)) bytes = join_bytes(RW, Tl::kNT);
-  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), bytes, B, st);
+  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), kThreads, bytes, B, st);
 }
-template <typename T, int DP, int QW, int KW, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
+template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
+  static std::atomic<uint32_t> asked{0};
+  return launch(k_attn_dq<T, DP, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.rows + kWaves * 32 - 1) / (kWaves * 32)), kThreads,
+                2 * Tile<T, DP>::template bytes<KS * 32>(), B, st);
+}
+template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytes<KW * KS * 32>();
-  if (bytes < join_bytes(KW, Tl::kNT)) bytes = join_bytes(KW, Tl::kNT);
-  return launch(k_attn_dq<T, DP, QW, KW, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.rows + QW * 32 - 1) / (QW * 32)), bytes, B, st);
+  size_t bytes = 2 * Tl::template bytes<32>() + 68 * sizeof(float) + KW * (Tl::template bytes<32>() + 32 * 36 * sizeof(float));
+  const size_t join = KW > 1 ? (size_t)KW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
+  if (bytes < join) bytes = join;
+  const int64_t units = (int64_t)B.f.a.B * B.f.a.Hk;
+  const int e = launch(k_attn_few_bwd<T, DP, KW>, asked, units * B.f.splits, 64 * KW, bytes, B, st);
+  if (e || B.f.splits == 1 || !B.g_q.p || !B.f.rows) return e;
+  DVGR_LAUNCH((k_attn_dq_join<T>), dim3((unsigned)(units * B.f.rows)), dim3(256), 0, st, B);
+  return (int)hipGetLastError();
 }
 
-// Few keys (or few rows): the four waves share them and go over different rows (keys).
-template <typename T, int DP> int launch_dp(const BwdArgs& B, hipStream_t st) {
+// Few keys for many rows: the four waves share them and go over different rows.
+template <typename T, int DP> int launch_many(const BwdArgs& B, hipStream_t st) {
   constexpr int S = sizeof(T) == 4 ? 1 : 2;                         // a turn of the shared arrangement: 32 rows of fp32, 64 of two bytes
   if (B.f.a.Lk && B.g_k.p) {
     const int e = B.f.a.Lk <= 32 ? launch_dkv<T, DP, 1, 4, 1>(B, st) : launch_dkv<T, DP, 4, 1, S>(B, st);
     if (e) return e;
   }
-  if (!B.f.rows || !B.g_q.p) return 0;
-  return B.f.rows <= 32 ? launch_dq<T, DP, 1, 4, 1>(B, st) : launch_dq<T, DP, 4, 1, S>(B, st);
+  return B.g_q.p ? launch_dq<T, DP, S>(B, st) : 0;
+}
+template <typename T, int DP> int launch_dp(const BwdArgs& B, int KW, hipStream_t st) {
+  return KW == 1 ? launch_few<T, DP, 1>(B, st) : KW == 4 ? launch_few<T, DP, 4>(B, st) : launch_many<T, DP>(B, st);
 }
 
-template <typename T> int launch_t(const BwdArgs& B, hipStream_t st) {
-  const int64_t rows = (int64_t)B.f.a.B * B.f.a.Hk * B.f.rows, groups = (int64_t)B.f.a.B * B.f.a.Hk;
-  if (Grad16<T>::on) DVGR_LAUNCH(k_attn_clear, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, B.top, groups);
-  if (rows) DVGR_LAUNCH((k_attn_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, B);
-  const int e = (int)hipGetLastError();
-  if (e) return e;
-  if (B.f.a.Dh <= 32) return launch_dp<T, 32>(B, st);
-  if (B.f.a.Dh <= 64) return launch_dp<T, 64>(B, st);
-  if (B.f.a.Dh <= 96) return launch_dp<T, 96>(B, st);
-  return launch_dp<T, 128>(B, st);
+template <typename T> int launch_t(const BwdArgs& B, int KW, hipStream_t st) {
+  if (!KW) {
+    const int64_t rows = (int64_t)B.f.a.B * B.f.a.Hk * B.f.rows, groups = (int64_t)B.f.a.B * B.f.a.Hk;
+    if (Grad16<T>::on) DVGR_LAUNCH(k_attn_clear, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, B.top, groups);
+    DVGR_LAUNCH((k_attn_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, B);
+    const int e = (int)hipGetLastError();
+    if (e) return e;
+  }
+  if (B.f.a.Dh <= 32) return launch_dp<T, 32>(B, KW, st);
+  if (B.f.a.Dh <= 64) return launch_dp<T, 64>(B, KW, st);
+  if (B.f.a.Dh <= 96) return launch_dp<T, 96>(B, KW, st);
+  return launch_dp<T, 128>(B, KW, st);
 }
 
 }  // namespace
 
-size_t backward_bytes(const dvgr_attn_problem& a) { return delta_bytes(a) + (a.elem == DVGR_ELEM_F16 ? (size_t)a.B * a.Hk * sizeof(uint32_t) : 0); }
+size_t backward_bytes(const dvgr_attn_problem& a) {
+  const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk);
+  if (rows <= 32) {
+    const FewPlan p = few_plan(a);
+    return p.splits > 1 ? (size_t)a.B * a.Hk * p.splits * rows * a.Dh * sizeof(float) : 0;
+  }
+  return delta_bytes(a) + (a.elem == DVGR_ELEM_F16 ? (size_t)a.B * a.Hk * sizeof(uint32_t) : 0);
+}
 
 int launch_backward(const Args& A, const dvgr_attn_grads& g, void* ws, hipStream_t st) {
-  BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, (float*)ws, (uint32_t*)((char*)ws + delta_bytes(A.a))};
-  return A.a.elem == DVGR_ELEM_F32 ? launch_t<float>(B, st) : A.a.elem == DVGR_ELEM_BF16 ? launch_t<bf16_t>(B, st) : launch_t<f16_t>(B, st);
+  BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, nullptr, nullptr};
+  int KW = 0;
+  if (A.rows <= 32) {
+    const FewPlan p = few_plan(A.a);
+    B.f.splits = p.splits; B.f.tiles_per_split = p.tiles_per_split; B.f.part_o = (float*)ws;
+    KW = p.KW;
+  } else {
+    B.delta = (float*)ws;
+    B.top = (uint32_t*)((char*)ws + delta_bytes(A.a));
+  }
+  return A.a.elem == DVGR_ELEM_F32 ? launch_t<float>(B, KW, st) : A.a.elem == DVGR_ELEM_BF16 ? launch_t<bf16_t>(B, KW, st) : launch_t<f16_t>(B, KW, st);
 }
 
 }  // namespace attn

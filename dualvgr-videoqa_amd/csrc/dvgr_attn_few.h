@@ -1,0 +1,79 @@
+// dvgr_attn_few.h -- attention where one 32-row tile holds all packed rows of a key head (a word over a video, a question over its
+// frames): bound by the keys' and values' memory, so the waves of a workgroup go over different keys at their own pace.  A wave
+// reads its 32 keys straight into the matrix unit's operands where a tile is used along its rows, and through LDS of its own where it
+// is used across them; nothing waits for another wave before the end.
+#pragma once
+#include "dvgr_attn.h"
+
+namespace dvgr {
+namespace attn {
+
+// 32 rows of a tensor on their way to a wave's own LDS
+template <typename T, int DP> struct WaveStage {
+  typedef Tile<T, DP> Tl;
+  static constexpr int N = Tl::kChunks / 2;
+  uint4 v[N];
+  __device__ __forceinline__ void fetch(const Side& s, int G, int r0, int end, int dh_bytes, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = lane + i * 64, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r, G) + c);
+    }
+  }
+  // rows without a bit are zeros, whatever was read
+  __device__ __forceinline__ void put(char* lds, uint32_t bits, int lane) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = lane + i * 64, r = e / Tl::kChunks;
+      *reinterpret_cast<uint4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// LDS operations of one wave complete in order; this keeps the compiler from moving them across each other
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// where a wave of a workgroup stands: key head, share of the keys, its first 32-key tile (it goes on in steps of KW)
+struct FewWork {
+  int b, hk, split, n, t0, t1;
+  int64_t w;
+  bool any;
+};
+template <int KW> __device__ __forceinline__ FewWork few_work(const Args& A, int kw) {
+  FewWork f{};
+  f.w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits);
+  f.any = f.w >= 0;
+  if (!f.any) return f;
+  f.split = (int)(f.w % A.splits);
+  f.hk = (int)(f.w / A.splits % A.a.Hk);
+  f.b = (int)(f.w / A.splits / A.a.Hk);
+  f.n = key_count(A, f.b);
+  const int tiles = (f.n + 31) / 32, per = A.tiles_per_split * KW;
+  f.t0 = f.split * per + kw;
+  f.t1 = (f.split + 1) * per < tiles ? (f.split + 1) * per : tiles;
+  return f;
+}
+
+// Turns of KW x 32 keys and shares of the keys for the few-rows kernels.  Up to 64 keys one wave does it all; otherwise four.  The keys are
+// split over workgroups while there are fewer than two for each compute unit, in shares of at least two turns.
+struct FewPlan { int KW, splits, tiles_per_split; };
+inline FewPlan few_plan(const dvgr_attn_problem& a) {
+  FewPlan p{};
+  p.KW = a.Lk <= 64 ? 1 : 4;
+  const int64_t turns = ((int64_t)a.Lk + p.KW * 32 - 1) / (p.KW * 32), units = (int64_t)a.B * a.Hk;
+  int64_t s = units ? 512 / units : 1;
+  if (s > turns / 2) s = turns / 2;
+  if (s < 1) s = 1;
+  p.tiles_per_split = (int)((turns + s - 1) / s);
+  if (p.tiles_per_split < 1) p.tiles_per_split = 1;
+  p.splits = turns ? (int)((turns + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
+  return p;
+}
+
+}  // namespace attn
+}  // namespace dvgr

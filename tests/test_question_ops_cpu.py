@@ -97,11 +97,11 @@ def test_attention_refusals():
     assert need > 0 and lib.dvgr_attn_forward(C.byref(long), None, 0, None) == E_NULL
     assert lib.dvgr_attn_forward(C.byref(long), A, need - 1, None) == E_WORKSPACE and lib.dvgr_attn_forward(C.byref(long), A + 4, need, None) == E_ALIGN
     g = lambda **kw: L.AttnGrads(**{n: kw.get(n, L.AttnView(A, 1024, 64, 16)) for n in ("g_o", "g_q", "g_k", "g_v")})  # noqa: E731
-    p = problem()
+    p = problem(Lq=40)
     need = lib.dvgr_attn_backward_workspace_bytes(C.byref(p))
     back = lambda q, gr, ws=A, n=need: lib.dvgr_attn_backward(C.byref(q), C.byref(gr) if gr else None, ws, n, None)  # noqa: E731
     assert need > 0 and back(p, None) == E_NULL and back(p, g(g_o=none)) == E_NULL and back(p, g(g_k=none)) == E_NULL
-    assert back(problem(lse=None), g()) == E_NULL and back(p, g(), None) == E_NULL
+    assert back(problem(Lq=40, lse=None), g()) == E_NULL and back(p, g(), None) == E_NULL
     assert back(p, g(), A, need - 1) == E_WORKSPACE and back(p, g(), A + 8) == E_ALIGN
     for n in ("g_o", "g_q", "g_k", "g_v"):
         assert back(p, g(**{n: odd})) == E_ALIGN
