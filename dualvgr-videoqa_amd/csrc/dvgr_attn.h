@@ -168,6 +168,7 @@ struct Args {
   int es;
   int splits, tiles_per_split;      // the keys of a sample in shares of whole tiles
   float c;                          // scale * log2 e
+  bool stream;                      // keys and values are read past the caches
   float *part_o, *part_ml;          // splits > 1: (work, rows of the tile, Dh) and (.., 2)
 };
 __device__ __forceinline__ Side q_side(const Args& A, const dvgr_attn_view& v, int b, int hk) {

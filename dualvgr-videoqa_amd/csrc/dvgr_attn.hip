@@ -124,13 +124,16 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Args A) {
 }
 
 // ---- up to 32 rows: KW waves over different keys -----------------------------------------------------------------------------------
+// (Two waves of a SIMD, in two-byte types, keep twice the loads in flight: the queries are read from LDS for it.)
 template <typename T, int DP, int KW>
-__global__ __launch_bounds__(64 * KW) void k_attn_few_fwd(Args A) {
+__global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_fwd(Args A) {
   typedef Tile<T, DP> Tl;
   constexpr int NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, kw = threadIdx.x >> 6;
-  char* lv = lds + kw * Tl::template bytes<32>();
+  char* lq = lds;
+  char* lk = lds + (1 + kw * 2) * Tl::template bytes<32>();
+  char* lv = lk + Tl::template bytes<32>();
   const FewWork f = few_work<KW>(A, kw);
   if (!f.any) return;
   const int dhb = A.a.Dh * A.es, row = lane & 31;
@@ -138,42 +141,37 @@ __global__ __launch_bounds__(64 * KW) void k_attn_few_fwd(Args A) {
   const Side ks = k_side(A, A.a.k, f.b, f.hk), vs = k_side(A, A.a.v, f.b, f.hk);
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)f.b * A.a.mask_stride : nullptr;
 
-  Frag<T> qf[Tl::kSteps], kf[Tl::kSteps];
-  {
-    const char* qr = q_side(A, A.a.q, f.b, f.hk).row(live ? row : 0, A.G);
-#pragma unroll
-    for (int s = 0; s < Tl::kSteps; ++s) qf[s] = Tl::gfrag(qr, s, lane, dhb, live);
-  }
   f32x16 o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = zero16();
   float m = -INFINITY, l = 0.f;
-  WaveStage<T, DP> sv;
+  WaveStage<T, DP> sk, sv;
   bool there = false;
-  const auto fetch_k = [&](int t) {
+  const auto fetch = [&](int t) {
+    sk.fetch(ks, t * 32, f.n, dhb, A.stream, lane);
+    sv.fetch(vs, t * 32, f.n, dhb, A.stream, lane);
     const int key = t * 32 + (lane & 31);
-    const char* kr = ks.row(key < f.n ? key : 0, 1);
-#pragma unroll
-    for (int s = 0; s < Tl::kSteps; ++s) kf[s] = Tl::gfrag(kr, s, lane, dhb, key < f.n);
     there = key < f.n && (!mask || mask[key]);
   };
-  if (f.t0 < f.t1) {
-    sv.fetch(vs, 1, f.t0 * 32, f.n, dhb, lane);
-    fetch_k(f.t0);
+  if (f.t0 < f.t1) fetch(f.t0);
+  for (int e = threadIdx.x; e < 32 * Tl::kChunks; e += 64 * KW) {
+    const int r = e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < A.rows && c < dhb) x = *reinterpret_cast<const uint4*>(q_side(A, A.a.q, f.b, f.hk).row(r, A.G) + c);
+    *reinterpret_cast<uint4*>(lq + r * Tl::kStride + c) = x;
   }
+  __syncthreads();
   for (int t = f.t0; t < f.t1; t += KW) {
     const uint32_t bits = (uint32_t)__ballot(there);                // (lanes 32 + j say the same as lanes j)
-    f32x16 s = zero16();
-#pragma unroll
-    for (int st = 0; st < Tl::kSteps; ++st) s = mma(kf[st], qf[st], s);
     wave_order();
+    sk.put(lk, bits, lane);
     sv.put(lv, bits, lane);
     wave_order();
-    if (t + KW < f.t1) {
-      sv.fetch(vs, 1, (t + KW) * 32, f.n, dhb, lane);
-      fetch_k(t + KW);
-    }
+    if (t + KW < f.t1) fetch(t + KW);
     if (!bits) continue;
+    f32x16 s = zero16();
+#pragma unroll
+    for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lk, st, lane), Tl::frag(lq, st, lane), s);
     softmax_tile(s, bits, A.c, m, l, o, lane);
     mma_tr<DP>(o, lv, s, lane, T());
   }
@@ -228,37 +226,53 @@ __global__ __launch_bounds__(64 * KW) void k_attn_few_fwd(Args A) {
   write_row<T>(A, f.b, f.hk, row, o, m, l, kw, KW, kw == 0, lane);
 }
 
-// join of the shares of the keys: a workgroup per packed row, its waves take every fourth share, added in the waves' order
+// Join of the shares of the keys: a workgroup per packed row, its waves take every fourth share, kAtOnce of them in flight, and are added
+// in order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_join(Args A) {
+  constexpr int kAtOnce = 8;
   __shared__ float sh[4][132];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = 2 * lane;
   const int row = (int)(blockIdx.x % A.rows), hk = (int)(blockIdx.x / A.rows % A.a.Hk), b = (int)(blockIdx.x / A.rows / A.a.Hk);
   const int64_t at0 = ((int64_t)b * A.a.Hk + hk) * A.splits * A.rows + row;
-  float m = -INFINITY;
-  for (int s = lane; s < A.splits; s += 64) m = fmaxf(m, A.part_ml[2 * (at0 + (int64_t)s * A.rows)]);
-  m = wave_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, x = 0.f, y = 0.f;
-  const int d = 2 * lane;
-#pragma unroll 8
-  for (int s = wave; s < A.splits; s += 4) {
-    const int64_t at = at0 + (int64_t)s * A.rows;
-    const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * at);
-    const float f = exp2_fast(ml.x - ref);
-    l += ml.y * f;
-    if (d < A.a.Dh) {
-      const float2 p = *reinterpret_cast<const float2*>(A.part_o + at * A.a.Dh + d);
-      x += p.x * f; y += p.y * f;
+  float m = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+  for (int s0 = wave; s0 < A.splits; s0 += 4 * kAtOnce) {
+    float2 ml[kAtOnce], o[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int s = s0 + 4 * i;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      o[i] = make_float2(0.f, 0.f);
+      if (s < A.splits) {
+        ml[i] = *reinterpret_cast<const float2*>(A.part_ml + 2 * (at0 + (int64_t)s * A.rows));
+        if (d < A.a.Dh) o[i] = *reinterpret_cast<const float2*>(A.part_o + (at0 + (int64_t)s * A.rows) * A.a.Dh + d);
+      }
     }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) mn = fmaxf(mn, ml[i].x);
+    const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_fast(m - ref);
+    l *= f0; x *= f0; y *= f0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float f = exp2_fast(ml[i].x - ref);
+      l += ml[i].y * f;
+      x += o[i].x * f; y += o[i].y * f;
+    }
+    m = mn;
   }
   sh[wave][d] = x; sh[wave][d + 1] = y;
-  if (lane == 0) sh[wave][128] = l;
+  if (lane == 0) { sh[wave][128] = l; sh[wave][129] = m; }
   __syncthreads();
   if (wave) return;
+  m = fmaxf(fmaxf(sh[0][129], sh[1][129]), fmaxf(sh[2][129], sh[3][129]));
+  const float ref = m == -INFINITY ? 0.f : m;
   x = y = l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) { x += sh[w][d]; y += sh[w][d + 1]; l += sh[w][128]; }
+  for (int w = 0; w < 4; ++w) {
+    const float f = exp2_fast(sh[w][129] - ref);
+    x += sh[w][d] * f; y += sh[w][d + 1] * f; l += sh[w][128] * f;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   x *= inv; y *= inv;
   T* out = (T*)q_side(A, A.a.o, b, hk).row(row, A.G);
@@ -281,7 +295,7 @@ template <typename T, int DP, int KS> int launch_many(const Args& A, hipStream_t
 }
 template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t st) {
   typedef Tile<T, DP> Tl;
-  size_t bytes = KW * Tl::template bytes<32>();
+  size_t bytes = (1 + 2 * KW) * Tl::template bytes<32>();
   const size_t join = KW > 1 ? (size_t)(KW * 64 + KW * Tl::kNT * 16 * 64) * sizeof(float) : 0;
   bytes = bytes > join ? bytes : join;
   static std::atomic<uint32_t> asked{0};
@@ -297,6 +311,8 @@ template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t 
 // (two-byte types take 64 keys a turn, fp32 32: the same bytes)
 template <typename T, int DP> int launch_dp(const Args& A, int KW, hipStream_t st) {
   if (A.rows > 32) return launch_many<T, DP, sizeof(T) == 4 ? 1 : 2>(A, st);
+  if constexpr (sizeof(T) == 2)
+    if (KW == 8) return launch_few<T, DP, 8>(A, st);
   return KW == 1 ? launch_few<T, DP, 1>(A, st) : launch_few<T, DP, 4>(A, st);
 }
 template <typename T> int launch_t(const Args& A, int KW, hipStream_t st) {
@@ -311,7 +327,7 @@ Parts parts(const dvgr_attn_problem& a) {
   Parts p{};
   const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk);
   if (rows > 32) return p;
-  p.few = few_plan(a);
+  p.few = few_plan(a, true);
   if (p.few.splits > 1) {
     p.o_bytes = (size_t)a.B * a.Hk * p.few.splits * rows * a.Dh * sizeof(float);          // (rows of 8 floats at least: 16-byte aligned)
     p.ml_bytes = (size_t)a.B * a.Hk * p.few.splits * rows * 2 * sizeof(float);
@@ -392,6 +408,8 @@ int dvgr_attn_forward(const dvgr_attn_problem* a, void* workspace, size_t worksp
     A.splits = p.few.splits;
     A.tiles_per_split = p.few.tiles_per_split;
   }
+  // One word at a time over states that no cache holds (256 MB): 63 -> 51 us for 268 MB; smaller ones stay where the next word finds them.
+  A.stream = !a->lse && (double)a->B * a->Lk * a->Hk * a->Dh * A.es * 2 > 256e6;
   A.part_o = (float*)workspace;
   A.part_ml = (float*)((char*)workspace + p.o_bytes);
   hipStream_t st = (hipStream_t)stream;

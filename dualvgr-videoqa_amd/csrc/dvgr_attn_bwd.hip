@@ -281,20 +281,31 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
 // ---- up to 32 rows: KW waves over different keys, everything in one pass ---------------------------------------------------------
 // The rows' queries and upstream gradients lie in LDS for all waves, with their log-sums and D (computed here: all rows of the head
 // group are in the tile, and so is the largest |dO|).  A wave's 32 keys meet all rows at once, so their dK and dV are final and
-// leave at once; dQ is added up over the keys.  Its product needs the score gradients transposed: through LDS, 4 KB a wave.
+// leave at once; dQ is added up over the keys.  Its product needs the score gradients transposed, through LDS; two-byte dK and dV leave
+// through LDS too, whole rows at a time and past the caches.  The values' tile is free for both once dP is there.  64 x 15 words over
+// 1024 frames (8 heads of 96, bf16): 84 us; gradients stored in 8-byte pieces 123, through the caches 95 (and the forward of the next
+// step 55 instead of 34, while their lines are written back).
+template <typename T, int DP> struct FewLds {
+  static constexpr bool kOut = sizeof(T) == 2;                      // fp32: values go straight to operands, gradients leave in 16-byte pieces
+  static constexpr int kScr = 36;                                   // floats of a scratch row: 16-byte aligned, spread over the banks
+  static constexpr int kTile = Tile<T, DP>::template bytes<32>(), kScrBytes = 32 * kScr * 4;
+  static constexpr int kOwn = kTile + (kOut && kTile > kScrBytes ? kTile : kScrBytes);
+  static constexpr int kBytes(int KW) { return 2 * kTile + 68 * 4 + KW * kOwn; }
+};
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void k_attn_few_bwd(BwdArgs B) {
   const Args& A = B.f;
   typedef Tile<T, DP> Tl;
-  constexpr int NT = Tl::kNT, kScr = 36;           // floats of a scratch row: 16-byte aligned, spread over the banks
+  constexpr int NT = Tl::kNT, kScr = FewLds<T, DP>::kScr;
+  constexpr bool kOut = FewLds<T, DP>::kOut;
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, kw = tid >> 6, col = lane & 31, h4 = (lane >> 5) * 4;
   char* lq = lds;
   char* lg = lq + Tl::template bytes<32>();
   float* stat = reinterpret_cast<float*>(lg + Tl::template bytes<32>());        // [lse, D][32], largest |dO|
-  char* own = reinterpret_cast<char*>(stat + 68) + kw * (Tl::template bytes<32>() + 32 * kScr * 4);
-  char* lk = own;
-  float* scr = reinterpret_cast<float*>(own + Tl::template bytes<32>());
+  char* lk = reinterpret_cast<char*>(stat + 68) + kw * FewLds<T, DP>::kOwn;
+  char* lx = lk + FewLds<T, DP>::kTile;                              // values, then score gradients, then dV, then dK
+  float* scr = reinterpret_cast<float*>(lx);
   const FewWork f = few_work<KW>(A, kw);
   if (!f.any) return;
   const int dhb = A.a.Dh * A.es;
@@ -302,20 +313,21 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
   const Side qs = q_side(A, A.a.q, f.b, f.hk), gs = q_side(A, B.g_o, f.b, f.hk);
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)f.b * A.a.mask_stride : nullptr;
 
-  WaveStage<T, DP> sk;
-  Frag<T> vf[Tl::kSteps];
+  WaveStage<T, DP> sk, sv;
+  Frag<T> vf[kOut ? 1 : Tl::kSteps];
   bool there = false;
-  const auto fetch_v = [&](int t) {
+  const auto fetch = [&](int t) {
     const int key = t * 32 + col;
-    const char* vr = vs.row(key < f.n ? key : 0, 1);
+    sk.fetch(ks, t * 32, f.n, dhb, false, lane);
+    if constexpr (kOut) sv.fetch(vs, t * 32, f.n, dhb, false, lane);
+    else {
+      const char* vr = vs.row(key < f.n ? key : 0, 1);
 #pragma unroll
-    for (int s = 0; s < Tl::kSteps; ++s) vf[s] = Tl::gfrag(vr, s, lane, dhb, key < f.n);
+      for (int s = 0; s < Tl::kSteps; ++s) vf[s] = Tl::gfrag(vr, s, lane, dhb, key < f.n);
+    }
     there = key < f.n && (!mask || mask[key]);
   };
-  if (f.t0 < f.t1) {
-    sk.fetch(ks, 1, f.t0 * 32, f.n, dhb, lane);
-    fetch_v(f.t0);
-  }
+  if (f.t0 < f.t1) fetch(f.t0);
   {                                                                 // the rows
     constexpr int per = 2 * KW;                                     // threads of a row
     const int r = tid / per, sub = tid % per;
@@ -360,17 +372,35 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
   f32x16 dq[NT], acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) dq[t] = zero16();
-  const auto out_row = [&](const dvgr_attn_view& v, int key) { return const_cast<char*>(k_side(A, v, f.b, f.hk).row(key, 1)); };
-  const auto leave = [&](const dvgr_attn_view& v, int key, float x) {
-    if (key >= A.a.Lk) return;
-    char* out = out_row(v, key);
+  // acc, 32 keys of tile t, to their rows of a gradient
+  const auto leave = [&](const dvgr_attn_view& v, int t, float x) {
+    const Side to = k_side(A, v, f.b, f.hk);
+    if constexpr (kOut) {
+      wave_order();
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * t + 8 * g + h4;
-        if (d < A.a.Dh) store4<T>(out + d * sizeof(T), acc[t][4 * g] * x, acc[t][4 * g + 1] * x, acc[t][4 * g + 2] * x, acc[t][4 * g + 3] * x);
+        for (int g = 0; g < 4; ++g)
+          store4<T>(lx + col * Tl::kStride + (32 * u + 8 * g + h4) * sizeof(T), acc[u][4 * g] * x, acc[u][4 * g + 1] * x, acc[u][4 * g + 2] * x,
+                    acc[u][4 * g + 3] * x);
+      wave_order();
+#pragma unroll
+      for (int i = 0; i < Tl::kChunks / 2; ++i) {
+        const int e = lane + i * 64, key = t * 32 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
+        typedef typename WaveStage<T, DP>::u32x4 u32x4;
+        if (key < A.a.Lk && c < dhb)
+          stream_store(reinterpret_cast<u32x4*>(const_cast<char*>(to.row(key, 1)) + c), *reinterpret_cast<const u32x4*>(lx + (e / Tl::kChunks) * Tl::kStride + c));
       }
+    } else if (t * 32 + col < A.a.Lk) {
+      char* out = const_cast<char*>(to.row(t * 32 + col, 1));
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int d = 32 * u + 8 * g + h4;
+          if (d < A.a.Dh) store4<T>(out + d * sizeof(T), acc[u][4 * g] * x, acc[u][4 * g + 1] * x, acc[u][4 * g + 2] * x, acc[u][4 * g + 3] * x);
+        }
+    }
   };
   int t = f.t0;
   for (; t < f.t1; t += KW) {
@@ -378,16 +408,18 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
     const bool here = there;
     wave_order();
     sk.put(lk, bits, lane);
+    if constexpr (kOut) sv.put(lx, bits, lane);
     wave_order();
     f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
 #pragma unroll
-    for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(lg, st, lane), vf[st], dp);
-    if (t + KW < f.t1) {
-      sk.fetch(ks, 1, (t + KW) * 32, f.n, dhb, lane);
-      fetch_v(t + KW);
+    for (int st = 0; st < Tl::kSteps; ++st) {
+      if constexpr (kOut) dp = mma(Tl::frag(lg, st, lane), Tl::frag(lx, st, lane), dp);
+      else dp = mma(Tl::frag(lg, st, lane), vf[st], dp);
     }
+    if (t + KW < f.t1) fetch(t + KW);
 #pragma unroll
     for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lq, st, lane), Tl::frag(lk, st, lane), s);
+    wave_order();
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float4 e = *reinterpret_cast<const float4*>(stat + 8 * g + h4), d = *reinterpret_cast<const float4*>(stat + 32 + 8 * g + h4);
@@ -402,31 +434,31 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
       }
     }
     wave_order();
+    if (B.g_q.p) {
+      f32x16 x;                                                     // rows = keys, column = this lane's packed row
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 y = *reinterpret_cast<const float4*>(scr + col * kScr + 8 * g + h4);
+        x[4 * g] = y.x; x[4 * g + 1] = y.y; x[4 * g + 2] = y.z; x[4 * g + 3] = y.w;
+      }
+      mma_tr<DP>(dq, lk, x, lane, T());
+    }
     if (B.g_k.p) {
-      const int key = t * 32 + col;
 #pragma unroll
       for (int u = 0; u < NT; ++u) acc[u] = zero16();
       mma_tr<DP>(acc, lg, s, lane, T());
-      leave(B.g_v, key, 1.f);
+      leave(B.g_v, t, 1.f);
 #pragma unroll
       for (int u = 0; u < NT; ++u) acc[u] = zero16();
       mma_tr<DP>(acc, lq, dp, lane, T());
-      leave(B.g_k, key, fac);
-    }
-    if (B.g_q.p) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {                                 // rows = keys, column = this lane's packed row
-        const float4 x = *reinterpret_cast<const float4*>(scr + col * kScr + 8 * g + h4);
-        s[4 * g] = x.x; s[4 * g + 1] = x.y; s[4 * g + 2] = x.z; s[4 * g + 3] = x.w;
-      }
-      mma_tr<DP>(dq, lk, s, lane, T());
+      leave(B.g_k, t, fac);
     }
   }
   if (B.g_k.p) {                                                    // keys behind the sample's last tile
     const int tiles = (A.a.Lk + 31) / 32, per = A.tiles_per_split * KW, t2 = (f.split + 1) * per < tiles ? (f.split + 1) * per : tiles;
 #pragma unroll
     for (int u = 0; u < NT; ++u) acc[u] = zero16();
-    for (; t < t2; t += KW) { leave(B.g_v, t * 32 + col, 1.f); leave(B.g_k, t * 32 + col, 1.f); }
+    for (; t < t2; t += KW) { leave(B.g_v, t, 1.f); leave(B.g_k, t, 1.f); }
   }
   if (!B.g_q.p) return;
   if (KW > 1) {
@@ -513,7 +545,7 @@ template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_
 template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytes<32>() + 68 * sizeof(float) + KW * (Tl::template bytes<32>() + 32 * 36 * sizeof(float));
+  size_t bytes = FewLds<T, DP>::kBytes(KW);
   const size_t join = KW > 1 ? (size_t)KW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
   if (bytes < join) bytes = join;
   const int64_t units = (int64_t)B.f.a.B * B.f.a.Hk;
@@ -555,7 +587,7 @@ template <typename T> int launch_t(const BwdArgs& B, int KW, hipStream_t st) {
 size_t backward_bytes(const dvgr_attn_problem& a) {
   const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk);
   if (rows <= 32) {
-    const FewPlan p = few_plan(a);
+    const FewPlan p = few_plan(a, false);
     return p.splits > 1 ? (size_t)a.B * a.Hk * p.splits * rows * a.Dh * sizeof(float) : 0;
   }
   return delta_bytes(a) + (a.elem == DVGR_ELEM_F16 ? (size_t)a.B * a.Hk * sizeof(uint32_t) : 0);
@@ -565,7 +597,7 @@ int launch_backward(const Args& A, const dvgr_attn_grads& g, void* ws, hipStream
   BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, nullptr, nullptr};
   int KW = 0;
   if (A.rows <= 32) {
-    const FewPlan p = few_plan(A.a);
+    const FewPlan p = few_plan(A.a, false);
     B.f.splits = p.splits; B.f.tiles_per_split = p.tiles_per_split; B.f.part_o = (float*)ws;
     KW = p.KW;
   } else {

@@ -1,7 +1,7 @@
 // dvgr_attn_few.h -- attention where one 32-row tile holds all packed rows of a key head (a word over a video, a question over its
 // frames): bound by the keys' and values' memory, so the waves of a workgroup go over different keys at their own pace.  A wave
-// reads its 32 keys straight into the matrix unit's operands where a tile is used along its rows, and through LDS of its own where it
-// is used across them; nothing waits for another wave before the end.
+// reads its 32 keys a row at a time (whole lines; read straight as operands, 32 bytes of 32 rows each, they fell out of the cache
+// between the steps) into LDS of its own; nothing waits for another wave before the end.
 #pragma once
 #include "dvgr_attn.h"
 
@@ -12,21 +12,29 @@ namespace attn {
 template <typename T, int DP> struct WaveStage {
   typedef Tile<T, DP> Tl;
   static constexpr int N = Tl::kChunks / 2;
-  uint4 v[N];
-  __device__ __forceinline__ void fetch(const Side& s, int G, int r0, int end, int dh_bytes, int lane) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 v[N];
+  template <bool STREAM> __device__ __forceinline__ void load(const Side& s, int r0, int end, int dh_bytes, int lane) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = lane + i * 64, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r, G) + c);
+      v[i] = 0;
+      if (r < end && c < dh_bytes) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(s.row(r, 1) + c);
+        v[i] = STREAM ? stream_load(p) : *p;
+      }
     }
+  }
+  __device__ __forceinline__ void fetch(const Side& s, int r0, int end, int dh_bytes, bool stream, int lane) {
+    if (stream) load<true>(s, r0, end, dh_bytes, lane);
+    else load<false>(s, r0, end, dh_bytes, lane);
   }
   // rows without a bit are zeros, whatever was read
   __device__ __forceinline__ void put(char* lds, uint32_t bits, int lane) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = lane + i * 64, r = e / Tl::kChunks;
-      *reinterpret_cast<uint4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<u32x4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : (u32x4)0;
     }
   }
 };
@@ -59,14 +67,16 @@ template <int KW> __device__ __forceinline__ FewWork few_work(const Args& A, int
   return f;
 }
 
-// Turns of KW x 32 keys and shares of the keys for the few-rows kernels.  Up to 64 keys one wave does it all; otherwise four.  The keys are
-// split over workgroups while there are fewer than two for each compute unit, in shares of at least two turns.
+// Waves of a workgroup and shares of the keys.  Up to 64 keys one wave does it all; otherwise four, and eight in the forward of two-byte
+// types while there are fewer than two workgroups for each compute unit (eight fill its registers as two of four do, with half the
+// shares to join).  The keys are split over workgroups while there are fewer than that, in shares of at least two turns.
 struct FewPlan { int KW, splits, tiles_per_split; };
-inline FewPlan few_plan(const dvgr_attn_problem& a) {
+inline FewPlan few_plan(const dvgr_attn_problem& a, bool forward) {
   FewPlan p{};
-  p.KW = a.Lk <= 64 ? 1 : 4;
-  const int64_t turns = ((int64_t)a.Lk + p.KW * 32 - 1) / (p.KW * 32), units = (int64_t)a.B * a.Hk;
-  int64_t s = units ? 512 / units : 1;
+  const int64_t units = (int64_t)a.B * a.Hk;
+  p.KW = a.Lk <= 64 ? 1 : forward && a.elem != DVGR_ELEM_F32 && units < 512 ? 8 : 4;
+  const int64_t turns = ((int64_t)a.Lk + p.KW * 32 - 1) / (p.KW * 32);
+  int64_t s = units ? (p.KW == 8 ? 256 : 512) / units : 1;
   if (s > turns / 2) s = turns / 2;
   if (s < 1) s = 1;
   p.tiles_per_split = (int)((turns + s - 1) / s);

@@ -85,7 +85,7 @@ __device__ __forceinline__ MaxSum row_part(const T* row, int64_t c0, int64_t c1,
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
               const int64_t x = at + (int64_t)u * kThreads * N;
-              if (x < e) v[u] = *reinterpret_cast<const typename Vec16<T>::type*>(row + x);
+              if (x < e) v[u] = stream_load(reinterpret_cast<const typename Vec16<T>::type*>(row + x));
               else v[u] = (T)-INFINITY;
             }
             float f[kUnroll * N];
@@ -229,16 +229,17 @@ __global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowSt
   if (SAME)
     for_row(row, c0, c1, tid, [&](int64_t at, int64_t e) {
       constexpr int N = Vec16<T>::N;
-      float f[kUnroll][N];
+      typename Vec16<T>::type v[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u)
-        if (at + (int64_t)u * kThreads * N < e) load_vec(row + at + (int64_t)u * kThreads * N, f[u]);
+        if (at + (int64_t)u * kThreads * N < e) v[u] = *reinterpret_cast<const typename Vec16<T>::type*>(row + at + (int64_t)u * kThreads * N);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         if (at + (int64_t)u * kThreads * N >= e) break;
+        float f[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[u][i] = grad(f[u][i]);
-        store_vec(out + at + (int64_t)u * kThreads * N, f[u]);
+        for (int i = 0; i < N; ++i) f[i] = grad((float)v[u][i]);
+        stream_store_vec(out + at + (int64_t)u * kThreads * N, f);
       }
     }, [&](int64_t at) { out[at] = (T)grad((float)row[at]); });
   else

@@ -37,11 +37,11 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const T* __restrict__ table, 
       if (more) load_vec(src + (c + 64) * N, g);
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = ok ? f[i] * scale : 0.f;
-      store_vec(dst + c * N, f);
+      stream_store_vec(dst + c * N, f);
       if (!more) break;
 #pragma unroll
       for (int i = 0; i < N; ++i) g[i] = ok ? g[i] * scale : 0.f;
-      store_vec(dst + (c + 64) * N, g);
+      stream_store_vec(dst + (c + 64) * N, g);
     }
   } else {
     for (int c = lane; c < wd; c += 64) dst[c] = (T)(ok ? (float)src[c] * scale : 0.f);
@@ -149,7 +149,7 @@ template <typename T, bool VEC> struct Cols {
   __device__ __forceinline__ Raw load(const T* row) const {
     Raw v;
     if (VEC) {
-      if (at(0) < wd) return *reinterpret_cast<const Raw*>(row + at(0));
+      if (at(0) < wd) return stream_load(reinterpret_cast<const Raw*>(row + at(0)));
       v = (T)0.f;
     } else {
 #pragma unroll
@@ -163,7 +163,7 @@ template <typename T, bool VEC> struct Cols {
   }
   __device__ __forceinline__ void store(T* row, const float (&f)[N]) const {
     if (VEC) {
-      if (at(0) < wd) store_vec(row + at(0), f);
+      if (at(0) < wd) stream_store_vec(row + at(0), f);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) if (at(i) < wd) row[at(i)] = (T)f[i];
@@ -215,7 +215,7 @@ __device__ __forceinline__ void zero_rows(const int32_t* key, int64_t n, int64_t
   for (int r = wave; r < rows && r0 + r < vocab; r += 4) {
     if (sh_there[r]) continue;
     T* row = g_table + (r0 + r) * wd;
-    if (VEC) for (int c = lane * N; c < wd; c += 64 * N) store_vec(row + c, z);
+    if (VEC) for (int c = lane * N; c < wd; c += 64 * N) stream_store_vec(row + c, z);
     else for (int c = lane; c < wd; c += 64) row[c] = (T)0.f;
   }
 }
