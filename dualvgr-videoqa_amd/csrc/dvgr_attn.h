@@ -106,33 +106,54 @@ template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32],
 template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32], const char* at, const f32x16& p, int lane, f16_t) { mma_tr16<f16_t, DP>(acc, at, p, lane); }
 
 // ROWS rows of a tensor on their way to LDS: fetched into registers one tile ahead, written behind the barrier that frees the tile.
+// Nothing between the two may look at what was fetched: the wait for it would be a wait for memory in every turn.
 template <typename T, int DP, int ROWS> struct Stage {
   typedef Tile<T, DP> Tl;
   static constexpr int N = ROWS * Tl::kChunks / kThreads;
   static_assert(ROWS * Tl::kChunks % kThreads == 0, "a tile is whole 16-byte pieces for every thread");
   uint4 v[N];
-  bool ok[N];
-  // rows r0 .. of which those below `end` exist; `mask`: bytes, by row, or nullptr
-  __device__ __forceinline__ void fetch(const Side& s, int G, int r0, int end, const uint8_t* mask, int dh_bytes, int tid) {
+  // rows r0 .. of which those below `end` exist
+  __device__ __forceinline__ void fetch(const Side& s, int G, int r0, int end, int dh_bytes, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * kThreads, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
       v[i] = make_uint4(0, 0, 0, 0);
-      ok[i] = true;
-      if (r < end && c < dh_bytes) {
-        v[i] = *reinterpret_cast<const uint4*>(s.row(r, G) + c);
-        if (mask) ok[i] = mask[r] != 0;
-      }
+      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r, G) + c);
+    }
+  }
+  // rows without a bit are zeros, whatever was read
+  __device__ __forceinline__ void put(char* lds, unsigned long long bits, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * kThreads, r = e / Tl::kChunks;
+      *reinterpret_cast<uint4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
     }
   }
   __device__ __forceinline__ void put(char* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * kThreads;
-      *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * Tl::kStride + (e % Tl::kChunks) * 16) = ok[i] ? v[i] : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * Tl::kStride + (e % Tl::kChunks) * 16) = v[i];
     }
   }
 };
+
+// is key j there, as a number that is not looked at before it is needed
+__device__ __forceinline__ uint32_t key_there(const uint8_t* mask, int j, int n) {
+  uint32_t x = 0;
+  if (j < n) {
+    x = 1;
+    if (mask) x = mask[j];
+  }
+  return x;
+}
+
+// Operands loaded in front of a loop are waited for here: left to their first use, inside the loop, that wait would also be one for the
+// loop's own loads, in every turn.
+template <typename F, int N> __device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
 
 // the value of both halves of the wave, combined
 __device__ __forceinline__ float half_max(float x) {

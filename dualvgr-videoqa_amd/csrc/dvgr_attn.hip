@@ -10,16 +10,22 @@ namespace dvgr {
 namespace attn {
 namespace {
 
-// one 32-key tile of a wave's online softmax: s in, probabilities out, m, l and o brought to the new maximum
-template <int NT> __device__ __forceinline__ void softmax_tile(f32x16& s, uint32_t bits, float c, float& m, float& l, f32x16 (&o)[NT], int lane) {
-  if (bits != 0xffffffffu) {
-    const uint32_t hb = half_bits(bits, lane);
+// KS 32-key tiles of a wave's online softmax: s in, probabilities out, m, l and o brought to the new maximum
+template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (&s)[KS], unsigned long long bits, float c, float& m, float& l, f32x16 (&o)[NT],
+                                                                        int lane) {
+  if (bits != (KS == 2 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = reg_bit(hb, r) ? s[r] : -INFINITY;
+    for (int i = 0; i < KS; ++i) {
+      const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[i][r] = reg_bit(hb, r) ? s[i][r] : -INFINITY;
+    }
   }
-  float mx = s[0];
+  float mx = s[0][0];
 #pragma unroll
-  for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+  for (int i = 0; i < KS; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
   mx = half_max(mx) * c;
   if (__any(mx > m)) {
     const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);      // nothing summed yet: o and l are 0
@@ -31,13 +37,16 @@ template <int NT> __device__ __forceinline__ void softmax_tile(f32x16& s, uint32
     m = mn;
   }
   const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = exp2_fast(fmaf(s[r], c, -ref));
-    sum += s[r];
+  for (int i = 0; i < KS; ++i) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[i][r] = exp2_fast(fmaf(s[i][r], c, -ref));
+      sum += s[i][r];
+    }
+    l += sum;
   }
-  l += sum;
 }
 
 // a row's output from o (unnormalised), with what its rounding leaves, and its log-sum
@@ -64,7 +73,7 @@ template <typename T, int NT> __device__ __forceinline__ void write_row(const Ar
 
 // ---- many rows: 4 x 32 of them, tiles of KS x 32 keys -----------------------------------------------------------------------------
 template <typename T, int DP, int KS>
-__global__ __launch_bounds__(kThreads) void k_attn_fwd(Args A) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(Args A) {
   typedef Tile<T, DP> Tl;
   constexpr int KT = KS * 32, RT = kWaves * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
@@ -86,6 +95,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Args A) {
     const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0, A.G);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) qf[s] = Tl::gfrag(qr, s, lane, dhb, live);
+    settle(qf);
   }
   f32x16 o[NT];
 #pragma unroll
@@ -93,31 +103,31 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Args A) {
   float m = -INFINITY, l = 0.f;
 
   Stage<T, DP, KT> sk, sv;
-  bool there = false;                                               // lane j: key j of the next tile
+  uint32_t there = 0;                                               // lane j: key j of the next tile
   const auto fetch = [&](int t) {
-    sk.fetch(ks, 1, t * KT, n, mask, dhb, tid);
-    sv.fetch(vs, 1, t * KT, n, mask, dhb, tid);
-    const int j = t * KT + lane;
-    there = lane < KT && j < n && (!mask || mask[j]);
+    sk.fetch(ks, 1, t * KT, n, dhb, tid);
+    sv.fetch(vs, 1, t * KT, n, dhb, tid);
+    there = key_there(mask, t * KT + lane, lane < KT ? n : 0);
   };
   if (tn) fetch(0);
   for (int t = 0; t < tn; ++t) {
+    const unsigned long long bits = __ballot(there != 0);
     __syncthreads();
-    sk.put(lk, tid);
-    sv.put(lv, tid);
-    const unsigned long long bits = __ballot(there);
+    sk.put(lk, bits, tid);
+    sv.put(lv, bits, tid);
     __syncthreads();
     if (t + 1 < tn) fetch(t + 1);
-#pragma unroll 1
-    for (int i = 0; i < KS; ++i) {
-      const uint32_t tile_bits = (uint32_t)(bits >> (32 * i));
-      if (!tile_bits) continue;                                     // (uniform over the wave)
-      f32x16 s = zero16();
+    if (!bits) continue;                                            // (uniform over the workgroup)
+    f32x16 s[KS];
 #pragma unroll
-      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lk + i * 32 * Tl::kStride, st, lane), qf[st], s);
-      softmax_tile(s, tile_bits, A.c, m, l, o, lane);
-      mma_tr<DP>(o, lv + i * 32 * Tl::kStride, s, lane, T());
-    }
+    for (int i = 0; i < KS; ++i) s[i] = zero16();
+#pragma unroll
+    for (int st = 0; st < Tl::kSteps; ++st)
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s[i] = mma(Tl::frag(lk + i * 32 * Tl::kStride, st, lane), qf[st], s[i]);
+    softmax_tiles(s, bits, A.c, m, l, o, lane);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) mma_tr<DP>(o, lv + i * 32 * Tl::kStride, s[i], lane, T());
   }
   l = half_sum(l);
   if (live) write_row<T>(A, b, hk, row, o, m, l, 0, 1, true, lane);
@@ -146,12 +156,11 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   for (int t = 0; t < NT; ++t) o[t] = zero16();
   float m = -INFINITY, l = 0.f;
   WaveStage<T, DP> sk, sv;
-  bool there = false;
+  uint32_t there = 0;
   const auto fetch = [&](int t) {
     sk.fetch(ks, t * 32, f.n, dhb, A.stream, lane);
     sv.fetch(vs, t * 32, f.n, dhb, A.stream, lane);
-    const int key = t * 32 + (lane & 31);
-    there = key < f.n && (!mask || mask[key]);
+    there = key_there(mask, t * 32 + (lane & 31), f.n);
   };
   if (f.t0 < f.t1) fetch(f.t0);
   for (int e = threadIdx.x; e < 32 * Tl::kChunks; e += 64 * KW) {
@@ -162,18 +171,18 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   }
   __syncthreads();
   for (int t = f.t0; t < f.t1; t += KW) {
-    const uint32_t bits = (uint32_t)__ballot(there);                // (lanes 32 + j say the same as lanes j)
+    const uint32_t bits = (uint32_t)__ballot(there != 0);              // (lanes 32 + j say the same as lanes j)
     wave_order();
     sk.put(lk, bits, lane);
     sv.put(lv, bits, lane);
     wave_order();
     if (t + KW < f.t1) fetch(t + KW);
     if (!bits) continue;
-    f32x16 s = zero16();
+    f32x16 s[1] = {zero16()};
 #pragma unroll
-    for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lk, st, lane), Tl::frag(lq, st, lane), s);
-    softmax_tile(s, bits, A.c, m, l, o, lane);
-    mma_tr<DP>(o, lv, s, lane, T());
+    for (int st = 0; st < Tl::kSteps; ++st) s[0] = mma(Tl::frag(lk, st, lane), Tl::frag(lq, st, lane), s[0]);
+    softmax_tiles(s, bits, A.c, m, l, o, lane);
+    mma_tr<DP>(o, lv, s[0], lane, T());
   }
   l = half_sum(l);
 

@@ -112,6 +112,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
     const char* vr = k_side(A, A.a.v, b, hk).row(there ? key : 0, 1);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) { kf[s] = Tl::gfrag(kr, s, lane, dhb, there); vf[s] = Tl::gfrag(vr, s, lane, dhb, there); }
+    settle(kf);
+    settle(vf);
   }
   f32x16 dk[NT], dv[NT];
 #pragma unroll
@@ -122,21 +124,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
 
   Stage<T, DP, RT> sq, sg;
   float stat = 0.f;
+  const float* from = tid < RT ? A.a.lse : B.delta;
   const auto fetch = [&](int t) {
-    sq.fetch(qs, A.G, t * RT, A.rows, nullptr, dhb, tid);
-    sg.fetch(gs, A.G, t * RT, A.rows, nullptr, dhb, tid);
-    if (tid < 2 * RT) {
-      const int r = t * RT + tid % RT;
-      const int64_t at = r < A.rows ? row_index(A, b, hk, r) : 0;
-      stat = r < A.rows ? (tid < RT ? A.a.lse[at] : B.delta[at]) : (tid < RT ? INFINITY : 0.f);
-    }
+    sq.fetch(qs, A.G, t * RT, A.rows, dhb, tid);
+    sg.fetch(gs, A.G, t * RT, A.rows, dhb, tid);
+    const int r = t * RT + tid % RT;
+    if (tid < 2 * RT) stat = from[row_index(A, b, hk, r < A.rows ? r : A.rows - 1)];
   };
   if (rtiles) fetch(0);
   for (int t = 0; t < rtiles; ++t) {
     __syncthreads();
     sq.put(lq, tid);
     sg.put(lg, tid);
-    if (tid < 2 * RT) lstat[tid] = stat;
+    if (tid < 2 * RT) lstat[tid] = t * RT + tid % RT < A.rows ? stat : tid < RT ? INFINITY : 0.f;      // (no row: p = 0)
     __syncthreads();
     if (t + 1 < rtiles) fetch(t + 1);
 #pragma unroll 1
@@ -232,28 +232,31 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
     const char* gr = q_side(A, B.g_o, b, hk).row(live ? row : 0, A.G);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) { qf[s] = Tl::gfrag(qr, s, lane, dhb, live); gf[s] = Tl::gfrag(gr, s, lane, dhb, live); }
+    settle(qf);
+    settle(gf);
   }
   const int64_t ri = row_index(A, b, hk, live ? row : 0);
-  const float lse = live ? A.a.lse[ri] : INFINITY, delta = live ? B.delta[ri] : 0.f;
+  float stats[2] = {live ? A.a.lse[ri] : INFINITY, live ? B.delta[ri] : 0.f};
+  settle(stats);
+  const float lse = stats[0], delta = stats[1];
   const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
   f32x16 dq[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) dq[t] = zero16();
 
   Stage<T, DP, KT> sk, sv;
-  bool there = false;
+  uint32_t there = 0;
   const auto fetch = [&](int t) {
-    sk.fetch(ks, 1, t * KT, n, mask, dhb, tid);
-    sv.fetch(vs, 1, t * KT, n, mask, dhb, tid);
-    const int j = t * KT + lane;
-    there = lane < KT && j < n && (!mask || mask[j]);
+    sk.fetch(ks, 1, t * KT, n, dhb, tid);
+    sv.fetch(vs, 1, t * KT, n, dhb, tid);
+    there = key_there(mask, t * KT + lane, lane < KT ? n : 0);
   };
   if (tn) fetch(0);
   for (int t = 0; t < tn; ++t) {
+    const unsigned long long bits = __ballot(there != 0);
     __syncthreads();
-    sk.put(lk, tid);
-    sv.put(lv, tid);
-    const unsigned long long bits = __ballot(there);
+    sk.put(lk, bits, tid);
+    sv.put(lv, bits, tid);
     __syncthreads();
     if (t + 1 < tn) fetch(t + 1);
 #pragma unroll 1
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 
   WaveStage<T, DP> sk, sv;
   Frag<T> vf[kOut ? 1 : Tl::kSteps];
-  bool there = false;
+  uint32_t there = 0;
   const auto fetch = [&](int t) {
     const int key = t * 32 + col;
     sk.fetch(ks, t * 32, f.n, dhb, false, lane);
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 #pragma unroll
       for (int s = 0; s < Tl::kSteps; ++s) vf[s] = Tl::gfrag(vr, s, lane, dhb, key < f.n);
     }
-    there = key < f.n && (!mask || mask[key]);
+    there = key_there(mask, key, f.n);
   };
   if (f.t0 < f.t1) fetch(f.t0);
   {                                                                 // the rows
@@ -404,8 +407,8 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
   };
   int t = f.t0;
   for (; t < f.t1; t += KW) {
-    const uint32_t bits = (uint32_t)__ballot(there);
-    const bool here = there;
+    const bool here = there != 0;
+    const uint32_t bits = (uint32_t)__ballot(here);
     wave_order();
     sk.put(lk, bits, lane);
     if constexpr (kOut) sv.put(lx, bits, lane);
