@@ -37,28 +37,38 @@ __device__ __forceinline__ f32x16 zero16() {
 
 constexpr int kThreads = 256, kWaves = 4;          // of the kernels for many rows
 
-// One head's side of a tensor: row r of the packed rows (query l, head g of the group, r = l * G + g) or key r (G = 1).
+// One head's side of a tensor: row r of the packed rows (query l, head g of the group, r = l * G + g) or key r (G = 1).  Every thread
+// finds several rows' places in every turn, so this is kept to few instructions: a shift where G is a power of two, and products of
+// 32 x 32 bits.
 struct Side {
   const char* p;
-  int64_t sl, sg;                   // bytes
-  __device__ __forceinline__ const char* row(int r, int G) const {
-    const int l = G == 1 ? r : r / G;
-    return p + (int64_t)l * sl + (int64_t)(r - l * G) * sg;
+  uint32_t sl;                      // bytes between rows, under 2^32
+  int64_t sg;                       // bytes between heads
+  int G, shift;                     // shift: log2 G, or -1
+  __device__ __forceinline__ const char* row(int r) const {
+    if (G == 1) return p + (uint64_t)(uint32_t)r * sl;
+    const int l = shift >= 0 ? r >> shift : r / G;
+    return p + (uint64_t)(uint32_t)l * sl + (uint32_t)(r - l * G) * sg;
   }
 };
 
 template <typename T, int DP> struct Tile {
   static constexpr int kRowBytes = DP * (int)sizeof(T);
-  static constexpr int kStride = kRowBytes + 16;          // bytes; the pad spreads the rows over the banks
+  // Bytes between rows in LDS.  16 rows of one 16-byte piece (a row product's operand) fall on different banks if the stride is an odd
+  // number of pieces; 4 rows of 4 pieces (an operand across the rows) need it to be 3, 5, 11 or 13 modulo 16 as well.
+  static constexpr int kStride = kRowBytes + 16;
+  static constexpr int kStrideT = sizeof(T) == 2 && DP == 128 ? kRowBytes + 48 : kStride;          // tiles read across their rows
   static constexpr int kSteps = kRowBytes / 32;
   static constexpr int kChunks = kRowBytes / 16;          // 16-byte pieces of a row
   static constexpr int kNT = DP / 32;                     // 32-wide tiles of the head dimension
   template <int ROWS> static constexpr int bytes() { return ROWS * kStride; }
+  template <int ROWS> static constexpr int bytesT() { return ROWS * kStrideT; }
 
   // operand of a row-wise product: row `lane & 31` of the 32 rows at `at`
-  static __device__ __forceinline__ Frag<T> frag(const char* at, int step, int lane) {
-    return *reinterpret_cast<const Frag<T>*>(at + (lane & 31) * kStride + step * 32 + (lane >> 5) * 16);
+  template <int S = kStride> static __device__ __forceinline__ Frag<T> frag(const char* at, int step, int lane) {
+    return *reinterpret_cast<const Frag<T>*>(at + (lane & 31) * S + step * 32 + (lane >> 5) * 16);
   }
+  static __device__ __forceinline__ Frag<T> fragT(const char* at, int step, int lane) { return frag<kStrideT>(at, step, lane); }
   // the same straight from memory, zeros beyond the head and where `ok` is false
   static __device__ __forceinline__ Frag<T> gfrag(const char* row, int step, int lane, int dh_bytes, bool ok) {
     Frag<T> f;
@@ -70,9 +80,9 @@ template <typename T, int DP> struct Tile {
   }
 };
 
-// acc[t] += M^T P: M = 32 rows of LDS at `at` (row-major, head dimension along the row), P = 32 x 32 in accumulator layout
+// acc[t] += M^T P: M = 32 rows of LDS at `at` (kStrideT apart, head dimension along the row), P = 32 x 32 in accumulator layout
 template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32], const char* at, const f32x16& p, int lane, float) {
-  constexpr int S = Tile<float, DP>::kStride;
+  constexpr int S = Tile<float, DP>::kStrideT;
   const char* base = at + (lane >> 5) * 4 * S + (lane & 31) * 4;
 #pragma unroll
   for (int r = 0; r < 16; ++r)
@@ -83,7 +93,7 @@ template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32],
     }
 }
 template <typename T, int DP> __device__ __forceinline__ void mma_tr16(f32x16 (&acc)[DP / 32], const char* at, const f32x16& p, int lane) {
-  constexpr int S = Tile<T, DP>::kStride;
+  constexpr int S = Tile<T, DP>::kStrideT;
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   // lanes of a group of 16 name 4 rows x 16 columns, 4 elements each, and get one column's 4 rows
   const char* base = at + ((lane >> 5) * 4 + (lane & 15) / 4) * S + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
@@ -113,27 +123,27 @@ template <typename T, int DP, int ROWS> struct Stage {
   static_assert(ROWS * Tl::kChunks % kThreads == 0, "a tile is whole 16-byte pieces for every thread");
   uint4 v[N];
   // rows r0 .. of which those below `end` exist
-  __device__ __forceinline__ void fetch(const Side& s, int G, int r0, int end, int dh_bytes, int tid) {
+  __device__ __forceinline__ void fetch(const Side& s, int r0, int end, int dh_bytes, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * kThreads, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
       v[i] = make_uint4(0, 0, 0, 0);
-      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r, G) + c);
+      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r) + c);
     }
   }
   // rows without a bit are zeros, whatever was read
-  __device__ __forceinline__ void put(char* lds, unsigned long long bits, int tid) const {
+  template <int S> __device__ __forceinline__ void put(char* lds, unsigned long long bits, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * kThreads, r = e / Tl::kChunks;
-      *reinterpret_cast<uint4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(lds + r * S + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
     }
   }
-  __device__ __forceinline__ void put(char* lds, int tid) const {
+  template <int S> __device__ __forceinline__ void put(char* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * kThreads;
-      *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * Tl::kStride + (e % Tl::kChunks) * 16) = v[i];
+      *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * S + (e % Tl::kChunks) * 16) = v[i];
     }
   }
 };
@@ -185,7 +195,7 @@ inline unsigned xcd_grid(int64_t total) { return (unsigned)((total + 7) / 8 * 8)
 
 struct Args {
   dvgr_attn_problem a;
-  int G, rows;                      // heads of a group; Lq * G packed rows of one key head
+  int G, shift, rows;               // heads of a group, log2 of it or -1; Lq * G packed rows of one key head
   int es;
   int splits, tiles_per_split;      // the keys of a sample in shares of whole tiles
   float c;                          // scale * log2 e
@@ -193,10 +203,10 @@ struct Args {
   float *part_o, *part_ml;          // splits > 1: (work, rows of the tile, Dh) and (.., 2)
 };
 __device__ __forceinline__ Side q_side(const Args& A, const dvgr_attn_view& v, int b, int hk) {
-  return Side{(const char*)v.p + ((int64_t)b * v.sb + (int64_t)hk * A.G * v.sh) * A.es, v.sl * A.es, v.sh * A.es};
+  return Side{(const char*)v.p + ((int64_t)b * v.sb + (int64_t)hk * A.G * v.sh) * A.es, (uint32_t)(v.sl * A.es), v.sh * A.es, A.G, A.shift};
 }
 __device__ __forceinline__ Side k_side(const Args& A, const dvgr_attn_view& v, int b, int hk) {
-  return Side{(const char*)v.p + ((int64_t)b * v.sb + (int64_t)hk * v.sh) * A.es, v.sl * A.es, 0};
+  return Side{(const char*)v.p + ((int64_t)b * v.sb + (int64_t)hk * v.sh) * A.es, (uint32_t)(v.sl * A.es), 0, 1, 0};
 }
 __device__ __forceinline__ int key_count(const Args& A, int b) {
   if (!A.a.lens) return A.a.Lk;
@@ -204,14 +214,14 @@ __device__ __forceinline__ int key_count(const Args& A, int b) {
   return n < 0 ? 0 : n > A.a.Lk ? A.a.Lk : (int)n;
 }
 __device__ __forceinline__ int64_t row_index(const Args& A, int b, int hk, int r) {          // (B, H, Lq) of packed row r
-  const int l = A.G == 1 ? r : r / A.G;
+  const int l = A.shift >= 0 ? r >> A.shift : r / A.G;
   return ((int64_t)b * A.a.H + hk * A.G + (r - l * A.G)) * A.a.Lq + l;
 }
 
 // row of what the output's rounding left (B, Lq, H, Dh), or nullptr
 template <typename T> __device__ __forceinline__ char* lo_row(const Args& A, int b, int hk, int r) {
   if (sizeof(T) == 4 || !A.a.o_lo) return nullptr;
-  const int l = A.G == 1 ? r : r / A.G;
+  const int l = A.shift >= 0 ? r >> A.shift : r / A.G;
   return (char*)A.a.o_lo + (((int64_t)b * A.a.Lq + l) * A.a.H + hk * A.G + (r - l * A.G)) * A.a.Dh * (int64_t)sizeof(T);
 }
 

@@ -53,7 +53,7 @@ template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (
 template <typename T, int NT> __device__ __forceinline__ void write_row(const Args& A, int b, int hk, int row, const f32x16 (&o)[NT], float m, float l,
                                                                         int first, int step, bool stats, int lane) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* out = const_cast<char*>(q_side(A, A.a.o, b, hk).row(row, A.G));
+  char* out = const_cast<char*>(q_side(A, A.a.o, b, hk).row(row));
   char* lo = lo_row<T>(A, b, hk, row);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
 
   Frag<T> qf[Tl::kSteps];
   {
-    const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0, A.G);
+    const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) qf[s] = Tl::gfrag(qr, s, lane, dhb, live);
     settle(qf);
@@ -105,16 +105,16 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
   Stage<T, DP, KT> sk, sv;
   uint32_t there = 0;                                               // lane j: key j of the next tile
   const auto fetch = [&](int t) {
-    sk.fetch(ks, 1, t * KT, n, dhb, tid);
-    sv.fetch(vs, 1, t * KT, n, dhb, tid);
+    sk.fetch(ks, t * KT, n, dhb, tid);
+    sv.fetch(vs, t * KT, n, dhb, tid);
     there = key_there(mask, t * KT + lane, lane < KT ? n : 0);
   };
   if (tn) fetch(0);
   for (int t = 0; t < tn; ++t) {
     const unsigned long long bits = __ballot(there != 0);
     __syncthreads();
-    sk.put(lk, bits, tid);
-    sv.put(lv, bits, tid);
+    sk.template put<Tl::kStride>(lk, bits, tid);
+    sv.template put<Tl::kStrideT>(lv, bits, tid);
     __syncthreads();
     if (t + 1 < tn) fetch(t + 1);
     if (!bits) continue;                                            // (uniform over the workgroup)
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
       for (int i = 0; i < KS; ++i) s[i] = mma(Tl::frag(lk + i * 32 * Tl::kStride, st, lane), qf[st], s[i]);
     softmax_tiles(s, bits, A.c, m, l, o, lane);
 #pragma unroll
-    for (int i = 0; i < KS; ++i) mma_tr<DP>(o, lv + i * 32 * Tl::kStride, s[i], lane, T());
+    for (int i = 0; i < KS; ++i) mma_tr<DP>(o, lv + i * 32 * Tl::kStrideT, s[i], lane, T());
   }
   l = half_sum(l);
   if (live) write_row<T>(A, b, hk, row, o, m, l, 0, 1, true, lane);
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, kw = threadIdx.x >> 6;
   char* lq = lds;
-  char* lk = lds + (1 + kw * 2) * Tl::template bytes<32>();
+  char* lk = lds + Tl::template bytes<32>() + kw * (Tl::template bytes<32>() + Tl::template bytesT<32>());
   char* lv = lk + Tl::template bytes<32>();
   const FewWork f = few_work<KW>(A, kw);
   if (!f.any) return;
@@ -166,15 +166,15 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   for (int e = threadIdx.x; e < 32 * Tl::kChunks; e += 64 * KW) {
     const int r = e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < A.rows && c < dhb) x = *reinterpret_cast<const uint4*>(q_side(A, A.a.q, f.b, f.hk).row(r, A.G) + c);
+    if (r < A.rows && c < dhb) x = *reinterpret_cast<const uint4*>(q_side(A, A.a.q, f.b, f.hk).row(r) + c);
     *reinterpret_cast<uint4*>(lq + r * Tl::kStride + c) = x;
   }
   __syncthreads();
   for (int t = f.t0; t < f.t1; t += KW) {
     const uint32_t bits = (uint32_t)__ballot(there != 0);              // (lanes 32 + j say the same as lanes j)
     wave_order();
-    sk.put(lk, bits, lane);
-    sv.put(lv, bits, lane);
+    sk.template put<Tl::kStride>(lk, bits, lane);
+    sv.template put<Tl::kStrideT>(lv, bits, lane);
     wave_order();
     if (t + KW < f.t1) fetch(t + KW);
     if (!bits) continue;
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   x *= inv; y *= inv;
-  T* out = (T*)q_side(A, A.a.o, b, hk).row(row, A.G);
+  T* out = (T*)q_side(A, A.a.o, b, hk).row(row);
   T* lo = (T*)lo_row<T>(A, b, hk, row);
   if (d < A.a.Dh) {
     out[d] = (T)x; out[d + 1] = (T)y;
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
 }
 
 template <typename T, int DP, int KS> int launch_many(const Args& A, hipStream_t st) {
-  const size_t bytes = 2 * Tile<T, DP>::template bytes<KS * 32>();
+  const size_t bytes = Tile<T, DP>::template bytes<KS * 32>() + Tile<T, DP>::template bytesT<KS * 32>();
   static std::atomic<uint32_t> asked{0};
   const auto kern = k_attn_fwd<T, DP, KS>;
   const int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
@@ -304,7 +304,7 @@ template <typename T, int DP, int KS> int launch_many(const Args& A, hipStream_t
 }
 template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t st) {
   typedef Tile<T, DP> Tl;
-  size_t bytes = (1 + 2 * KW) * Tl::template bytes<32>();
+  size_t bytes = (1 + KW) * Tl::template bytes<32>() + KW * Tl::template bytesT<32>();
   const size_t join = KW > 1 ? (size_t)(KW * 64 + KW * Tl::kNT * 16 * 64) * sizeof(float) : 0;
   bytes = bytes > join ? bytes : join;
   static std::atomic<uint32_t> asked{0};
@@ -346,7 +346,7 @@ Parts parts(const dvgr_attn_problem& a) {
 
 bool view_ok(const dvgr_attn_view& v, int es, int64_t B, int64_t L, int64_t H) {
   const auto bad = [es](int64_t s) { return (s * es) % 16 != 0; };
-  return ptr16(v.p) && !(B > 1 && bad(v.sb)) && !(L > 1 && bad(v.sl)) && !(H > 1 && bad(v.sh));
+  return ptr16(v.p) && v.sl >= 0 && v.sl * es < (1ll << 32) && !(B > 1 && bad(v.sb)) && !(L > 1 && bad(v.sl)) && !(H > 1 && bad(v.sh));
 }
 
 int check(const dvgr_attn_problem* a) {
@@ -377,6 +377,7 @@ Args make_args(const dvgr_attn_problem& a) {
   Args A{};
   A.a = a;
   A.G = a.H / a.Hk;
+  A.shift = (A.G & (A.G - 1)) == 0 ? __builtin_ctz(A.G) : -1;
   A.rows = a.Lq * A.G;
   A.es = elem_size(a.elem);
   A.splits = A.tiles_per_split = 1;

@@ -41,8 +41,8 @@ __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
   const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (i >= (int64_t)A.a.B * A.a.Hk * A.rows) return;
   const int row = (int)(i % A.rows), hk = (int)(i / A.rows % A.a.Hk), b = (int)(i / A.rows / A.a.Hk);
-  const T* o = (const T*)q_side(A, A.a.o, b, hk).row(row, A.G);
-  const T* g = (const T*)q_side(A, B.g_o, b, hk).row(row, A.G);
+  const T* o = (const T*)q_side(A, A.a.o, b, hk).row(row);
+  const T* g = (const T*)q_side(A, B.g_o, b, hk).row(row);
   const T* lo = (const T*)lo_row<T>(A, b, hk, row);
   constexpr int N = Vec16<T>::N;
   float s = 0.f, top = 0.f;
@@ -73,7 +73,7 @@ template <typename T> __device__ __forceinline__ float grad16(float ds, float sc
 
 template <typename T, int NT> __device__ __forceinline__ void write_dq(const BwdArgs& B, int b, int hk, int row, const f32x16 (&dq)[NT], float f, int first,
                                                                        int step, int lane) {
-  char* out = const_cast<char*>(q_side(B.f, B.g_q, b, hk).row(row, B.f.G));
+  char* out = const_cast<char*>(q_side(B.f, B.g_q, b, hk).row(row));
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t % step != first) continue;
@@ -94,8 +94,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
   constexpr int RT = RW * RS * 32, KT = KW * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   char* lq = lds;
-  char* lg = lq + Tl::template bytes<RT>();
-  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytes<RT>());       // [lse, D][RT]
+  char* lg = lq + Tl::template bytesT<RT>();
+  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [lse, D][RT]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * ktiles);
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
 
   Frag<T> kf[Tl::kSteps], vf[Tl::kSteps];
   {
-    const char* kr = k_side(A, A.a.k, b, hk).row(there ? key : 0, 1);
-    const char* vr = k_side(A, A.a.v, b, hk).row(there ? key : 0, 1);
+    const char* kr = k_side(A, A.a.k, b, hk).row(there ? key : 0);
+    const char* vr = k_side(A, A.a.v, b, hk).row(there ? key : 0);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) { kf[s] = Tl::gfrag(kr, s, lane, dhb, there); vf[s] = Tl::gfrag(vr, s, lane, dhb, there); }
     settle(kf);
@@ -126,28 +126,28 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
   float stat = 0.f;
   const float* from = tid < RT ? A.a.lse : B.delta;
   const auto fetch = [&](int t) {
-    sq.fetch(qs, A.G, t * RT, A.rows, dhb, tid);
-    sg.fetch(gs, A.G, t * RT, A.rows, dhb, tid);
+    sq.fetch(qs, t * RT, A.rows, dhb, tid);
+    sg.fetch(gs, t * RT, A.rows, dhb, tid);
     const int r = t * RT + tid % RT;
     if (tid < 2 * RT) stat = from[row_index(A, b, hk, r < A.rows ? r : A.rows - 1)];
   };
   if (rtiles) fetch(0);
   for (int t = 0; t < rtiles; ++t) {
     __syncthreads();
-    sq.put(lq, tid);
-    sg.put(lg, tid);
+    sq.template put<Tl::kStrideT>(lq, tid);
+    sg.template put<Tl::kStrideT>(lg, tid);
     if (tid < 2 * RT) lstat[tid] = t * RT + tid % RT < A.rows ? stat : tid < RT ? INFINITY : 0.f;      // (no row: p = 0)
     __syncthreads();
     if (t + 1 < rtiles) fetch(t + 1);
 #pragma unroll 1
     for (int i = 0; i < RS; ++i) {
-      const char* tq = lq + (rw * RS + i) * 32 * Tl::kStride;
-      const char* tg = lg + (rw * RS + i) * 32 * Tl::kStride;
+      const char* tq = lq + (rw * RS + i) * 32 * Tl::kStrideT;
+      const char* tg = lg + (rw * RS + i) * 32 * Tl::kStrideT;
       f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
 #pragma unroll
-      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(tq, st, lane), kf[st], s);
+      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tq, st, lane), kf[st], s);
 #pragma unroll
-      for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tg, st, lane), vf[st], dp);
+      for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::fragT(tg, st, lane), vf[st], dp);
       const float* ls = lstat + (rw * RS + i) * 32 + (lane >> 5) * 4;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -191,8 +191,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
   }
   if (key >= A.a.Lk) return;
   const float f = A.a.scale / sc;
-  char* gk = const_cast<char*>(k_side(A, B.g_k, b, hk).row(key, 1));
-  char* gv = const_cast<char*>(k_side(A, B.g_v, b, hk).row(key, 1));
+  char* gk = const_cast<char*>(k_side(A, B.g_k, b, hk).row(key));
+  char* gv = const_cast<char*>(k_side(A, B.g_v, b, hk).row(key));
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (RW > 1 && t % RW != rw) continue;
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   constexpr int KT = KS * 32, RT = kWaves * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   char* lk = lds;
-  char* lv = lds + Tl::template bytes<KT>();
+  char* lv = lds + Tl::template bytesT<KT>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rtiles = (A.rows + RT - 1) / RT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles);
@@ -228,8 +228,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
 
   Frag<T> qf[Tl::kSteps], gf[Tl::kSteps];
   {
-    const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0, A.G);
-    const char* gr = q_side(A, B.g_o, b, hk).row(live ? row : 0, A.G);
+    const char* qr = q_side(A, A.a.q, b, hk).row(live ? row : 0);
+    const char* gr = q_side(A, B.g_o, b, hk).row(live ? row : 0);
 #pragma unroll
     for (int s = 0; s < Tl::kSteps; ++s) { qf[s] = Tl::gfrag(qr, s, lane, dhb, live); gf[s] = Tl::gfrag(gr, s, lane, dhb, live); }
     settle(qf);
@@ -247,26 +247,26 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   Stage<T, DP, KT> sk, sv;
   uint32_t there = 0;
   const auto fetch = [&](int t) {
-    sk.fetch(ks, 1, t * KT, n, dhb, tid);
-    sv.fetch(vs, 1, t * KT, n, dhb, tid);
+    sk.fetch(ks, t * KT, n, dhb, tid);
+    sv.fetch(vs, t * KT, n, dhb, tid);
     there = key_there(mask, t * KT + lane, lane < KT ? n : 0);
   };
   if (tn) fetch(0);
   for (int t = 0; t < tn; ++t) {
     const unsigned long long bits = __ballot(there != 0);
     __syncthreads();
-    sk.put(lk, bits, tid);
-    sv.put(lv, bits, tid);
+    sk.template put<Tl::kStrideT>(lk, bits, tid);
+    sv.template put<Tl::kStride>(lv, bits, tid);
     __syncthreads();
     if (t + 1 < tn) fetch(t + 1);
 #pragma unroll 1
     for (int i = 0; i < KS; ++i) {
       if (!(uint32_t)(bits >> (32 * i))) continue;                  // (uniform over the wave)
-      const char* tk = lk + i * 32 * Tl::kStride;
+      const char* tk = lk + i * 32 * Tl::kStrideT;
       const char* tv = lv + i * 32 * Tl::kStride;
       f32x16 s = zero16(), dp = zero16();                           // rows = keys, column = this lane's packed row
 #pragma unroll
-      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(tk, st, lane), qf[st], s);
+      for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tk, st, lane), qf[st], s);
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tv, st, lane), gf[st], dp);
       const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
@@ -291,9 +291,9 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
 template <typename T, int DP> struct FewLds {
   static constexpr bool kOut = sizeof(T) == 2;                      // fp32: values go straight to operands, gradients leave in 16-byte pieces
   static constexpr int kScr = 36;                                   // floats of a scratch row: 16-byte aligned, spread over the banks
-  static constexpr int kTile = Tile<T, DP>::template bytes<32>(), kScrBytes = 32 * kScr * 4;
-  static constexpr int kOwn = kTile + (kOut && kTile > kScrBytes ? kTile : kScrBytes);
-  static constexpr int kBytes(int KW) { return 2 * kTile + 68 * 4 + KW * kOwn; }
+  static constexpr int kTile = Tile<T, DP>::template bytes<32>(), kTileT = Tile<T, DP>::template bytesT<32>(), kScrBytes = 32 * kScr * 4;
+  static constexpr int kOwn = kTileT + (kOut && kTile > kScrBytes ? kTile : kScrBytes);
+  static constexpr int kBytes(int KW) { return 2 * kTileT + 68 * 4 + KW * kOwn; }
 };
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void k_attn_few_bwd(BwdArgs B) {
@@ -304,10 +304,10 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, kw = tid >> 6, col = lane & 31, h4 = (lane >> 5) * 4;
   char* lq = lds;
-  char* lg = lq + Tl::template bytes<32>();
-  float* stat = reinterpret_cast<float*>(lg + Tl::template bytes<32>());        // [lse, D][32], largest |dO|
+  char* lg = lq + Tl::template bytesT<32>();
+  float* stat = reinterpret_cast<float*>(lg + Tl::template bytesT<32>());        // [lse, D][32], largest |dO|
   char* lk = reinterpret_cast<char*>(stat + 68) + kw * FewLds<T, DP>::kOwn;
-  char* lx = lk + FewLds<T, DP>::kTile;                              // values, then score gradients, then dV, then dK
+  char* lx = lk + FewLds<T, DP>::kTileT;                              // values, then score gradients, then dV, then dK
   float* scr = reinterpret_cast<float*>(lx);
   const FewWork f = few_work<KW>(A, kw);
   if (!f.any) return;
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
     sk.fetch(ks, t * 32, f.n, dhb, false, lane);
     if constexpr (kOut) sv.fetch(vs, t * 32, f.n, dhb, false, lane);
     else {
-      const char* vr = vs.row(key < f.n ? key : 0, 1);
+      const char* vr = vs.row(key < f.n ? key : 0);
 #pragma unroll
       for (int s = 0; s < Tl::kSteps; ++s) vf[s] = Tl::gfrag(vr, s, lane, dhb, key < f.n);
     }
@@ -335,9 +335,9 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
     constexpr int per = 2 * KW;                                     // threads of a row
     const int r = tid / per, sub = tid % per;
     const bool live = r < A.rows;
-    const char* qr = qs.row(live ? r : 0, A.G);
-    const char* gr = gs.row(live ? r : 0, A.G);
-    const char* orow = q_side(A, A.a.o, f.b, f.hk).row(live ? r : 0, A.G);
+    const char* qr = qs.row(live ? r : 0);
+    const char* gr = gs.row(live ? r : 0);
+    const char* orow = q_side(A, A.a.o, f.b, f.hk).row(live ? r : 0);
     const char* lo = lo_row<T>(A, f.b, f.hk, live ? r : 0);
     float d = 0.f, top = 0.f;
     for (int c = sub * 16; c < Tl::kRowBytes; c += per * 16) {
@@ -355,8 +355,8 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
           top = fmaxf(top, fabsf(y[i]));
         }
       }
-      *reinterpret_cast<uint4*>(lq + r * Tl::kStride + c) = q;
-      *reinterpret_cast<uint4*>(lg + r * Tl::kStride + c) = g;
+      *reinterpret_cast<uint4*>(lq + r * Tl::kStrideT + c) = q;
+      *reinterpret_cast<uint4*>(lg + r * Tl::kStrideT + c) = g;
     }
 #pragma unroll
     for (int o = 1; o < per; o <<= 1) { d += __shfl_xor(d, o); top = fmaxf(top, __shfl_xor(top, o)); }
@@ -392,10 +392,10 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
         const int e = lane + i * 64, key = t * 32 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
         typedef typename WaveStage<T, DP>::u32x4 u32x4;
         if (key < A.a.Lk && c < dhb)
-          stream_store(reinterpret_cast<u32x4*>(const_cast<char*>(to.row(key, 1)) + c), *reinterpret_cast<const u32x4*>(lx + (e / Tl::kChunks) * Tl::kStride + c));
+          stream_store(reinterpret_cast<u32x4*>(const_cast<char*>(to.row(key)) + c), *reinterpret_cast<const u32x4*>(lx + (e / Tl::kChunks) * Tl::kStride + c));
       }
     } else if (t * 32 + col < A.a.Lk) {
-      char* out = const_cast<char*>(to.row(t * 32 + col, 1));
+      char* out = const_cast<char*>(to.row(t * 32 + col));
 #pragma unroll
       for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -410,18 +410,18 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
     const bool here = there != 0;
     const uint32_t bits = (uint32_t)__ballot(here);
     wave_order();
-    sk.put(lk, bits, lane);
-    if constexpr (kOut) sv.put(lx, bits, lane);
+    sk.template put<Tl::kStrideT>(lk, bits, lane);
+    if constexpr (kOut) sv.template put<Tl::kStride>(lx, bits, lane);
     wave_order();
     f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
 #pragma unroll
     for (int st = 0; st < Tl::kSteps; ++st) {
-      if constexpr (kOut) dp = mma(Tl::frag(lg, st, lane), Tl::frag(lx, st, lane), dp);
-      else dp = mma(Tl::frag(lg, st, lane), vf[st], dp);
+      if constexpr (kOut) dp = mma(Tl::fragT(lg, st, lane), Tl::frag(lx, st, lane), dp);
+      else dp = mma(Tl::fragT(lg, st, lane), vf[st], dp);
     }
     if (t + KW < f.t1) fetch(t + KW);
 #pragma unroll
-    for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::frag(lq, st, lane), Tl::frag(lk, st, lane), s);
+    for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(lq, st, lane), Tl::fragT(lk, st, lane), s);
     wave_order();
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256) void k_attn_dq_join(BwdArgs B) {
   sh[wave][d] = x; sh[wave][d + 1] = y;
   __syncthreads();
   if (wave || d >= A.a.Dh) return;
-  T* out = (T*)const_cast<char*>(q_side(A, B.g_q, b, hk).row(row, A.G));
+  T* out = (T*)const_cast<char*>(q_side(A, B.g_q, b, hk).row(row));
   out[d] = (T)(sh[0][d] + sh[1][d] + sh[2][d] + sh[3][d]);
   out[d + 1] = (T)(sh[0][d + 1] + sh[1][d + 1] + sh[2][d + 1] + sh[3][d + 1]);
 }
@@ -536,14 +536,14 @@ size_t join_bytes(int waves, int NT) { return waves > 1 ? (size_t)kWaves * NT * 
 template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytes<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float);
+  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float);
   if (bytes < join_bytes(RW, Tl::kNT)) bytes = join_bytes(RW, Tl::kNT);
   return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), kThreads, bytes, B, st);
 }
 template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
   static std::atomic<uint32_t> asked{0};
   return launch(k_attn_dq<T, DP, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.rows + kWaves * 32 - 1) / (kWaves * 32)), kThreads,
-                2 * Tile<T, DP>::template bytes<KS * 32>(), B, st);
+                Tile<T, DP>::template bytes<KS * 32>() + Tile<T, DP>::template bytesT<KS * 32>(), B, st);
 }
 template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;

@@ -20,7 +20,7 @@ template <typename T, int DP> struct WaveStage {
       const int e = lane + i * 64, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
       v[i] = 0;
       if (r < end && c < dh_bytes) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(s.row(r, 1) + c);
+        const u32x4* p = reinterpret_cast<const u32x4*>(s.row(r) + c);
         v[i] = STREAM ? stream_load(p) : *p;
       }
     }
@@ -30,11 +30,11 @@ template <typename T, int DP> struct WaveStage {
     else load<false>(s, r0, end, dh_bytes, lane);
   }
   // rows without a bit are zeros, whatever was read
-  __device__ __forceinline__ void put(char* lds, uint32_t bits, int lane) const {
+  template <int S> __device__ __forceinline__ void put(char* lds, uint32_t bits, int lane) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = lane + i * 64, r = e / Tl::kChunks;
-      *reinterpret_cast<u32x4*>(lds + r * Tl::kStride + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : (u32x4)0;
+      *reinterpret_cast<u32x4*>(lds + r * S + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : (u32x4)0;
     }
   }
 };

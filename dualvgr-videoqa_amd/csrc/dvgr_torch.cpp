@@ -255,14 +255,19 @@ Tensor distillation_loss(Tensor z, Tensor v, Tensor i, double temperature, int64
 }
 
 // ---- cross attention ------------------------------------------------------------------------------------------------------------
-// `t`, or a copy whose heads start at multiples of 16 bytes
+// `t`, or a copy whose heads start at multiples of 16 bytes (the stride of a dimension of one element does not count)
 Tensor ready(const Tensor& t) {
   const int64_t per = 16 / t.element_size();
-  if (t.stride(3) != 1 || t.stride(2) % per || t.stride(1) % per || t.stride(0) % per || ((uintptr_t)t.data_ptr() & 15))
+  const auto off = [&](int d) { return t.size(d) > 1 && t.stride(d) % per != 0; };
+  if ((t.size(3) > 1 && t.stride(3) != 1) || off(2) || off(1) || off(0) || ((uintptr_t)t.data_ptr() & 15) ||
+      (t.size(1) > 1 && t.stride(1) * (int64_t)t.element_size() >= (1ll << 32)))
     return t.clone(at::MemoryFormat::Contiguous);
   return t;
 }
-dvgr_attn_view view(const Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+dvgr_attn_view view(const Tensor& t) {
+  const auto stride = [&](int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  return {t.data_ptr(), stride(0), stride(1), stride(2)};
+}
 
 dvgr_attn_problem problem(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& o_lo, const Tensor& lens, const Tensor& mask,
                           float scale, const Tensor& lse) {

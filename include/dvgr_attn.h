@@ -17,7 +17,8 @@
 extern "C" {
 #endif
 
-/* element (b, l, h, d) at p[b * sb + l * sl + h * sh + d]; p and the strides of dimensions longer than 1 are multiples of 16 bytes */
+/* element (b, l, h, d) at p[b * sb + l * sl + h * sh + d]; p and the strides of dimensions longer than 1 are multiples of 16 bytes,
+ * 0 <= sl < 4 GB */
 typedef struct dvgr_attn_view {
   void *p;
   int64_t sb, sl, sh;
