@@ -117,33 +117,34 @@ template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32],
 
 // ROWS rows of a tensor on their way to LDS: fetched into registers one tile ahead, written behind the barrier that frees the tile.
 // Nothing between the two may look at what was fetched: the wait for it would be a wait for memory in every turn.
-template <typename T, int DP, int ROWS> struct Stage {
+template <typename T, int DP, int ROWS, int THREADS = kThreads> struct Stage {
   typedef Tile<T, DP> Tl;
-  static constexpr int N = ROWS * Tl::kChunks / kThreads;
-  static_assert(ROWS * Tl::kChunks % kThreads == 0, "a tile is whole 16-byte pieces for every thread");
+  static constexpr int kPieces = ROWS * Tl::kChunks, N = (kPieces + THREADS - 1) / THREADS;
+  static constexpr bool kEven = kPieces % THREADS == 0;             // otherwise the last round is some threads' only
   uint4 v[N];
   // rows r0 .. of which those below `end` exist
   __device__ __forceinline__ void fetch(const Side& s, int r0, int end, int dh_bytes, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = tid + i * kThreads, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
+      const int e = tid + i * THREADS, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
       v[i] = make_uint4(0, 0, 0, 0);
-      if (r < end && c < dh_bytes) v[i] = *reinterpret_cast<const uint4*>(s.row(r) + c);
+      if (r < end && c < dh_bytes && (kEven || e < kPieces)) v[i] = *reinterpret_cast<const uint4*>(s.row(r) + c);
     }
   }
   // rows without a bit are zeros, whatever was read
   template <int S> __device__ __forceinline__ void put(char* lds, unsigned long long bits, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = tid + i * kThreads, r = e / Tl::kChunks;
-      *reinterpret_cast<uint4*>(lds + r * S + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
+      const int e = tid + i * THREADS, r = e / Tl::kChunks;
+      if (kEven || e < kPieces)
+        *reinterpret_cast<uint4*>(lds + r * S + (e % Tl::kChunks) * 16) = (bits >> r) & 1 ? v[i] : make_uint4(0, 0, 0, 0);
     }
   }
   template <int S> __device__ __forceinline__ void put(char* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int e = tid + i * kThreads;
-      *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * S + (e % Tl::kChunks) * 16) = v[i];
+      const int e = tid + i * THREADS;
+      if (kEven || e < kPieces) *reinterpret_cast<uint4*>(lds + (e / Tl::kChunks) * S + (e % Tl::kChunks) * 16) = v[i];
     }
   }
 };

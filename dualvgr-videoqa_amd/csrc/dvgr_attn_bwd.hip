@@ -86,16 +86,19 @@ template <typename T, int NT> __device__ __forceinline__ void write_dq(const Bwd
 }
 
 // ---- dK, dV: KW x 32 keys of one key head, RW x RS x 32 packed rows a turn -------------------------------------------------------
-// (The accumulators are 2 DP / 32 x 16 registers; up to 96 two waves of a SIMD hold theirs, at 128 one.)
+// A wave holds 2 DP / 32 x 16 accumulators and its keys' operands; at 128 two-byte values wait in LDS instead (VL), so that two waves of a
+// SIMD fit: one alone spent 40 % of its time waiting for LDS.
 template <typename T, int DP, int KW, int RW, int RS>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 2 : 1)) void k_attn_dkv(BwdArgs B) {
+__global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) void k_attn_dkv(BwdArgs B) {
   const Args& A = B.f;
   typedef Tile<T, DP> Tl;
-  constexpr int RT = RW * RS * 32, KT = KW * 32, NT = Tl::kNT;
+  constexpr int RT = RW * RS * 32, KT = KW * 32, NT = Tl::kNT, NTHR = 64 * KW * RW;
+  constexpr bool VL = sizeof(T) == 2 && DP == 128 && KW > 1;
   extern __shared__ __align__(16) char lds[];
   char* lq = lds;
   char* lg = lq + Tl::template bytesT<RT>();
   float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [lse, D][RT]
+  char* lval = reinterpret_cast<char*>(lstat + 2 * RT);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * ktiles);
@@ -106,14 +109,20 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)b * A.a.mask_stride : nullptr;
   const bool there = key < n && (!mask || mask[key]);
 
-  Frag<T> kf[Tl::kSteps], vf[Tl::kSteps];
+  Frag<T> kf[Tl::kSteps], vf[VL ? 1 : Tl::kSteps];
+  lval += kw * Tl::template bytes<32>();
   {
     const char* kr = k_side(A, A.a.k, b, hk).row(there ? key : 0);
     const char* vr = k_side(A, A.a.v, b, hk).row(there ? key : 0);
 #pragma unroll
-    for (int s = 0; s < Tl::kSteps; ++s) { kf[s] = Tl::gfrag(kr, s, lane, dhb, there); vf[s] = Tl::gfrag(vr, s, lane, dhb, there); }
+    for (int s = 0; s < Tl::kSteps; ++s) {
+      kf[s] = Tl::gfrag(kr, s, lane, dhb, there);
+      const Frag<T> x = Tl::gfrag(vr, s, lane, dhb, there);
+      if constexpr (!VL) vf[s] = x;
+      else if (rw == 0) *reinterpret_cast<Frag<T>*>(lval + (lane & 31) * Tl::kStride + s * 32 + (lane >> 5) * 16) = x;
+    }
     settle(kf);
-    settle(vf);
+    if constexpr (!VL) settle(vf);
   }
   f32x16 dk[NT], dv[NT];
 #pragma unroll
@@ -122,7 +131,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
   const Side qs = q_side(A, A.a.q, b, hk), gs = q_side(A, B.g_o, b, hk);
   const int rtiles = kt * KT < n ? (A.rows + RT - 1) / RT : 0;                   // keys behind the sample's: zeros
 
-  Stage<T, DP, RT> sq, sg;
+  Stage<T, DP, RT, NTHR> sq, sg;
   float stat = 0.f;
   const float* from = tid < RT ? A.a.lse : B.delta;
   const auto fetch = [&](int t) {
@@ -147,7 +156,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 96 && RW == 1 ? 
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tq, st, lane), kf[st], s);
 #pragma unroll
-      for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::fragT(tg, st, lane), vf[st], dp);
+      for (int st = 0; st < Tl::kSteps; ++st) {
+        if constexpr (VL) dp = mma(Tl::fragT(tg, st, lane), Tl::frag(lval, st, lane), dp);
+        else dp = mma(Tl::fragT(tg, st, lane), vf[st], dp);
+      }
       const float* ls = lstat + (rw * RS + i) * 32 + (lane >> 5) * 4;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -531,14 +543,14 @@ template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t w
   DVGR_LAUNCH(kern, dim3(xcd_grid(work)), dim3(threads), bytes, st, B);
   return (int)hipGetLastError();
 }
-size_t join_bytes(int waves, int NT) { return waves > 1 ? (size_t)kWaves * NT * 16 * 64 * sizeof(float) : 0; }
 
 template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float);
-  if (bytes < join_bytes(RW, Tl::kNT)) bytes = join_bytes(RW, Tl::kNT);
-  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), kThreads, bytes, B, st);
+  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
+  const size_t join = RW > 1 ? (size_t)KW * RW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
+  if (bytes < join) bytes = join;
+  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), 64 * KW * RW, bytes, B, st);
 }
 template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
   static std::atomic<uint32_t> asked{0};
@@ -558,11 +570,12 @@ template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream
   return (int)hipGetLastError();
 }
 
-// Few keys for many rows: the four waves share them and go over different rows.
+// 128 keys of a workgroup: four waves, and four more on other rows where two of a SIMD fit (two-byte types).  Few keys for many rows: four
+// waves share them and go over different rows.
 template <typename T, int DP> int launch_many(const BwdArgs& B, hipStream_t st) {
-  constexpr int S = sizeof(T) == 4 ? 1 : 2;                         // a turn of the shared arrangement: 32 rows of fp32, 64 of two bytes
+  constexpr int S = sizeof(T) == 4 ? 1 : 2;                         // a turn: 32 rows (keys) of fp32, 64 of two bytes
   if (B.f.a.Lk && B.g_k.p) {
-    const int e = B.f.a.Lk <= 32 ? launch_dkv<T, DP, 1, 4, 1>(B, st) : launch_dkv<T, DP, 4, 1, S>(B, st);
+    const int e = B.f.a.Lk <= 32 ? launch_dkv<T, DP, 1, 4, 1>(B, st) : launch_dkv<T, DP, 4, S, 1>(B, st);
     if (e) return e;
   }
   return B.g_q.p ? launch_dq<T, DP, S>(B, st) : 0;
