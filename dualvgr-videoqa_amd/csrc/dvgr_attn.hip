@@ -2,8 +2,9 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax (in powers of two: scale and log2 e are one factor).
 // The H / Hk query heads that share a key head are rows of the same tiles, so a key is read once for all of them.  Many rows: a
-// workgroup of four waves takes 128 rows and shares tiles of keys in LDS.  Up to 32 rows: the waves go over different keys and are
-// joined at the end (dvgr_attn_few.h); the keys are split over workgroups, joined by a second launch, while there are few of them.
+// workgroup of four waves takes 128 rows and shares tiles of keys in LDS.  Few rows: a workgroup takes 32, its waves go over different
+// keys and are joined at the end (dvgr_attn_few.h); the keys are split over workgroups, joined by a second launch, while there are
+// few of them.
 #include "dvgr_attn_few.h"
 
 namespace dvgr {
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
   if (live) write_row<T>(A, b, hk, row, o, m, l, 0, 1, true, lane);
 }
 
-// ---- up to 32 rows: KW waves over different keys -----------------------------------------------------------------------------------
+// ---- 32 rows: KW waves over different keys -----------------------------------------------------------------------------------------
 // (Two waves of a SIMD, in two-byte types, keep twice the loads in flight: the queries are read from LDS for it.)
 template <typename T, int DP, int KW>
 __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_fwd(Args A) {
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   char* lv = lk + Tl::template bytes<32>();
   const FewWork f = few_work<KW>(A, kw);
   if (!f.any) return;
-  const int dhb = A.a.Dh * A.es, row = lane & 31;
+  const int dhb = A.a.Dh * A.es, col = lane & 31, row = f.r0 + col;
   const bool live = row < A.rows;
   const Side ks = k_side(A, A.a.k, f.b, f.hk), vs = k_side(A, A.a.v, f.b, f.hk);
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)f.b * A.a.mask_stride : nullptr;
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   for (int e = threadIdx.x; e < 32 * Tl::kChunks; e += 64 * KW) {
     const int r = e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < A.rows && c < dhb) x = *reinterpret_cast<const uint4*>(q_side(A, A.a.q, f.b, f.hk).row(r) + c);
+    if (f.r0 + r < A.rows && c < dhb) x = *reinterpret_cast<const uint4*>(q_side(A, A.a.q, f.b, f.hk).row(f.r0 + r) + c);
     *reinterpret_cast<uint4*>(lq + r * Tl::kStride + c) = x;
   }
   __syncthreads();
@@ -194,11 +195,11 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
     __syncthreads();
     float mj = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) mj = fmaxf(mj, ml[k * 64 + row]);
+    for (int k = 0; k < KW; ++k) mj = fmaxf(mj, ml[k * 64 + col]);
     const float ref = mj == -INFINITY ? 0.f : mj, fac = exp2_fast(m - ref);
     l = 0.f;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) l += ml[k * 64 + 32 + row] * exp2_fast(ml[k * 64 + row] - ref);
+    for (int k = 0; k < KW; ++k) l += ml[k * 64 + 32 + col] * exp2_fast(ml[k * 64 + col] - ref);
     m = mj;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   }
   if (!live) return;
   if (A.splits > 1) {
-    const int64_t at = f.w * A.rows + row;
+    const int64_t at = (((int64_t)f.b * A.a.Hk + f.hk) * A.splits + f.split) * A.rows + row;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (t % KW != kw) continue;
@@ -311,7 +312,7 @@ template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t 
   const auto kern = k_attn_few_fwd<T, DP, KW>;
   int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
   if (e) return e;
-  DVGR_LAUNCH(kern, dim3(xcd_grid((int64_t)A.a.B * A.a.Hk * A.splits)), dim3(64 * KW), bytes, st, A);
+  DVGR_LAUNCH(kern, dim3(xcd_grid((int64_t)A.a.B * A.a.Hk * A.splits * ((A.rows + 31) / 32))), dim3(64 * KW), bytes, st, A);
   e = (int)hipGetLastError();
   if (e || A.splits == 1) return e;
   DVGR_LAUNCH((k_attn_join<T>), dim3((unsigned)((int64_t)A.a.B * A.a.Hk * A.rows)), dim3(256), 0, st, A);
@@ -319,7 +320,7 @@ template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t 
 }
 // (two-byte types take 64 keys a turn, fp32 32: the same bytes)
 template <typename T, int DP> int launch_dp(const Args& A, int KW, hipStream_t st) {
-  if (A.rows > 32) return launch_many<T, DP, sizeof(T) == 4 ? 1 : 2>(A, st);
+  if (!KW) return launch_many<T, DP, sizeof(T) == 4 ? 1 : 2>(A, st);
   if constexpr (sizeof(T) == 2)
     if (KW == 8) return launch_few<T, DP, 8>(A, st);
   return KW == 1 ? launch_few<T, DP, 1>(A, st) : launch_few<T, DP, 4>(A, st);
@@ -335,7 +336,6 @@ struct Parts { FewPlan few; size_t o_bytes, ml_bytes; };
 Parts parts(const dvgr_attn_problem& a) {
   Parts p{};
   const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk);
-  if (rows > 32) return p;
   p.few = few_plan(a, true);
   if (p.few.splits > 1) {
     p.o_bytes = (size_t)a.B * a.Hk * p.few.splits * rows * a.Dh * sizeof(float);          // (rows of 8 floats at least: 16-byte aligned)
@@ -414,7 +414,7 @@ int dvgr_attn_forward(const dvgr_attn_problem* a, void* workspace, size_t worksp
     if (workspace_bytes < p.o_bytes + p.ml_bytes) return DVGR_E_WORKSPACE;
     if (!ptr16(workspace)) return DVGR_E_ALIGN;
   }
-  if (p.few.splits) {
+  if (p.few.KW) {
     A.splits = p.few.splits;
     A.tiles_per_split = p.few.tiles_per_split;
   }

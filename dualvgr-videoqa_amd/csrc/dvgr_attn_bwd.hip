@@ -26,6 +26,8 @@ struct BwdArgs {
   dvgr_attn_view g_o, g_q, g_k, g_v;
   float* delta;                     // (B, H, Lq)
   uint32_t* top;                    // (B, Hk): bits of the largest |dO| (fp16)
+  Shares rs;                        // of the packed rows, for dK and dV
+  float* part_kv;                   // rs.splits > 1: (split, B, Hk, Lk, [dK, dV], Dh)
 };
 
 __global__ __launch_bounds__(256) void k_attn_clear(uint32_t* p, int64_t n) {
@@ -33,37 +35,48 @@ __global__ __launch_bounds__(256) void k_attn_clear(uint32_t* p, int64_t n) {
   if (i < n) p[i] = 0u;
 }
 
-// D of a packed row: 16 lanes per row
+// D of the packed rows: a workgroup takes kDeltaRows of one key head, 16 lanes a row (one atomic for all of them: one for each row
+// took 1.4 ms where few heads have many rows)
+constexpr int kDeltaRows = 64;
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
   const Args& A = B.f;
-  const int lane = threadIdx.x & 15;
-  const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (i >= (int64_t)A.a.B * A.a.Hk * A.rows) return;
-  const int row = (int)(i % A.rows), hk = (int)(i / A.rows % A.a.Hk), b = (int)(i / A.rows / A.a.Hk);
-  const T* o = (const T*)q_side(A, A.a.o, b, hk).row(row);
-  const T* g = (const T*)q_side(A, B.g_o, b, hk).row(row);
-  const T* lo = (const T*)lo_row<T>(A, b, hk, row);
+  const int lane = threadIdx.x & 15, tiles = (A.rows + kDeltaRows - 1) / kDeltaRows;
+  const int r0 = (int)(blockIdx.x % tiles) * kDeltaRows + (threadIdx.x >> 4), hk = (int)(blockIdx.x / tiles % A.a.Hk), b = (int)(blockIdx.x / tiles / A.a.Hk);
+  const Side os = q_side(A, A.a.o, b, hk), gs = q_side(A, B.g_o, b, hk);
   constexpr int N = Vec16<T>::N;
-  float s = 0.f, top = 0.f;
-  for (int d = lane * N; d < A.a.Dh; d += 16 * N) {
-    float x[N], y[N];
-    load_vec(o + d, x);
-    load_vec(g + d, y);
+  float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) { s += x[j] * y[j]; top = fmaxf(top, fabsf(y[j])); }
-    if (lo) {
-      load_vec(lo + d, x);
+  for (int i = 0; i < kDeltaRows / 16; ++i) {
+    const int row = r0 + i * 16;
+    float s = 0.f;
+    if (row < A.rows) {
+      const T* o = (const T*)os.row(row);
+      const T* g = (const T*)gs.row(row);
+      const T* lo = (const T*)lo_row<T>(A, b, hk, row);
+      for (int d = lane * N; d < A.a.Dh; d += 16 * N) {
+        float x[N], y[N];
+        load_vec(o + d, x);
+        load_vec(g + d, y);
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += x[j] * y[j];
+        for (int j = 0; j < N; ++j) { s += x[j] * y[j]; top = fmaxf(top, fabsf(y[j])); }
+        if (lo) {
+          load_vec(lo + d, x);
+#pragma unroll
+          for (int j = 0; j < N; ++j) s += x[j] * y[j];
+        }
+      }
     }
-  }
 #pragma unroll
-  for (int d = 8; d; d >>= 1) { s += __shfl_xor(s, d); top = fmaxf(top, __shfl_xor(top, d)); }
-  if (lane == 0) {
-    B.delta[row_index(A, b, hk, row)] = s;
-    if (Grad16<T>::on) atomicMax(&B.top[b * A.a.Hk + hk], __float_as_uint(top));
+    for (int d = 8; d; d >>= 1) s += __shfl_xor(s, d);
+    if (lane == 0 && row < A.rows) B.delta[row_index(A, b, hk, row)] = s;
   }
+  if (!Grad16<T>::on) return;
+  __shared__ float sh[4];
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) atomicMax(&B.top[b * A.a.Hk + hk], __float_as_uint(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]))));
 }
 
 // score gradient as the matrix unit takes it
@@ -71,16 +84,22 @@ template <typename T> __device__ __forceinline__ float grad16(float ds, float sc
   return Grad16<T>::on ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
 }
 
-template <typename T, int NT> __device__ __forceinline__ void write_dq(const BwdArgs& B, int b, int hk, int row, const f32x16 (&dq)[NT], float f, int first,
-                                                                       int step, int lane) {
-  char* out = const_cast<char*>(q_side(B.f, B.g_q, b, hk).row(row));
+// a row of dQ, or of its part from one share of the keys
+template <typename T, int NT> __device__ __forceinline__ void write_dq(const BwdArgs& B, int b, int hk, int split, int row, const f32x16 (&dq)[NT], float f,
+                                                                       int first, int step, int lane) {
+  const Args& A = B.f;
+  char* out = const_cast<char*>(q_side(A, B.g_q, b, hk).row(row));
+  float* part = A.part_o + ((((int64_t)b * A.a.Hk + hk) * A.splits + split) * A.rows + row) * A.a.Dh;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if (t % step != first) continue;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * t + 8 * g + (lane >> 5) * 4;
-      if (d < B.f.a.Dh) store4<T>(out + d * sizeof(T), dq[t][4 * g] * f, dq[t][4 * g + 1] * f, dq[t][4 * g + 2] * f, dq[t][4 * g + 3] * f);
+      if (d >= A.a.Dh) continue;
+      const float4 x = make_float4(dq[t][4 * g] * f, dq[t][4 * g + 1] * f, dq[t][4 * g + 2] * f, dq[t][4 * g + 3] * f);
+      if (A.splits > 1) *reinterpret_cast<float4*>(part + d) = x;
+      else store4<T>(out + d * sizeof(T), x.x, x.y, x.z, x.w);
     }
   }
 }
@@ -101,9 +120,10 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   char* lval = reinterpret_cast<char*>(lstat + 2 * RT);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
-  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * ktiles);
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * B.rs.splits * ktiles);
   if (w < 0) return;
-  const int kt = (int)(w % ktiles), hk = (int)(w / ktiles % A.a.Hk), b = (int)(w / ktiles / A.a.Hk);
+  const int kt = (int)(w % ktiles), split = (int)(w / ktiles % B.rs.splits);
+  const int hk = (int)(w / ktiles / B.rs.splits % A.a.Hk), b = (int)(w / ktiles / B.rs.splits / A.a.Hk);
   const int n = key_count(A, b), dhb = A.a.Dh * A.es;
   const int key = kt * KT + kw * 32 + (lane & 31);
   const uint8_t* mask = A.a.mask ? A.a.mask + (int64_t)b * A.a.mask_stride : nullptr;
@@ -129,7 +149,8 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   for (int t = 0; t < NT; ++t) dk[t] = dv[t] = zero16();
   const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
   const Side qs = q_side(A, A.a.q, b, hk), gs = q_side(A, B.g_o, b, hk);
-  const int rtiles = kt * KT < n ? (A.rows + RT - 1) / RT : 0;                   // keys behind the sample's: zeros
+  const int turns = kt * KT < n ? (A.rows + RT - 1) / RT : 0, t0 = split * B.rs.turns_per_split;           // keys behind the sample's: zeros
+  const int t1 = t0 + B.rs.turns_per_split < turns ? t0 + B.rs.turns_per_split : turns;
 
   Stage<T, DP, RT, NTHR> sq, sg;
   float stat = 0.f;
@@ -140,14 +161,14 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     const int r = t * RT + tid % RT;
     if (tid < 2 * RT) stat = from[row_index(A, b, hk, r < A.rows ? r : A.rows - 1)];
   };
-  if (rtiles) fetch(0);
-  for (int t = 0; t < rtiles; ++t) {
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
     __syncthreads();
     sq.template put<Tl::kStrideT>(lq, tid);
     sg.template put<Tl::kStrideT>(lg, tid);
     if (tid < 2 * RT) lstat[tid] = t * RT + tid % RT < A.rows ? stat : tid < RT ? INFINITY : 0.f;      // (no row: p = 0)
     __syncthreads();
-    if (t + 1 < rtiles) fetch(t + 1);
+    if (t + 1 < t1) fetch(t + 1);
 #pragma unroll 1
     for (int i = 0; i < RS; ++i) {
       const char* tq = lq + (rw * RS + i) * 32 * Tl::kStrideT;
@@ -203,6 +224,21 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   }
   if (key >= A.a.Lk) return;
   const float f = A.a.scale / sc;
+  if (B.rs.splits > 1) {
+    float* out = B.part_kv + ((((int64_t)split * A.a.B + b) * A.a.Hk + hk) * A.a.Lk + key) * 2 * A.a.Dh;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (RW > 1 && t % RW != rw) continue;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * t + 8 * g + (lane >> 5) * 4;
+        if (d >= A.a.Dh) continue;
+        *reinterpret_cast<float4*>(out + d) = make_float4(dk[t][4 * g] * f, dk[t][4 * g + 1] * f, dk[t][4 * g + 2] * f, dk[t][4 * g + 3] * f);
+        *reinterpret_cast<float4*>(out + A.a.Dh + d) = make_float4(dv[t][4 * g], dv[t][4 * g + 1], dv[t][4 * g + 2], dv[t][4 * g + 3]);
+      }
+    }
+    return;
+  }
   char* gk = const_cast<char*>(k_side(A, B.g_k, b, hk).row(key));
   char* gv = const_cast<char*>(k_side(A, B.g_v, b, hk).row(key));
 #pragma unroll
@@ -218,6 +254,27 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   }
 }
 
+// dK and dV from the shares of the rows, added in order: 4 elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(BwdArgs B) {
+  const Args& A = B.f;
+  const int per = A.a.Dh / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)A.a.B * A.a.Hk * A.a.Lk * 2;
+  if (i >= rows * per) return;
+  const int d = (int)(i % per) * 4;
+  const int64_t row = i / per, key = row / 2;
+  const float4* at = reinterpret_cast<const float4*>(B.part_kv + row * A.a.Dh + d);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < B.rs.splits; ++s) {
+    const float4 y = at[(int64_t)s * rows * per];
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
+  const int b = (int)(key / A.a.Lk / A.a.Hk), hk = (int)(key / A.a.Lk % A.a.Hk);
+  char* out = const_cast<char*>(k_side(A, row & 1 ? B.g_v : B.g_k, b, hk).row((int)(key % A.a.Lk)));
+  store4<T>(out + d * sizeof(T), x.x, x.y, x.z, x.w);
+}
+
 // ---- dQ: 4 x 32 packed rows, KS x 32 keys a turn (the forward's arrangement) ---------------------------------------------------
 template <typename T, int DP, int KS>
 __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
@@ -229,10 +286,12 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   char* lv = lds + Tl::template bytesT<KT>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rtiles = (A.rows + RT - 1) / RT;
-  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles);
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits * rtiles);
   if (w < 0) return;
-  const int rt = (int)(w % rtiles), hk = (int)(w / rtiles % A.a.Hk), b = (int)(w / rtiles / A.a.Hk);
-  const int n = key_count(A, b), dhb = A.a.Dh * A.es, tn = (n + KT - 1) / KT;
+  const int rt = (int)(w % rtiles), split = (int)(w / rtiles % A.splits);
+  const int hk = (int)(w / rtiles / A.splits % A.a.Hk), b = (int)(w / rtiles / A.splits / A.a.Hk);
+  const int n = key_count(A, b), dhb = A.a.Dh * A.es, turns = (n + KT - 1) / KT, t0 = split * A.tiles_per_split;
+  const int t1 = t0 + A.tiles_per_split < turns ? t0 + A.tiles_per_split : turns;
   const int row = rt * RT + wave * 32 + (lane & 31);
   const bool live = row < A.rows;
   const Side ks = k_side(A, A.a.k, b, hk), vs = k_side(A, A.a.v, b, hk);
@@ -263,14 +322,14 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
     sv.fetch(vs, t * KT, n, dhb, tid);
     there = key_there(mask, t * KT + lane, lane < KT ? n : 0);
   };
-  if (tn) fetch(0);
-  for (int t = 0; t < tn; ++t) {
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
     const unsigned long long bits = __ballot(there != 0);
     __syncthreads();
     sk.template put<Tl::kStrideT>(lk, bits, tid);
     sv.template put<Tl::kStride>(lv, bits, tid);
     __syncthreads();
-    if (t + 1 < tn) fetch(t + 1);
+    if (t + 1 < t1) fetch(t + 1);
 #pragma unroll 1
     for (int i = 0; i < KS; ++i) {
       if (!(uint32_t)(bits >> (32 * i))) continue;                  // (uniform over the wave)
@@ -290,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
       mma_tr<DP>(dq, tk, s, lane, T());
     }
   }
-  if (live) write_dq<T>(B, b, hk, row, dq, A.a.scale / sc, 0, 1, lane);
+  if (live) write_dq<T>(B, b, hk, split, row, dq, A.a.scale / sc, 0, 1, lane);
 }
 
 // ---- up to 32 rows: KW waves over different keys, everything in one pass ---------------------------------------------------------
@@ -497,18 +556,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
     }
   }
   if (col >= A.rows) return;
-  if (A.splits == 1) { write_dq<T>(B, f.b, f.hk, col, dq, fac, kw, KW, lane); return; }
-#pragma unroll
-  for (int u = 0; u < NT; ++u) {
-    if (u % KW != kw) continue;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * u + 8 * g + h4;
-      if (d < A.a.Dh)
-        *reinterpret_cast<float4*>(A.part_o + (f.w * A.rows + col) * A.a.Dh + d) =
-            make_float4(dq[u][4 * g] * fac, dq[u][4 * g + 1] * fac, dq[u][4 * g + 2] * fac, dq[u][4 * g + 3] * fac);
-    }
-  }
+  write_dq<T>(B, f.b, f.hk, f.split, col, dq, fac, kw, KW, lane);
 }
 
 // dQ from the shares of the keys: a workgroup per packed row, its waves take every fourth share, added in the waves' order
@@ -534,8 +582,6 @@ __global__ __launch_bounds__(256) void k_attn_dq_join(BwdArgs B) {
   out[d + 1] = (T)(sh[0][d + 1] + sh[1][d + 1] + sh[2][d + 1] + sh[3][d + 1]);
 }
 
-size_t delta_bytes(const dvgr_attn_problem& a) { return ((size_t)a.B * a.H * a.Lq * sizeof(float) + 255) / 256 * 256; }
-
 template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t work, int threads, size_t bytes, const BwdArgs& B,
                                 hipStream_t st) {
   const int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
@@ -550,12 +596,23 @@ template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdAr
   size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
   const size_t join = RW > 1 ? (size_t)KW * RW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
   if (bytes < join) bytes = join;
-  return launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), 64 * KW * RW, bytes, B, st);
+  const int64_t keys = (int64_t)B.f.a.B * B.f.a.Hk * B.f.a.Lk;
+  const int e = launch(k_attn_dkv<T, DP, KW, RW, RS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * B.rs.splits * ((B.f.a.Lk + KW * 32 - 1) / (KW * 32)), 64 * KW * RW,
+                       bytes, B, st);
+  if (e || B.rs.splits == 1) return e;
+  DVGR_LAUNCH((k_attn_dkv_join<T>), dim3((unsigned)((keys * 2 * (B.f.a.Dh / 4) + 255) / 256)), dim3(256), 0, st, B);
+  return (int)hipGetLastError();
+}
+template <typename T> int join_dq(const BwdArgs& B, hipStream_t st) {
+  if (B.f.splits == 1 || !B.f.rows) return 0;
+  DVGR_LAUNCH((k_attn_dq_join<T>), dim3((unsigned)((int64_t)B.f.a.B * B.f.a.Hk * B.f.rows)), dim3(256), 0, st, B);
+  return (int)hipGetLastError();
 }
 template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
   static std::atomic<uint32_t> asked{0};
-  return launch(k_attn_dq<T, DP, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * ((B.f.rows + kWaves * 32 - 1) / (kWaves * 32)), kThreads,
+  const int e = launch(k_attn_dq<T, DP, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * B.f.splits * ((B.f.rows + kWaves * 32 - 1) / (kWaves * 32)), kThreads,
                 Tile<T, DP>::template bytes<KS * 32>() + Tile<T, DP>::template bytesT<KS * 32>(), B, st);
+  return e ? e : join_dq<T>(B, st);
 }
 template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
@@ -563,11 +620,9 @@ template <typename T, int DP, int KW> int launch_few(const BwdArgs& B, hipStream
   size_t bytes = FewLds<T, DP>::kBytes(KW);
   const size_t join = KW > 1 ? (size_t)KW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
   if (bytes < join) bytes = join;
-  const int64_t units = (int64_t)B.f.a.B * B.f.a.Hk;
+  const int64_t units = (int64_t)B.f.a.B * B.f.a.Hk;                // (one tile of rows; without rows one that has none)
   const int e = launch(k_attn_few_bwd<T, DP, KW>, asked, units * B.f.splits, 64 * KW, bytes, B, st);
-  if (e || B.f.splits == 1 || !B.g_q.p || !B.f.rows) return e;
-  DVGR_LAUNCH((k_attn_dq_join<T>), dim3((unsigned)(units * B.f.rows)), dim3(256), 0, st, B);
-  return (int)hipGetLastError();
+  return e || !B.g_q.p ? e : join_dq<T>(B, st);
 }
 
 // 128 keys of a workgroup: four waves, and four more on other rows where two of a SIMD fit (two-byte types).  Few keys for many rows: four
@@ -586,9 +641,9 @@ template <typename T, int DP> int launch_dp(const BwdArgs& B, int KW, hipStream_
 
 template <typename T> int launch_t(const BwdArgs& B, int KW, hipStream_t st) {
   if (!KW) {
-    const int64_t rows = (int64_t)B.f.a.B * B.f.a.Hk * B.f.rows, groups = (int64_t)B.f.a.B * B.f.a.Hk;
+    const int64_t groups = (int64_t)B.f.a.B * B.f.a.Hk;
     if (Grad16<T>::on) DVGR_LAUNCH(k_attn_clear, dim3((unsigned)((groups + 255) / 256)), dim3(256), 0, st, B.top, groups);
-    DVGR_LAUNCH((k_attn_delta<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, B);
+    DVGR_LAUNCH((k_attn_delta<T>), dim3((unsigned)(groups * ((B.f.rows + kDeltaRows - 1) / kDeltaRows))), dim3(256), 0, st, B);
     const int e = (int)hipGetLastError();
     if (e) return e;
   }
@@ -600,26 +655,42 @@ template <typename T> int launch_t(const BwdArgs& B, int KW, hipStream_t st) {
 
 }  // namespace
 
-size_t backward_bytes(const dvgr_attn_problem& a) {
-  const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk);
-  if (rows <= 32) {
-    const FewPlan p = few_plan(a, false);
-    return p.splits > 1 ? (size_t)a.B * a.Hk * p.splits * rows * a.Dh * sizeof(float) : 0;
+namespace {
+// Workgroups of both passes of many rows: split where there is less than one for each compute unit, in shares of at least four turns.
+struct BwdPlan { FewPlan few; Shares ks, rs; size_t delta, top, part_q, part_kv, total; };
+BwdPlan bwd_plan(const dvgr_attn_problem& a) {
+  BwdPlan p{};
+  const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk), heads = (int64_t)a.B * a.Hk;
+  const int turn = a.elem == DVGR_ELEM_F32 ? 32 : 64;               // rows or keys of a turn
+  p.few = few_plan(a, false);
+  p.ks = p.rs = Shares{1, 1 << 30};
+  if (p.few.KW) p.ks = Shares{p.few.splits, p.few.tiles_per_split};
+  else {
+    const int64_t qu = heads * ((rows + 127) / 128), ku = heads * (a.Lk <= 32 ? 1 : (a.Lk + 127) / 128);
+    if (qu < 256) p.ks = shares_of(qu, (a.Lk + turn - 1) / turn, 512, 4);
+    if (ku < 256) p.rs = shares_of(ku, a.Lk <= 32 ? (rows + 127) / 128 : (rows + turn - 1) / turn, 512, 4);
   }
-  return delta_bytes(a) + (a.elem == DVGR_ELEM_F16 ? (size_t)a.B * a.Hk * sizeof(uint32_t) : 0);
+  size_t o = 0;
+  const auto take = [&o](size_t b) { const size_t at = o; o += (b + 255) / 256 * 256; return at; };
+  p.delta = take(p.few.KW ? 0 : (size_t)heads * rows * sizeof(float));
+  p.top = take(p.few.KW || a.elem != DVGR_ELEM_F16 ? 0 : (size_t)heads * sizeof(uint32_t));
+  p.part_q = take(p.ks.splits > 1 ? (size_t)heads * p.ks.splits * rows * a.Dh * sizeof(float) : 0);
+  p.part_kv = take(p.rs.splits > 1 ? (size_t)heads * p.rs.splits * a.Lk * 2 * a.Dh * sizeof(float) : 0);
+  p.total = o;
+  return p;
 }
+}  // namespace
+
+size_t backward_bytes(const dvgr_attn_problem& a) { return bwd_plan(a).total; }
 
 int launch_backward(const Args& A, const dvgr_attn_grads& g, void* ws, hipStream_t st) {
-  BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, nullptr, nullptr};
-  int KW = 0;
-  if (A.rows <= 32) {
-    const FewPlan p = few_plan(A.a, false);
-    B.f.splits = p.splits; B.f.tiles_per_split = p.tiles_per_split; B.f.part_o = (float*)ws;
-    KW = p.KW;
-  } else {
-    B.delta = (float*)ws;
-    B.top = (uint32_t*)((char*)ws + delta_bytes(A.a));
-  }
+  const BwdPlan p = bwd_plan(A.a);
+  char* at = (char*)ws;
+  BwdArgs B{A, g.g_o, g.g_q, g.g_k, g.g_v, (float*)(at + p.delta), (uint32_t*)(at + p.top), p.rs, (float*)(at + p.part_kv)};
+  B.f.splits = p.ks.splits;
+  B.f.tiles_per_split = p.ks.turns_per_split;
+  B.f.part_o = (float*)(at + p.part_q);
+  const int KW = p.few.KW;
   return A.a.elem == DVGR_ELEM_F32 ? launch_t<float>(B, KW, st) : A.a.elem == DVGR_ELEM_BF16 ? launch_t<bf16_t>(B, KW, st) : launch_t<f16_t>(B, KW, st);
 }
 

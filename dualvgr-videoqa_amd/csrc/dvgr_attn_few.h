@@ -1,5 +1,5 @@
 // dvgr_attn_few.h -- attention where one 32-row tile holds all packed rows of a key head (a word over a video, a question over its
-// frames): bound by the keys' and values' memory, so the waves of a workgroup go over different keys at their own pace.  A wave
+// frames), or where larger tiles would leave most of the chip idle: bound by the keys' and values' memory, so the waves of a workgroup go over different keys at their own pace.  A wave
 // reads its 32 keys a row at a time (whole lines; read straight as operands, 32 bytes of 32 rows each, they fell out of the cache
 // between the steps) into LDS of its own; nothing waits for another wave before the end.
 #pragma once
@@ -46,20 +46,21 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// where a wave of a workgroup stands: key head, share of the keys, its first 32-key tile (it goes on in steps of KW)
+// where a wave of a workgroup stands: 32 rows of a key head, share of the keys, its first 32-key tile (it goes on in steps of KW)
 struct FewWork {
-  int b, hk, split, n, t0, t1;
-  int64_t w;
+  int b, hk, split, r0, n, t0, t1;
   bool any;
 };
 template <int KW> __device__ __forceinline__ FewWork few_work(const Args& A, int kw) {
   FewWork f{};
-  f.w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits);
-  f.any = f.w >= 0;
+  const int rtiles = A.rows > 32 ? (A.rows + 31) / 32 : 1;         // (without rows: one tile, for the keys' zeros)
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits * rtiles);
+  f.any = w >= 0;
   if (!f.any) return f;
-  f.split = (int)(f.w % A.splits);
-  f.hk = (int)(f.w / A.splits % A.a.Hk);
-  f.b = (int)(f.w / A.splits / A.a.Hk);
+  f.r0 = (int)(w % rtiles) * 32;
+  f.split = (int)(w / rtiles % A.splits);
+  f.hk = (int)(w / rtiles / A.splits % A.a.Hk);
+  f.b = (int)(w / rtiles / A.splits / A.a.Hk);
   f.n = key_count(A, f.b);
   const int tiles = (f.n + 31) / 32, per = A.tiles_per_split * KW;
   f.t0 = f.split * per + kw;
@@ -67,21 +68,33 @@ template <int KW> __device__ __forceinline__ FewWork few_work(const Args& A, int
   return f;
 }
 
+// Work in shares: `units` workgroups of `turns` turns each are split until there are `want` of them, in shares of at least `least` turns.
+struct Shares { int splits, turns_per_split; };
+inline Shares shares_of(int64_t units, int64_t turns, int64_t want, int least) {
+  int64_t s = units ? want / units : 1;
+  if (s > turns / least) s = turns / least;
+  if (s < 1) s = 1;
+  Shares x{};
+  x.turns_per_split = (int)((turns + s - 1) / s);
+  if (x.turns_per_split < 1) x.turns_per_split = 1;
+  x.splits = turns ? (int)((turns + x.turns_per_split - 1) / x.turns_per_split) : 1;
+  return x;
+}
+
 // Waves of a workgroup and shares of the keys.  Up to 64 keys one wave does it all; otherwise four, and eight in the forward of two-byte
 // types while there are fewer than two workgroups for each compute unit (eight fill its registers as two of four do, with half the
 // shares to join).  The keys are split over workgroups while there are fewer than that, in shares of at least two turns.
+// KW = 0: the kernels for many rows, which have no need of it: every compute unit has a workgroup of 128 rows.  (The backward adds up
+// over all rows at once, so it takes at most 32.)
 struct FewPlan { int KW, splits, tiles_per_split; };
 inline FewPlan few_plan(const dvgr_attn_problem& a, bool forward) {
   FewPlan p{};
-  const int64_t units = (int64_t)a.B * a.Hk;
+  const int64_t rows = (int64_t)a.Lq * (a.H / a.Hk), heads = (int64_t)a.B * a.Hk, units = heads * ((rows + 31) / 32);
+  if (rows > 32 && (!forward || heads * ((rows + 127) / 128) >= 256)) return p;
   p.KW = a.Lk <= 64 ? 1 : forward && a.elem != DVGR_ELEM_F32 && units < 512 ? 8 : 4;
-  const int64_t turns = ((int64_t)a.Lk + p.KW * 32 - 1) / (p.KW * 32);
-  int64_t s = units ? (p.KW == 8 ? 256 : 512) / units : 1;
-  if (s > turns / 2) s = turns / 2;
-  if (s < 1) s = 1;
-  p.tiles_per_split = (int)((turns + s - 1) / s);
-  if (p.tiles_per_split < 1) p.tiles_per_split = 1;
-  p.splits = turns ? (int)((turns + p.tiles_per_split - 1) / p.tiles_per_split) : 1;
+  const Shares s = shares_of(units, ((int64_t)a.Lk + p.KW * 32 - 1) / (p.KW * 32), p.KW == 8 ? 256 : 512, 2);
+  p.splits = s.splits;
+  p.tiles_per_split = s.turns_per_split;
   return p;
 }
 

@@ -154,6 +154,16 @@ def test_one_word_over_a_long_video_splits_the_keys(t, B, H, Hk, Lk, Dh):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,Dh", [(1, 50, 2100, 2, 1, 64), (1, 3000, 20, 2, 1, 96), (2, 700, 300, 3, 1, 128), (1, 33, 1300, 1, 1, 40),
+                                             (3, 1025, 65, 2, 2, 32)])
+def test_small_batches_are_split_over_keys_and_rows(t, B, Lq, Lk, H, Hk, Dh):
+    q, k, v, gen = tensors(B, Lq, Lk, H, Hk, Dh, t)
+    a, b = check(q, k, v), check(q, k, v)
+    assert torch.equal(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[1], b[1]))
+    check(q, k, v, torch.randint(0, Lk + 1, (B,), generator=gen, device="cuda"), torch.rand(B, Lk, generator=gen, device="cuda") < 0.8)
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_strides_and_alignment(t):
     q, k, v, gen = tensors(2, 20, 70, 4, 2, 64, t)
     want = check(q, k, v)
