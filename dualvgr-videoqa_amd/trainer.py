@@ -16,6 +16,9 @@ flat segments (include/dvgr_optim.h) instead of PyTorch's per-tensor loops.  `st
 Data parallel (one process per GPU): pass `world` and the reducers; every rank's losses are means over its shard, the
 batch-SUM HSIC term is multiplied by `world`, and gradients are AVERAGED before the clip, so the
 step equals the single-process step on the concatenated batch.
+
+A teacher's top answers can take part: `TrainStep(..., distill_weight=w, distill_temperature=T)` and `step(..., teacher=(values,
+indices))` add w * distillation_loss(logits, values, indices, T) to the loss (losses.distillation_loss).
 """
 from __future__ import annotations
 
@@ -25,6 +28,7 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _lib as L_
+from .losses import distillation_loss
 
 
 class OptimSeg(C.Structure):
@@ -141,8 +145,11 @@ class TrainStep:
     tensors (nothing is synchronised): {'loss', 'ce', 'common', 'dependence', 'grad_sqnorm', 'logits'}."""
 
     def __init__(self, model, lr: float = 1e-4, alpha: float = 1.0, beta: float = 1e-8, max_norm: float = 12.0,
-                 betas=(0.9, 0.999), eps: float = 1e-8, world: int = 1, unit_reducer=None, param_reducer=None):
+                 betas=(0.9, 0.999), eps: float = 1e-8, world: int = 1, unit_reducer=None, param_reducer=None,
+                 distill_weight: float = 0.0, distill_temperature: float = 2.0):
         self.model = model
+        self.distill_weight, self.distill_temperature = float(distill_weight), float(distill_temperature)
+        self._distill_up = None                      # the weight as the upstream gradient of the distillation term
         self.unit = model.visual_input_unit
         self.head = model._head
         self.alpha, self.beta, self.world = float(alpha), float(beta), int(world)
@@ -253,7 +260,10 @@ class TrainStep:
         if "max_norm" in sd:
             self.opt.max_norm = float(sd["max_norm"])
 
-    def __call__(self, video_appearance_feat, video_motion_feat, question, question_len, answers):
+    def __call__(self, video_appearance_feat, video_motion_feat, question, question_len, answers, teacher=None):
+        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None."""
+        if (teacher is None) != (self.distill_weight == 0.0):
+            raise ValueError("a teacher's top logits and distill_weight != 0 go together")
         m, unit, head = self.model, self.unit, self.head
         # optimizer.zero_grad() (train.py:139): the unit's flat buffer is simply overwritten by the next backward
         unit.zero_grad_flat()
@@ -269,7 +279,14 @@ class TrainStep:
         ce, g_logits = head.cross_entropy(logits, answers)                   # train.py:147, value + gradient in one launch
         terms, g = unit.last_loss                                            # {0, mean_l common, mean_l dependence}, upstream grads
         raw = m.last_raw                                                     # (L, B, N, D) list tensors as the kernels wrote them
-        torch.autograd.backward([logits, raw[3], raw[4], raw[5], raw[6]], [g_logits, g[3], g[4], g[5], g[6]])
+        roots, ups, kd = [logits, raw[3], raw[4], raw[5], raw[6]], [g_logits, g[3], g[4], g[5], g[6]], None
+        if teacher is not None:
+            kd = distillation_loss(logits, *teacher, self.distill_temperature)
+            if self._distill_up is None or self._distill_up.device != kd.device:
+                self._distill_up = torch.full_like(kd, self.distill_weight, requires_grad=False)
+            roots.append(kd)
+            ups.append(self._distill_up)
+        torch.autograd.backward(roots, ups)
         if self.unit_reducer is not None and not self._unit_shared:
             self.unit_reducer.finish()
         if self.param_reducer is not None:
@@ -291,4 +308,8 @@ class TrainStep:
         if self.timing is not None:
             self.timing["end"].record()
         loss = ce[0] + self.alpha * terms[1] + self.beta * terms[2]
-        return {"loss": loss, "ce": ce[0], "common": terms[1], "dependence": terms[2], "grad_sqnorm": sq[0], "logits": logits}
+        out = {"loss": loss, "ce": ce[0], "common": terms[1], "dependence": terms[2], "grad_sqnorm": sq[0], "logits": logits}
+        if kd is not None:
+            out["distill"] = kd.detach()
+            out["loss"] = loss + self.distill_weight * out["distill"]
+        return out

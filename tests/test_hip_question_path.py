@@ -1,0 +1,234 @@
+"""GPU: the question-side operators as a program uses them -- together, in the training step, and where they refuse."""
+import pytest
+import torch
+import torch.nn as nn
+
+import dualvgr_videoqa_amd as dv
+from dualvgr_videoqa_amd import synth
+from test_hip_model import model_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+class Reader(nn.Module):
+    """words -> embedding -> attention to the video's frames -> answers"""
+
+    def __init__(self, words, answers, dim, frames_dim):
+        super().__init__()
+        self.embed = dv.TokenEmbedding(words, dim, padding_idx=0, scale=dim ** 0.5)
+        self.attend = dv.CrossAttention(dim, 4, state_dim=frames_dim, key_heads=2)
+        self.answer = dv.HipLinear(dim, answers)
+
+    def forward(self, tokens, frames, lens):
+        x = self.embed(tokens)
+        return self.answer((x + self.attend(x, frames, lens)).mean(1))
+
+
+def plain(sd, tokens, frames, lens, values, indices, T, dim):
+    """the same program in 64 bits on the CPU: (loss, gradients)"""
+    p = {k: v.detach().cpu().double().requires_grad_(True) for k, v in sd.items()}
+    x = p["embed.weight"][tokens] * dim ** 0.5
+    lin = lambda n, z: z @ p[n + ".weight"].t() + p[n + ".bias"]  # noqa: E731
+    B, L, _ = x.shape
+    q = lin("attend.query", x).view(B, L, 4, dim // 4)
+    kv = lin("attend.key_value", frames.double()).view(B, -1, 2, 2, dim // 4)
+    k, v = kv[:, :, 0].repeat_interleave(2, 2), kv[:, :, 1].repeat_interleave(2, 2)
+    s = torch.einsum("blhd,bjhd->bhlj", q, k) * (dim // 4) ** -0.5
+    s = s.masked_fill(torch.arange(k.shape[1]) >= lens.view(-1, 1, 1, 1), -torch.inf)
+    o = torch.einsum("bhlj,bjhd->blhd", s.softmax(3), v).reshape(B, L, dim)
+    z = lin("answer", (x + lin("attend.out", o)).mean(1))
+    logp, logq = torch.log_softmax(values.double() / T, 1), torch.log_softmax(z / T, 1).gather(1, indices)
+    loss = (logp.exp() * (logp - logq)).sum(1).mean() * T * T
+    loss.backward()
+    grads = {k: t.grad for k, t in p.items()}
+    grads["embed.weight"][0] = 0
+    return float(loss.detach()), grads
+
+
+def test_embedding_attention_and_distillation_together():
+    torch.manual_seed(3)
+    dim, B, L, F = 64, 6, 7, 90
+    m = Reader(50, 40, dim, 48).cuda()
+    g = torch.Generator().manual_seed(4)
+    tokens, frames = torch.randint(0, 50, (B, L), generator=g), torch.randn(B, F, 48, generator=g)
+    lens = torch.tensor([90, 1, 33, 64, 65, 17])
+    values, indices = torch.randn(B, 40, generator=g).topk(5, 1)
+    args = tokens.cuda(), frames.cuda(), lens.cuda()
+    loss = dv.distillation_loss(m(*args), values.cuda(), indices.cuda(), 2.0)
+    loss.backward()
+    want, grads = plain(m.state_dict(), tokens, frames, lens, values, indices, 2.0, dim)
+    # fp32 throughout: chains of dot products of up to 128 terms, a few 2^-24 of their size each
+    assert abs(float(loss.detach()) - want) <= 2e-5 * abs(want)
+    for n, p in m.named_parameters():
+        off = (p.grad.cpu().double() - grads[n]).abs().max()
+        assert float(off) <= 5e-5 * float(grads[n].abs().max()) + (1e-7 if n == "attend.key_value.bias" else 0), (n, float(off))
+    again = {n: p.grad.clone() for n, p in m.named_parameters()}
+    m.zero_grad()
+    dv.distillation_loss(m(*args), values.cuda(), indices.cuda(), 2.0).backward()
+    assert torch.equal(m.embed.weight.grad, again["embed.weight"])
+    m.embed.check_tokens()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def test_one_pass_of_gradient_steps_runs():
+    torch.manual_seed(5)
+    m = Reader(30, 20, 64, 48).cuda()
+    opt = torch.optim.SGD(m.parameters(), lr=0.1)
+    values, indices = torch.randn(8, 20, device="cuda").topk(4, 1)
+    for i in range(3):
+        opt.zero_grad()
+        z = m(torch.randint(0, 30, (8, 5), device="cuda"), torch.randn(8, 40, 48, device="cuda"), torch.randint(1, 41, (8,), device="cuda"))
+        dv.distillation_loss(z, values, indices).backward()
+        opt.step()
+    assert all(torch.isfinite(p).all() for p in m.parameters())
+
+
+def small_step(weight, teacher_on, lr=0.0):
+    V, D, Wd, N, Fr, Lr, B, T, vq, va = 64, 64, 32, 5, 3, 2, 8, 6, 40, 10
+    vocab = {"question_token_to_idx": {str(i): i for i in range(vq)}, "answer_token_to_idx": {str(i): i for i in range(va)}}
+    torch.manual_seed(11)
+    m = dv.DualVGR(vision_dim=V, module_dim=D, word_dim=Wd, vocab=vocab, num_of_nodes=N, graph_module="GAT", graph_layers=1, unit_layers=Lr, dtype="fp32")
+    m = m.cuda().train().set_dropout_enabled(False)
+    app, mot, q, qlen = [torch.from_numpy(x).cuda() for x in model_inputs(B, N, Fr, V, T, vq, 5)]
+    answers = torch.arange(B).cuda() % va
+    g = torch.Generator().manual_seed(6)
+    values, indices = torch.randn(B, va, generator=g).topk(4, 1)
+    indices[2] = -1                                                 # a pair the teacher says nothing about
+    teacher = (values.cuda(), indices.cuda())
+    step = dv.TrainStep(m, lr=lr, max_norm=1e9, distill_weight=weight, distill_temperature=2.0)
+    out = step(app, mot, q, qlen, answers, teacher=teacher if teacher_on else None)
+    grads = {n: p.grad.clone() for n, p in step.other}
+    return out, grads, step.unit.last_flat_grad.clone(), teacher
+
+
+def test_a_teacher_in_the_training_step():
+    base, g0, u0, _ = small_step(0.0, False)
+    assert "distill" not in base
+    one, g1, u1, teacher = small_step(0.5, True)
+    two, g2, u2, _ = small_step(1.0, True)
+    z = one["logits"].detach().requires_grad_(True)
+    kd = dv.distillation_loss(z, *teacher, 2.0)
+    gz, = torch.autograd.grad(kd, z)
+    assert torch.equal(one["distill"], kd.detach())
+    # the cross entropy adds its 8 terms atomically: each of 8 roundings is half a step of at most the sum, in either run
+    assert abs(float(one["ce"] - base["ce"])) <= 2 * 8 * 2.0 ** -24 * float(base["ce"])
+    assert abs(float(one["loss"] - base["loss"]) - 0.5 * float(kd.detach())) <= 1e-6 * float(one["loss"])
+    # the last bias sees the logits' gradient alone: the sum over the 8 pairs of (q - p) / 8, whose q moves by no more than the logits do
+    # from run to run (the step adds atomically; the forward's own gate is 1e-4 of their size)
+    bias = [n for n in g0 if n.endswith("classifier.5.bias")][0]
+    noise = 1e-4 * float(z.detach().abs().max())
+    for w, g in ((0.5, g1), (1.0, g2)):
+        assert float(((g[bias] - g0[bias]) - w * gz.sum(0)).abs().max()) <= noise
+    assert float(gz.sum(0).abs().max()) > 20 * noise
+    assert float((u2 - u0).abs().max()) > 0
+    with pytest.raises(ValueError):
+        small_step(0.0, True)
+    with pytest.raises(ValueError):
+        small_step(0.5, False)
+
+
+def test_refusals_on_the_device():
+    t = lambda *s, **k: torch.zeros(*s, device="cuda", **k)  # noqa: E731
+    ids = t(3, dtype=torch.int64)
+    for bad, args in (("takes fp32", (t(4, 8, dtype=torch.float64), ids)), ("integers", (t(4, 8), t(3))), ("integers", (t(4, 8), t(3, dtype=torch.bool))),
+                      ("vocab, wd", (t(4), ids)), ("vocab, wd", (t(0, 8), ids)), ("tokens are on", (t(4, 8), ids.cpu()))):
+        with pytest.raises(RuntimeError, match=bad):
+            dv.embed_tokens(*args)
+    for p in (4, -5):
+        with pytest.raises(RuntimeError, match="padding_idx"):
+            dv.embed_tokens(t(4, 8), ids, padding_idx=p)
+    with pytest.raises(RuntimeError, match="one int32"):
+        dv.embed_tokens(t(4, 8), ids, bad=t(1))
+
+    z, v, i = t(2, 9), t(2, 3), t(2, 3, dtype=torch.int64)
+    for bad, args in (("takes fp32", (z.double(), v, i)), ("logits \\(", (z, v, i[:1])), ("logits \\(", (z, v[:1], i[:1])), ("int64 or int32", (z, v, v)),
+                      ("one device", (z, v, i.cpu())), ("entries a row", (z, t(2, 0), t(2, 0, dtype=torch.int64))),
+                      ("entries a row", (t(2, 2000), t(2, 1025), t(2, 1025, dtype=torch.int64))), ("temperature", (z, v, i, 0.0)),
+                      ("temperature", (z, v, i, float("nan"))), ("reduction", (z, v, i, 1.0, "batchmean"))):
+        with pytest.raises(RuntimeError, match=bad):
+            dv.distillation_loss(*args)
+
+    q, k = t(2, 3, 4, 16), t(2, 5, 2, 16)
+    for bad, args in (("takes fp32", (q.double(), k.double(), k.double())), ("one type", (q, k.half(), k.half())), ("one device", (q, k.cpu(), k)),
+                      ("q \\(B", (q[0], k, k)), ("q \\(B", (q, k, k[:, :4])), ("q \\(B", (q[:1], k, k)), ("multiple of the key heads", (q[:, :, :3], k, k)),
+                      ("head size", (t(2, 3, 4, 12), t(2, 5, 2, 12), t(2, 5, 2, 12))), ("head size", (t(2, 3, 4, 136), t(2, 5, 2, 136), t(2, 5, 2, 136))),
+                      ("lens", (q, k, k, t(3, dtype=torch.int64))), ("lens", (q, k, k, t(2))), ("lens", (q, k, k, torch.zeros(2, dtype=torch.int64))),
+                      ("mask", (q, k, k, None, t(2, 5))), ("mask", (q, k, k, None, t(2, 4, dtype=torch.bool))), ("scale", (q, k, k, None, None, 0.0)),
+                      ("scale", (q, k, k, None, None, -1.0)), ("scale", (q, k, k, None, None, float("inf")))):
+        with pytest.raises(RuntimeError, match=bad):
+            dv.cross_attention(*args)
+    with pytest.raises(RuntimeError, match="states or the keys"):
+        dv.CrossAttention(64, 2).cuda()(t(1, 4, 64))
+
+
+def test_a_gradient_says_when_it_is_differentiated_again():
+    table = torch.randn(5, 8, device="cuda", requires_grad=True)
+    up = torch.randn(3, 8, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(dv.embed_tokens(table, torch.arange(3, device="cuda")), table, up, create_graph=True)
+    assert torch.equal(g.detach()[:3], up.detach())
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        g.sum().backward()
+    z = torch.randn(2, 9, device="cuda", requires_grad=True)
+    loss = dv.distillation_loss(z, torch.randn(2, 3, device="cuda"), torch.zeros(2, 3, device="cuda", dtype=torch.int64))
+    loss.backward(retain_graph=True)
+    first = z.grad.clone()
+    loss.backward()                                                 # twice over one graph: the gradients add up
+    assert torch.equal(z.grad, 2 * first)
+    with pytest.raises(RuntimeError):
+        loss.backward()                                             # its tensors are gone
+    q = torch.randn(1, 2, 1, 8, device="cuda", requires_grad=True)
+    o = dv.cross_attention(q, q.detach(), q.detach())
+    with torch.no_grad():
+        q.add_(1.0)                                                 # what the backward needs is not what it was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+
+
+@pytest.mark.parametrize("which", ["distil", "attend"])
+def test_captured_backwards_refuse_while_an_eager_graph_of_a_leaf_lives(which):
+    x = torch.randn(2, 6, 1, 16, device="cuda", requires_grad=True)
+    v, i = torch.randn(2, 3, device="cuda"), torch.zeros(2, 3, device="cuda", dtype=torch.int64)
+    z = torch.randn(2, 16, device="cuda", requires_grad=True)
+    call = (lambda: dv.distillation_loss(z, v, i)) if which == "distil" else (lambda: dv.cross_attention(x, x, x).sum())
+    leaf = z if which == "distil" else x
+    alive = dv.distillation_loss(z, v, i) if which == "distil" else dv.cross_attention(x, x, x)
+    up = torch.ones((), device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+        with pytest.raises(RuntimeError, match="captured while"):
+            torch.autograd.grad(out, leaf, up)
+        del out
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g, = torch.autograd.grad(call(), leaf, up)
+    want, = torch.autograd.grad(call(), leaf, up)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(g, want)
+
+
+def test_two_streams_at_once():
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q = torch.randn(4, 40, 4, 64, generator=gen, device="cuda").bfloat16().requires_grad_(True)
+    kv = torch.randn(4, 900, 4, 64, generator=gen, device="cuda").bfloat16()
+    table = torch.randn(9000, 64, generator=gen, device="cuda", requires_grad=True)
+    tokens = torch.randint(0, 9000, (9000,), generator=gen, device="cuda")
+    up = torch.randn(9000, 64, generator=gen, device="cuda")
+
+    def work():
+        o = dv.cross_attention(q, kv, kv)
+        return [o.detach(), *torch.autograd.grad(o, q, torch.ones_like(o)), *torch.autograd.grad(dv.embed_tokens(table, tokens), table, up)]
+
+    want = work()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
