@@ -19,7 +19,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens: tor
     fp32, bf16 or fp16; Dh a multiple of 8 up to 128; H a multiple of Hk (query head h reads key head h // (H // Hk)).  Any strides
     (heads that do not start at multiples of 16 bytes are copied first).  Key j of sample b is there if j < lens[b] (integers (B),
     clamped to [0, Lk]) and mask[b, j] (bool (B, Lk)); keys that are not there are never used, NaN included, and get zero gradients.
-    A query without keys gives zeros.  scale > 0, default 1 / sqrt(Dh).  Without a gradient wanted (one word at a time, serving)
+    A query without keys gives zeros.  1e-30 <= scale <= 1e30, default 1 / sqrt(Dh).  Without a gradient wanted (one word at a time, serving)
     nothing is kept for a backward."""
     return L_.torch_ops().cross_attention(q, k, v, lens, mask, scale)
 

@@ -323,7 +323,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   TORCH_CHECK(Dh % 8 == 0 && Dh >= 8 && Dh <= 128, what, ": the head size is a multiple of 8 up to 128; got ", Dh);
   for (const int64_t s : {B, Lq, Lk, H}) TORCH_CHECK(s < (1ll << 30), what, ": a dimension of ", s, " is too large");
   const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)Dh);
-  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), what, ": scale is a positive number; got ", scale);
+  TORCH_CHECK(scale >= 1e-30 && scale <= 1e30, what, ": scale is a positive number, 1e-30 to 1e30; got ", scale);
   const c10::DeviceGuard guard(q.device());
   const hipStream_t st = stream_of(q);
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());

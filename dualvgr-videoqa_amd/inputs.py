@@ -140,16 +140,14 @@ class TokenEmbedding(nn.Embedding):
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale: float = 1.0):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx)
         self.scale = float(scale)
-        self._bad = None
+        self.register_buffer("_bad", torch.zeros(1, dtype=torch.int32), persistent=False)
 
     def forward(self, tokens):
-        if self._bad is None or self._bad.device != self.weight.device:
-            self._bad = torch.zeros(1, device=self.weight.device, dtype=torch.int32)
         return embed_tokens(self.weight, tokens, self.scale, self.padding_idx, self._bad)
 
     def check_tokens(self):
         """Synchronises: raises if any call so far met a token outside the table (torch raises at the lookup itself)."""
-        if self._bad is not None and int(self._bad.item()) != 0:
+        if int(self._bad.item()) != 0:
             self._bad.zero_()
             raise IndexError("TokenEmbedding: a token is outside the embedding table")
 

@@ -27,13 +27,13 @@ typedef struct dvgr_attn_view {
 typedef struct dvgr_attn_problem {
   int32_t B, Lq, Lk;       /* samples, queries and keys of a sample; any may be 0                        */
   int32_t H, Hk;           /* query heads, key heads; H a multiple of Hk                                 */
-  int32_t Dh;              /* head size: a multiple of 8, 8 .. 128                                       */
+  int32_t Dh;              /* head size: a multiple of 8, 8 .. 128.  B Hk (Lq H / Hk / 64 + 1) < 2^24, B Hk (Lk / 128 + 1) < 2^23 */
   int32_t elem;            /* DVGR_ELEM_*                                                                */
-  float scale;             /* > 0                                                                        */
+  float scale;             /* 1e-30 .. 1e30                                                              */
   dvgr_attn_view q, k, v;
   dvgr_attn_view o;        /* written by the forward, read by the backward                               */
-  void *o_lo;              /* bf16 / fp16, (B, Lq, H, Dh) contiguous, or NULL: what o's rounding left, to the type; the forward fills it and
-                              the backward takes rowsum(g_o o) with it, which halves the error of the score gradients' common part */
+  void *o_lo;              /* bf16 / fp16, (B, Lq, H, Dh) contiguous, or NULL: what o's rounding left, rounded to the type.  The forward
+                              fills it; with it the backward's rowsum(g_o o) is that of the unrounded output            */
   const int64_t *lens;     /* (B) number of keys, clamped to [0, Lk], or NULL: Lk                        */
   const uint8_t *mask;     /* (B, Lk) 0 / 1, rows `mask_stride` bytes apart, or NULL                     */
   int64_t mask_stride;
