@@ -210,7 +210,7 @@ struct DistillNode : OpNode {
     const Tensor z = logits_.unpack(), v = values_.unpack(), i = indices_.unpack(), stats = stats_.unpack(), g = grads[0].contiguous();
     const int64_t R = z.size(0), C = z.size(1);
     Tensor out = at::empty({R, C}, z.options());
-    check(E.distill_backward(z.data_ptr(), z.stride(0), elem_code(z, what), R, C, v.data_ptr(), elem_code(v, what), i.data_ptr<int64_t>(), (int)v.size(1),
+    check(E.distill_backward(z.data_ptr(), R > 1 ? z.stride(0) : C, elem_code(z, what), R, C, v.data_ptr(), elem_code(v, what), i.data_ptr<int64_t>(), (int)v.size(1),
                              temperature, stats.data_ptr<float>(), g.data_ptr<float>(), reduction ? 0 : 1, out.data_ptr(), C, stream_of(z)),
           "dvgr_distill_backward");
     return {out};

@@ -144,6 +144,17 @@ def test_strided_logits_and_leading_dimensions():
     assert torch.equal(dv.distillation_loss(last, v, idx, 2.0), want)
 
 
+def test_a_single_row_that_is_a_column_of_another_tensor():
+    x = torch.randn(37, 1, generator=torch.Generator().manual_seed(8)).cuda().requires_grad_(True)
+    z = x.t()                                                       # (1, 37), its one row's stride is 1
+    assert z.stride() == (1, 1)
+    v, idx = torch.randn(1, 3, generator=torch.Generator().manual_seed(9)).cuda(), torch.tensor([[4, 0, 36]], device="cuda")
+    dv.distillation_loss(z, v, idx, 1.5).backward()
+    y = x.detach().t().clone().requires_grad_(True)
+    dv.distillation_loss(y, v, idx, 1.5).backward()
+    assert torch.equal(x.grad.t(), y.grad)
+
+
 def test_gradient_against_differences():
     z, v, idx = case(6, 77, 9, torch.float32, 9)
     gen = torch.Generator(device="cuda").manual_seed(10)
