@@ -79,9 +79,9 @@ __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
   if (threadIdx.x == 0) atomicMax(&B.top[b * A.a.Hk + hk], __float_as_uint(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]))));
 }
 
-// score gradient as the matrix unit takes it
+// score gradient as the matrix unit takes it; infinities and NaN stay what they are (a scaled loss that overflows is found by them)
 template <typename T> __device__ __forceinline__ float grad16(float ds, float sc) {
-  return Grad16<T>::on ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
+  return Grad16<T>::on && fabsf(ds) < INFINITY ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
 }
 
 // a row of dQ, or of its part from one share of the keys
@@ -223,6 +223,10 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     }
   }
   if (key >= A.a.Lk) return;
+  if (!there) {                                                     // zeros, where an infinite upstream gradient times p = 0 is NaN
+#pragma unroll
+    for (int t = 0; t < NT; ++t) dk[t] = dv[t] = zero16();
+  }
   const float f = A.a.scale / sc;
   if (B.rs.splits > 1) {
     float* out = B.part_kv + ((((int64_t)split * A.a.B + b) * A.a.Hk + hk) * A.a.Lk + key) * 2 * A.a.Dh;
@@ -447,8 +451,12 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 #pragma unroll
   for (int t = 0; t < NT; ++t) dq[t] = zero16();
   // acc, 32 keys of tile t, to their rows of a gradient
-  const auto leave = [&](const dvgr_attn_view& v, int t, float x) {
+  const auto leave = [&](const dvgr_attn_view& v, int t, float x, uint32_t bits) {
     const Side to = k_side(A, v, f.b, f.hk);
+    if (bits != ~0u && !((bits >> col) & 1)) {                      // zeros, where an infinite upstream gradient times p = 0 is NaN
+#pragma unroll
+      for (int u = 0; u < NT; ++u) acc[u] = zero16();
+    }
     if constexpr (kOut) {
       wave_order();
 #pragma unroll
@@ -521,18 +529,18 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 #pragma unroll
       for (int u = 0; u < NT; ++u) acc[u] = zero16();
       mma_tr<DP>(acc, lg, s, lane, T());
-      leave(B.g_v, t, 1.f);
+      leave(B.g_v, t, 1.f, bits);
 #pragma unroll
       for (int u = 0; u < NT; ++u) acc[u] = zero16();
       mma_tr<DP>(acc, lq, dp, lane, T());
-      leave(B.g_k, t, fac);
+      leave(B.g_k, t, fac, bits);
     }
   }
   if (B.g_k.p) {                                                    // keys behind the sample's last tile
     const int tiles = (A.a.Lk + 31) / 32, per = A.tiles_per_split * KW, t2 = (f.split + 1) * per < tiles ? (f.split + 1) * per : tiles;
 #pragma unroll
     for (int u = 0; u < NT; ++u) acc[u] = zero16();
-    for (; t < t2; t += KW) { leave(B.g_v, t, 1.f); leave(B.g_k, t, 1.f); }
+    for (; t < t2; t += KW) { leave(B.g_v, t, 1.f, ~0u); leave(B.g_k, t, 1.f, ~0u); }
   }
   if (!B.g_q.p) return;
   if (KW > 1) {

@@ -205,6 +205,25 @@ def test_small_upstream_gradients_of_half_precision_do_not_vanish():
         assert float((a.double() * 2.0 ** 9 - b.double()).abs().max()) <= float(b.double().abs().max()) * 2.0 ** -10 + 2.0 ** -25 * 2 ** 9
 
 
+@pytest.mark.parametrize("worst", [float("nan"), float("inf")])
+@pytest.mark.parametrize("Lq,Lk", [(5, 40), (5, 100), (40, 20), (40, 100)])
+@pytest.mark.parametrize("t", TYPES)
+def test_an_upstream_gradient_that_is_not_finite_reaches_what_it_touches(t, Lq, Lk, worst):
+    q, k, v, _ = tensors(2, Lq, Lk, 2, 1, 32, t)
+    mask = torch.ones(2, Lk, dtype=torch.bool, device="cuda")
+    mask[:, 3] = False
+    lens = torch.tensor([Lk - 2, Lk], device="cuda")
+    up = torch.ones_like(q)
+    up[0, 2, 1] = worst                                             # one query of one head of sample 0
+    gq, gk, gv = torch.autograd.grad(cross_attention(q, k, v, lens, mask), [q, k, v], up)
+    assert not torch.isfinite(gq[0, 2, 1]).any()
+    assert torch.isfinite(gq[0, 2, 0]).all() and torch.isfinite(gq[0, :2]).all() and torch.isfinite(gq[0, 3:]).all()
+    there = mask[0] & (torch.arange(Lk, device="cuda") < Lk - 2)
+    assert not torch.isfinite(gk[0][there]).any() and not torch.isfinite(gv[0][there]).any()
+    assert not gk[0][~there].any() and not gv[0][~there].any()
+    assert all(torch.isfinite(x[1]).all() for x in (gq, gk, gv))
+
+
 def test_gradients_against_differences():
     q, k, v, gen = tensors(2, 9, 40, 4, 2, 24, torch.float32, sharp=1.0)
     lens = torch.tensor([40, 23], device="cuda")
