@@ -149,7 +149,6 @@ class TrainStep:
                  distill_weight: float = 0.0, distill_temperature: float = 2.0):
         self.model = model
         self.distill_weight, self.distill_temperature = float(distill_weight), float(distill_temperature)
-        self._distill_up = None                      # the weight as the upstream gradient of the distillation term
         self.unit = model.visual_input_unit
         self.head = model._head
         self.alpha, self.beta, self.world = float(alpha), float(beta), int(world)
@@ -282,10 +281,8 @@ class TrainStep:
         roots, ups, kd = [logits, raw[3], raw[4], raw[5], raw[6]], [g_logits, g[3], g[4], g[5], g[6]], None
         if teacher is not None:
             kd = distillation_loss(logits, *teacher, self.distill_temperature)
-            if self._distill_up is None or self._distill_up.device != kd.device:
-                self._distill_up = torch.full_like(kd, self.distill_weight, requires_grad=False)
             roots.append(kd)
-            ups.append(self._distill_up)
+            ups.append(torch.full_like(kd, self.distill_weight, requires_grad=False))          # (a schedule may move the weight)
         torch.autograd.backward(roots, ups)
         if self.unit_reducer is not None and not self._unit_shared:
             self.unit_reducer.finish()

@@ -83,7 +83,7 @@ def test_one_pass_of_gradient_steps_runs():
     assert all(torch.isfinite(p).all() for p in m.parameters())
 
 
-def small_step(weight, teacher_on, lr=0.0):
+def small_step(weight, teacher_on, lr=0.0, keep=False):
     V, D, Wd, N, Fr, Lr, B, T, vq, va = 64, 64, 32, 5, 3, 2, 8, 6, 40, 10
     vocab = {"question_token_to_idx": {str(i): i for i in range(vq)}, "answer_token_to_idx": {str(i): i for i in range(va)}}
     torch.manual_seed(11)
@@ -98,7 +98,8 @@ def small_step(weight, teacher_on, lr=0.0):
     step = dv.TrainStep(m, lr=lr, max_norm=1e9, distill_weight=weight, distill_temperature=2.0)
     out = step(app, mot, q, qlen, answers, teacher=teacher if teacher_on else None)
     grads = {n: p.grad.clone() for n, p in step.other}
-    return out, grads, step.unit.last_flat_grad.clone(), teacher
+    first = out, grads, step.unit.last_flat_grad.clone(), teacher
+    return first + (step, (app, mot, q, qlen, answers)) if keep else first
 
 
 def test_a_teacher_in_the_training_step():
@@ -125,6 +126,20 @@ def test_a_teacher_in_the_training_step():
         small_step(0.0, True)
     with pytest.raises(ValueError):
         small_step(0.5, False)
+
+
+def test_the_weight_of_the_teacher_may_move_between_steps():
+    _, _, _, teacher, step, batch = small_step(0.5, True, keep=True)
+    bias = [n for n, _ in step.other if n.endswith("classifier.5.bias")][0]
+    seen = {}
+    for w in (0.5, 4.0):
+        step.distill_weight = w
+        out = step(*batch, teacher=teacher)
+        seen[w] = dict(step.other)[bias].grad.clone()
+    z = out["logits"].detach().requires_grad_(True)
+    gz, = torch.autograd.grad(dv.distillation_loss(z, *teacher, 2.0), z)
+    # (lr = 0: the logits are those of the first step up to its atomics, 1e-4 of their size as above)
+    assert float((seen[4.0] - seen[0.5] - 3.5 * gz.sum(0)).abs().max()) <= 1e-4 * float(z.detach().abs().max())
 
 
 def test_refusals_on_the_device():
