@@ -486,7 +486,7 @@ EmbedPlan embed_plan(int64_t n, int64_t vocab, int wd, int elem) {
 
 int embed_check(int64_t n, int64_t vocab, int wd, int elem) {
   if (!elem_size(elem)) return DVGR_E_KIND;
-  if (vocab < 1 || vocab >= (1ll << 31) - 1 || wd < 1 || wd >= (1 << 30) || n < 0 || n >= (1ll << 26)) return DVGR_E_DIMS;
+  if (vocab < 1 || vocab >= (1ll << 31) - 1 || wd < 1 || wd >= (1 << 30) || n < 0 || n > (1ll << 26) - 64) return DVGR_E_DIMS;
   if (n / kChunk * (wd / 256 + 1) >= (1ll << 23)) return DVGR_E_DIMS;            // a launch holds at most 2^32 threads
   return 0;
 }

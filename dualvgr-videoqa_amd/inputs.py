@@ -135,7 +135,8 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, 
 
 class TokenEmbedding(nn.Embedding):
     """nn.Embedding(num_embeddings, embedding_dim, padding_idx) on `embed_tokens`: same parameter, state_dict key and default init;
-    rows are multiplied by `scale` (sqrt(embedding_dim) in many language models)."""
+    rows are multiplied by `scale` (sqrt(embedding_dim) in many language models).  The flag of `check_tokens` is a buffer of this
+    process (a wrapper that broadcasts buffers between processes has to leave it out)."""
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale: float = 1.0):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx)

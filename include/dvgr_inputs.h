@@ -36,7 +36,7 @@ int dvgr_words_dbg_keep_mask(uint64_t seed, int64_t count, float *keep, void *st
 
 /* ---- token embedding with scaling, and its gradient by sorted tokens -------------------------------------------------------
  * Tensors of `elem` (DVGR_ELEM_*), rows of 1 <= `wd` < 2^30 elements, contiguous; any alignment of the element (16-byte aligned rows take
- * the vector path).  n < 2^26 positions, vocab < 2^31 - 1.
+ * the vector path).  n <= 2^26 - 64 positions, vocab < 2^31 - 1.
  *
  * y[i][:] = scale * table[tokens[i]][:].  A token outside [0, vocab) gives a row of zeros and sets *bad_tokens (int32, device,
  * nullable) to 1. */
