@@ -124,15 +124,28 @@ template <typename T, int DP, int ROWS, int THREADS = kThreads> struct Stage {
   uint4 v[N];
   // rows r0 .. of which those below `end` exist
   __device__ __forceinline__ void fetch(const Side& s, int r0, int end, int dh_bytes, int tid) {
+    const bool whole = kEven && r0 + ROWS <= end && dh_bytes == Tl::kRowBytes;          // (uniform: no zeros to write, no lane to switch off)
+    if (whole) load<true>(s, r0, end, dh_bytes, tid);
+    else load<false>(s, r0, end, dh_bytes, tid);
+  }
+  template <bool whole> __device__ __forceinline__ void load(const Side& s, int r0, int end, int dh_bytes, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * THREADS, r = r0 + e / Tl::kChunks, c = (e % Tl::kChunks) * 16;
+      if (whole) {
+        v[i] = *reinterpret_cast<const uint4*>(s.row(r) + c);
+        continue;
+      }
       v[i] = make_uint4(0, 0, 0, 0);
       if (r < end && c < dh_bytes && (kEven || e < kPieces)) v[i] = *reinterpret_cast<const uint4*>(s.row(r) + c);
     }
   }
   // rows without a bit are zeros, whatever was read
   template <int S> __device__ __forceinline__ void put(char* lds, unsigned long long bits, int tid) const {
+    if (bits == (ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1)) {
+      put<S>(lds, tid);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int e = tid + i * THREADS, r = e / Tl::kChunks;
@@ -187,8 +200,10 @@ template <typename T> __device__ __forceinline__ void store4(char* p, float a, f
 }
 
 // An 8-XCD chip hands workgroup i to XCD i % 8: give every XCD a contiguous run of the work, so that the workgroups that read the same
-// keys share an L2.  -1: nothing to do.
-__device__ __forceinline__ int64_t xcd_work(int64_t total) {
+// keys share an L2.  A head with 8 workgroups or more (`tiles`) has one on every XCD instead: samples of different lengths would leave
+// XCDs without work (captions over long videos of 50 to 100 % of 4096 states: dK and dV 750 us with runs, 620 without; the forward 340, 310).  -1: nothing to do.
+__device__ __forceinline__ int64_t xcd_work(int64_t total, int tiles = 1) {
+  if (tiles >= 8) return blockIdx.x < total ? (int64_t)blockIdx.x : -1;
   const int64_t per = (total + 7) / 8, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   return (int64_t)(blockIdx.x >> 3) < per && w < total ? w : -1;
 }

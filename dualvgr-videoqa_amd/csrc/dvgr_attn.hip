@@ -11,6 +11,8 @@ namespace dvgr {
 namespace attn {
 namespace {
 
+constexpr float kSlack = 8.f;
+
 // KS 32-key tiles of a wave's online softmax: s in, probabilities out, m, l and o brought to the new maximum
 template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (&s)[KS], unsigned long long bits, float c, float& m, float& l, f32x16 (&o)[NT],
                                                                         int lane) {
@@ -28,7 +30,9 @@ template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
   mx = half_max(mx) * c;
-  if (__any(mx > m)) {
+  // The maximum moves when a tile exceeds it by 2^kSlack in some row: p is at most 2^kSlack, as exact as any, and the accumulators are
+  // scaled again a few times in all instead of in every other tile.
+  if (__any(mx > m + kSlack)) {
     const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);      // nothing summed yet: o and l are 0
     l *= f;
 #pragma unroll
@@ -82,7 +86,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
   char* lv = lds + Tl::template bytes<KT>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rtiles = (A.rows + RT - 1) / RT;
-  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles);
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * rtiles, rtiles);
   if (w < 0) return;
   const int rt = (int)(w % rtiles), hk = (int)(w / rtiles % A.a.Hk), b = (int)(w / rtiles / A.a.Hk);
   const int n = key_count(A, b), dhb = A.a.Dh * A.es, tn = (n + KT - 1) / KT;

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   char* lval = reinterpret_cast<char*>(lstat + 2 * RT);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
-  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * B.rs.splits * ktiles);
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * B.rs.splits * ktiles, ktiles);
   if (w < 0) return;
   const int kt = (int)(w % ktiles), split = (int)(w / ktiles % B.rs.splits);
   const int hk = (int)(w / ktiles / B.rs.splits % A.a.Hk), b = (int)(w / ktiles / B.rs.splits / A.a.Hk);
@@ -189,9 +189,9 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * g + j;
-          const float p = there ? exp2_fast(fmaf(s[r], A.c, -ee[j])) : 0.f;
+          const float p = exp2_fast(fmaf(s[r], A.c, -ee[j]));       // (a key that is not there: its column alone, cleared at the end)
           s[r] = p;
-          dp[r] = there ? grad16<T>(p * (dp[r] - dd[j]), sc) : 0.f;
+          dp[r] = grad16<T>(p * (dp[r] - dd[j]), sc);
         }
       }
       mma_tr<DP>(dv, tg, s, lane, T());
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     }
   }
   if (key >= A.a.Lk) return;
-  if (!there) {                                                     // zeros, where an infinite upstream gradient times p = 0 is NaN
+  if (!there) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) dk[t] = dv[t] = zero16();
   }
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
   char* lv = lds + Tl::template bytesT<KT>();
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rtiles = (A.rows + RT - 1) / RT;
-  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits * rtiles);
+  const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * A.splits * rtiles, rtiles);
   if (w < 0) return;
   const int rt = (int)(w % rtiles), split = (int)(w / rtiles % A.splits);
   const int hk = (int)(w / rtiles / A.splits % A.a.Hk), b = (int)(w / rtiles / A.splits / A.a.Hk);
@@ -344,11 +344,12 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
       for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tk, st, lane), qf[st], s);
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tv, st, lane), gf[st], dp);
-      const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float ds = grad16<T>(exp2_fast(fmaf(s[r], A.c, -lse)) * (dp[r] - delta), sc);
-        s[r] = reg_bit(hb, r) ? ds : 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = grad16<T>(exp2_fast(fmaf(s[r], A.c, -lse)) * (dp[r] - delta), sc);
+      if ((uint32_t)(bits >> (32 * i)) != ~0u) {
+        const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = reg_bit(hb, r) ? s[r] : 0.f;
       }
       mma_tr<DP>(dq, tk, s, lane, T());
     }
@@ -509,7 +510,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * g + j;
-        const float p = here ? exp2_fast(fmaf(s[r], A.c, -ee[j])) : 0.f;
+        const float p = exp2_fast(fmaf(s[r], A.c, -ee[j]));         // (a key that is not there: its column alone, cleared as it leaves)
         s[r] = p;
         dp[r] = here ? grad16<T>(p * (dp[r] - dd[j]), sc) : 0.f;
         scr[(8 * g + h4 + j) * kScr + col] = dp[r];
