@@ -35,7 +35,10 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-constexpr int kThreads = 256, kWaves = 4;          // of the kernels for many rows
+// Waves of a workgroup for many rows, 32 rows each.  Eight fetch and write half as much of a tile each (captions over long videos: forward
+// 301 -> 288 us, dQ 400 -> 357), four make twice the workgroups: eight where every compute unit has one of them, and two waves of a SIMD fit
+// (two-byte types).
+inline int many_waves(int64_t heads, int64_t rows, int es) { return es == 2 && heads * ((rows + 255) / 256) >= 256 ? 8 : 4; }
 
 // One head's side of a tensor: row r of the packed rows (query l, head g of the group, r = l * G + g) or key r (G = 1).  Every thread
 // finds several rows' places in every turn, so this is kept to few instructions: a shift where G is a power of two, and products of
@@ -117,7 +120,7 @@ template <int DP> __device__ __forceinline__ void mma_tr(f32x16 (&acc)[DP / 32],
 
 // ROWS rows of a tensor on their way to LDS: fetched into registers one tile ahead, written behind the barrier that frees the tile.
 // Nothing between the two may look at what was fetched: the wait for it would be a wait for memory in every turn.
-template <typename T, int DP, int ROWS, int THREADS = kThreads> struct Stage {
+template <typename T, int DP, int ROWS, int THREADS> struct Stage {
   typedef Tile<T, DP> Tl;
   static constexpr int kPieces = ROWS * Tl::kChunks, N = (kPieces + THREADS - 1) / THREADS;
   static constexpr bool kEven = kPieces % THREADS == 0;             // otherwise the last round is some threads' only

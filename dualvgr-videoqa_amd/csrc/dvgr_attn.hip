@@ -76,11 +76,11 @@ template <typename T, int NT> __device__ __forceinline__ void write_row(const Ar
   if (A.a.lse && lane < 32 && stats) A.a.lse[row_index(A, b, hk, row)] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
-// ---- many rows: 4 x 32 of them, tiles of KS x 32 keys -----------------------------------------------------------------------------
-template <typename T, int DP, int KS>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(Args A) {
+// ---- many rows: W x 32 of them, tiles of KS x 32 keys -----------------------------------------------------------------------------
+template <typename T, int DP, int KS, int W>
+__global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(Args A) {
   typedef Tile<T, DP> Tl;
-  constexpr int KT = KS * 32, RT = kWaves * 32, NT = Tl::kNT;
+  constexpr int KT = KS * 32, RT = W * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   char* lk = lds;
   char* lv = lds + Tl::template bytes<KT>();
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd
   for (int t = 0; t < NT; ++t) o[t] = zero16();
   float m = -INFINITY, l = 0.f;
 
-  Stage<T, DP, KT> sk, sv;
+  Stage<T, DP, KT, 64 * W> sk, sv;
   uint32_t there = 0;                                               // lane j: key j of the next tile
   const auto fetch = [&](int t) {
     sk.fetch(ks, t * KT, n, dhb, tid);
@@ -298,13 +298,13 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
   if (A.a.lse && lane == 0) A.a.lse[row_index(A, b, hk, row)] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
-template <typename T, int DP, int KS> int launch_many(const Args& A, hipStream_t st) {
+template <typename T, int DP, int KS, int W> int launch_many(const Args& A, hipStream_t st) {
   const size_t bytes = Tile<T, DP>::template bytes<KS * 32>() + Tile<T, DP>::template bytesT<KS * 32>();
   static std::atomic<uint32_t> asked{0};
-  const auto kern = k_attn_fwd<T, DP, KS>;
+  const auto kern = k_attn_fwd<T, DP, KS, W>;
   const int e = allow_lds(reinterpret_cast<const void*>(kern), bytes, asked);
   if (e) return e;
-  DVGR_LAUNCH(kern, dim3(xcd_grid((int64_t)A.a.B * A.a.Hk * ((A.rows + kWaves * 32 - 1) / (kWaves * 32)))), dim3(kThreads), bytes, st, A);
+  DVGR_LAUNCH(kern, dim3(xcd_grid((int64_t)A.a.B * A.a.Hk * ((A.rows + W * 32 - 1) / (W * 32)))), dim3(64 * W), bytes, st, A);
   return (int)hipGetLastError();
 }
 template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t st) {
@@ -324,9 +324,11 @@ template <typename T, int DP, int KW> int launch_few(const Args& A, hipStream_t 
 }
 // (two-byte types take 64 keys a turn, fp32 32: the same bytes)
 template <typename T, int DP> int launch_dp(const Args& A, int KW, hipStream_t st) {
-  if (!KW) return launch_many<T, DP, sizeof(T) == 4 ? 1 : 2>(A, st);
-  if constexpr (sizeof(T) == 2)
+  if constexpr (sizeof(T) == 2) {
+    if (!KW && many_waves((int64_t)A.a.B * A.a.Hk, A.rows, 2) == 8) return launch_many<T, DP, 2, 8>(A, st);
     if (KW == 8) return launch_few<T, DP, 8>(A, st);
+  }
+  if (!KW) return launch_many<T, DP, sizeof(T) == 4 ? 1 : 2, 4>(A, st);
   return KW == 1 ? launch_few<T, DP, 1>(A, st) : launch_few<T, DP, 4>(A, st);
 }
 template <typename T> int launch_t(const Args& A, int KW, hipStream_t st) {

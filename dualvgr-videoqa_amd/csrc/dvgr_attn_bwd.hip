@@ -279,12 +279,12 @@ __global__ __launch_bounds__(256) void k_attn_dkv_join(BwdArgs B) {
   store4<T>(out + d * sizeof(T), x.x, x.y, x.z, x.w);
 }
 
-// ---- dQ: 4 x 32 packed rows, KS x 32 keys a turn (the forward's arrangement) ---------------------------------------------------
-template <typename T, int DP, int KS>
-__global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
+// ---- dQ: W x 32 packed rows, KS x 32 keys a turn (the forward's arrangement) ---------------------------------------------------
+template <typename T, int DP, int KS, int W>
+__global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(BwdArgs B) {
   const Args& A = B.f;
   typedef Tile<T, DP> Tl;
-  constexpr int KT = KS * 32, RT = kWaves * 32, NT = Tl::kNT;
+  constexpr int KT = KS * 32, RT = W * 32, NT = Tl::kNT;
   extern __shared__ __align__(16) char lds[];
   char* lk = lds;
   char* lv = lds + Tl::template bytesT<KT>();
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_dq(BwdArgs B) {
 #pragma unroll
   for (int t = 0; t < NT; ++t) dq[t] = zero16();
 
-  Stage<T, DP, KT> sk, sv;
+  Stage<T, DP, KT, 64 * W> sk, sv;
   uint32_t there = 0;
   const auto fetch = [&](int t) {
     sk.fetch(ks, t * KT, n, dhb, tid);
@@ -617,9 +617,9 @@ template <typename T> int join_dq(const BwdArgs& B, hipStream_t st) {
   DVGR_LAUNCH((k_attn_dq_join<T>), dim3((unsigned)((int64_t)B.f.a.B * B.f.a.Hk * B.f.rows)), dim3(256), 0, st, B);
   return (int)hipGetLastError();
 }
-template <typename T, int DP, int KS> int launch_dq(const BwdArgs& B, hipStream_t st) {
+template <typename T, int DP, int KS, int W> int launch_dq(const BwdArgs& B, hipStream_t st) {
   static std::atomic<uint32_t> asked{0};
-  const int e = launch(k_attn_dq<T, DP, KS>, asked, (int64_t)B.f.a.B * B.f.a.Hk * B.f.splits * ((B.f.rows + kWaves * 32 - 1) / (kWaves * 32)), kThreads,
+  const int e = launch(k_attn_dq<T, DP, KS, W>, asked, (int64_t)B.f.a.B * B.f.a.Hk * B.f.splits * ((B.f.rows + W * 32 - 1) / (W * 32)), 64 * W,
                 Tile<T, DP>::template bytes<KS * 32>() + Tile<T, DP>::template bytesT<KS * 32>(), B, st);
   return e ? e : join_dq<T>(B, st);
 }
@@ -642,7 +642,10 @@ template <typename T, int DP> int launch_many(const BwdArgs& B, hipStream_t st) 
     const int e = B.f.a.Lk <= 32 ? launch_dkv<T, DP, 1, 4, 1>(B, st) : launch_dkv<T, DP, 4, S, 1>(B, st);
     if (e) return e;
   }
-  return B.g_q.p ? launch_dq<T, DP, S>(B, st) : 0;
+  if (!B.g_q.p) return 0;
+  if constexpr (S == 2)
+    if (many_waves((int64_t)B.f.a.B * B.f.a.Hk, B.f.rows, 2) == 8) return launch_dq<T, DP, S, 8>(B, st);
+  return launch_dq<T, DP, S, 4>(B, st);
 }
 template <typename T, int DP> int launch_dp(const BwdArgs& B, int KW, hipStream_t st) {
   return KW == 1 ? launch_few<T, DP, 1>(B, st) : KW == 4 ? launch_few<T, DP, 4>(B, st) : launch_many<T, DP>(B, st);

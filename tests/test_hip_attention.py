@@ -205,6 +205,27 @@ def test_small_upstream_gradients_of_half_precision_do_not_vanish():
         assert float((a.double() * 2.0 ** 9 - b.double()).abs().max()) <= float(b.double().abs().max()) * 2.0 ** -10 + 2.0 ** -25 * 2 ** 9
 
 
+@pytest.mark.parametrize("shape", [(32, 33, 70, 8, 8, 40), (16, 257, 33, 16, 8, 96), (64, 100, 130, 4, 4, 128), (32, 1030, 64, 1, 1, 32), (64, 2100, 40, 1, 1, 64)])
+@pytest.mark.parametrize("t", TYPES)
+def test_many_rows_of_many_heads(t, shape):
+    q, k, v, gen = tensors(*shape, t)
+    B, _, Lk = shape[:3]
+    check(q, k, v, torch.randint(0, Lk + 1, (B,), generator=gen, device="cuda"), torch.rand(B, Lk, generator=gen, device="cuda") < 0.9)
+    check(q, k, v)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_scores_that_grow_and_fall_from_key_to_key(t):
+    # the running maximum moves by less and by more than 2^8 between tiles, up and down, in some rows only
+    B, Lq, Lk, H, Dh = 16, 130, 400, 16, 32
+    q, k, v, gen = tensors(B, Lq, Lk, H, H, Dh, t)
+    with torch.no_grad():
+        slope = torch.linspace(-3.0, 3.0, Lk, device="cuda")[None, :, None, None]
+        k.copy_((k.float() * slope.abs() + 0.4 * slope).to(t))
+    check(q, k, v)
+    check(q[:2].detach().requires_grad_(True), k[:2].detach().requires_grad_(True), v[:2].detach().requires_grad_(True))
+
+
 @pytest.mark.parametrize("worst", [float("nan"), float("inf")])
 @pytest.mark.parametrize("Lq,Lk", [(5, 40), (5, 100), (40, 20), (40, 100)])
 @pytest.mark.parametrize("t", TYPES)
