@@ -130,6 +130,7 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(A
     for (int st = 0; st < Tl::kSteps; ++st)
 #pragma unroll
       for (int i = 0; i < KS; ++i) s[i] = mma(Tl::frag(lk + i * 32 * Tl::kStride, st, lane), qf[st], s[i]);
+    if (sizeof(T) == 2) reads_ahead<KS * Tl::kSteps>();
     softmax_tiles(s, bits, A.c, m, l, o, lane);
 #pragma unroll
     for (int i = 0; i < KS; ++i) mma_tr<DP>(o, lv + i * 32 * Tl::kStrideT, s[i], lane, T());
