@@ -8,6 +8,8 @@
 // every workgroup picks the tokens of its own rows of the table; beyond, a stable radix sort of (token, position) pairs.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/dvgr.h"
 #include "../../include/dvgr_inputs.h"
 #include "dvgr_elem.h"
@@ -15,8 +17,12 @@
 namespace dvgr {
 namespace {
 
-// One wave per token position.  VEC: rows of 16-byte vectors; otherwise single elements, neighbouring lanes on neighbours.
-template <typename T, bool VEC>
+// Rows are handled V elements at a time: 16 bytes where rows start at multiples of 16 bytes, otherwise pairs where an even width allows it
+// (53291 x 806 fp16 of 19164 words, forward and backward: 198 us by single elements, 112 by pairs), otherwise single elements.  Neighbouring lanes take neighbouring pieces.
+template <typename T, int V> using Piece = T __attribute__((ext_vector_type(V)));
+
+// One wave per token position, a few pieces in flight.
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_embed_fwd(const T* __restrict__ table, int64_t vocab, int wd, const int64_t* __restrict__ tokens, int64_t n,
                                                    float scale, T* __restrict__ y, int32_t* bad) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -27,24 +33,21 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const T* __restrict__ table, 
   if (!ok && lane == 0 && bad) *bad = 1;
   T* dst = y + row * wd;
   const T* src = table + (ok ? tok : 0) * (int64_t)wd;
-  constexpr int N = Vec16<T>::N;
-  if (VEC) {
-    const int nv = wd / N;
-    for (int c = lane; c < nv; c += 128) {                          // two loads in flight
-      float f[N], g[N];
-      const bool more = c + 64 < nv;
-      load_vec(src + c * N, f);
-      if (more) load_vec(src + (c + 64) * N, g);
+  constexpr int U = V == Vec16<T>::N ? 2 : 4;
+  for (int c0 = lane * V; c0 < wd; c0 += U * 64 * V) {
+    Piece<T, V> f[U];
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = ok ? f[i] * scale : 0.f;
-      stream_store_vec(dst + c * N, f);
-      if (!more) break;
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * 64 * V < wd) f[u] = *reinterpret_cast<const Piece<T, V>*>(src + c0 + u * 64 * V);
 #pragma unroll
-      for (int i = 0; i < N; ++i) g[i] = ok ? g[i] * scale : 0.f;
-      stream_store_vec(dst + (c + 64) * N, g);
+    for (int u = 0; u < U; ++u) {
+      if (c0 + u * 64 * V >= wd) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[u][i] = (T)(ok ? (float)f[u][i] * scale : 0.f);
+      Piece<T, V>* to = reinterpret_cast<Piece<T, V>*>(dst + c0 + u * 64 * V);
+      if (V == Vec16<T>::N) stream_store(to, f[u]);
+      else *to = f[u];
     }
-  } else {
-    for (int c = lane; c < wd; c += 64) dst[c] = (T)(ok ? (float)src[c] * scale : 0.f);
   }
 }
 
@@ -140,20 +143,25 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(SortPass s) {
 // once; one that crosses the chunk's ends leaves fp32 partial sums, head (0) and tail (1), which k_embed_join adds in chunk order.
 constexpr int kChunk = 32;
 
-template <typename T, bool VEC> struct Cols {
+template <typename T, int V> struct Cols {
   static constexpr int N = Vec16<T>::N;
   int c0, wd, lane;
   __device__ Cols(int block, int wd_, int lane_) : c0(block * 64 * N), wd(wd_), lane(lane_) {}
-  __device__ __forceinline__ int at(int i) const { return VEC ? c0 + lane * N + i : c0 + i * 64 + lane; }
+  __device__ __forceinline__ int at(int i) const { return c0 + (i / V * 64 + lane) * V + i % V; }
   typedef typename Vec16<T>::type Raw;                              // held as loaded: half the registers of floats for two-byte types
   __device__ __forceinline__ Raw load(const T* row) const {
     Raw v;
-    if (VEC) {
+    if constexpr (V == N) {
       if (at(0) < wd) return stream_load(reinterpret_cast<const Raw*>(row + at(0)));
       v = (T)0.f;
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = at(i) < wd ? row[at(i)] : (T)0.f;
+      for (int p = 0; p < N; p += V) {
+        Piece<T, V> x = (T)0.f;
+        if (at(p) < wd) x = *reinterpret_cast<const Piece<T, V>*>(row + at(p));
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[p + i] = x[i];
+      }
     }
     return v;
   }
@@ -162,40 +170,42 @@ template <typename T, bool VEC> struct Cols {
     for (int i = 0; i < N; ++i) acc[i] += (float)v[i];
   }
   __device__ __forceinline__ void store(T* row, const float (&f)[N]) const {
-    if (VEC) {
+    if constexpr (V == N) {
       if (at(0) < wd) stream_store_vec(row + at(0), f);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) if (at(i) < wd) row[at(i)] = (T)f[i];
+      for (int p = 0; p < N; p += V) {
+        Piece<T, V> x;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = (T)f[p + i];
+        if (at(p) < wd) *reinterpret_cast<Piece<T, V>*>(row + at(p)) = x;
+      }
     }
   }
+  // fp32 sums of a row, up to four elements at a time
+  static constexpr int VP = V < 4 ? V : 4;
   __device__ __forceinline__ void store_part(float* row, const float (&f)[N]) const {
-    if (VEC) {
-      if (at(0) < wd)
 #pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(row + at(i)) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-    } else {
+    for (int p = 0; p < N; p += VP) {
+      Piece<float, VP> x;
 #pragma unroll
-      for (int i = 0; i < N; ++i) if (at(i) < wd) row[at(i)] = f[i];
+      for (int i = 0; i < VP; ++i) x[i] = f[p + i];
+      if (at(p) < wd) *reinterpret_cast<Piece<float, VP>*>(row + at(p)) = x;
     }
   }
   __device__ __forceinline__ void add_part(const float* row, float (&f)[N]) const {
-    if (VEC) {
-      if (at(0) < wd)
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(row + at(i));
-          f[i] += v.x; f[i + 1] += v.y; f[i + 2] += v.z; f[i + 3] += v.w;
-        }
-    } else {
+    for (int p = 0; p < N; p += VP)
+      if (at(p) < wd) {
+        const Piece<float, VP> x = *reinterpret_cast<const Piece<float, VP>*>(row + at(p));
 #pragma unroll
-      for (int i = 0; i < N; ++i) if (at(i) < wd) f[i] += row[at(i)];
-    }
+        for (int i = 0; i < VP; ++i) f[p + i] += x[i];
+      }
   }
 };
 
 // the rows of the table that no pair names are zero: blocks behind those of the sums look their rows up and clear them
-template <typename T, bool VEC>
+template <typename T, int V>
 __device__ __forceinline__ void zero_rows(const int32_t* key, int64_t n, int64_t vocab, int wd, int64_t r0, int rows, T* g_table) {
   constexpr int N = Vec16<T>::N;
   __shared__ int sh_there[256];
@@ -209,30 +219,30 @@ __device__ __forceinline__ void zero_rows(const int32_t* key, int64_t n, int64_t
     sh_there[tid] = a < n && key[a] == r0 + tid;
   }
   __syncthreads();
-  float z[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) z[i] = 0.f;
   for (int r = wave; r < rows && r0 + r < vocab; r += 4) {
     if (sh_there[r]) continue;
     T* row = g_table + (r0 + r) * wd;
-    if (VEC) for (int c = lane * N; c < wd; c += 64 * N) stream_store_vec(row + c, z);
-    else for (int c = lane; c < wd; c += 64) row[c] = (T)0.f;
+    for (int c = lane * V; c < wd; c += 64 * V) {
+      const Piece<T, V> z = (T)0.f;
+      if (V == N) stream_store(reinterpret_cast<Piece<T, V>*>(row + c), z);
+      else *reinterpret_cast<Piece<T, V>*>(row + c) = z;
+    }
   }
 }
 
-template <typename T, bool VEC>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_embed_sum(const T* __restrict__ g_y, const int32_t* key, const int32_t* pos, int64_t n, int64_t vocab, int wd,
                                                    int colblocks, float scale, T* __restrict__ g_table, float* part, int sum_blocks, int zero_per) {
   constexpr int N = Vec16<T>::N, U = 8;
   if ((int)blockIdx.x >= sum_blocks) {
-    zero_rows<T, VEC>(key, n, vocab, wd, (int64_t)((int)blockIdx.x - sum_blocks) * zero_per, zero_per, g_table);
+    zero_rows<T, V>(key, n, vocab, wd, (int64_t)((int)blockIdx.x - sum_blocks) * zero_per, zero_per, g_table);
     return;
   }
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int64_t chunk = unit / colblocks, a = chunk * kChunk;
   if (a >= n) return;
-  const Cols<T, VEC> cols((int)(unit % colblocks), wd, lane);
+  const Cols<T, V> cols((int)(unit % colblocks), wd, lane);
   const int m = (int)(n - a < kChunk ? n - a : kChunk);
   const int32_t mykey = lane < m ? key[a + lane] : (int32_t)vocab;
   const int32_t mypos = lane < m ? pos[a + lane] : 0;
@@ -245,7 +255,7 @@ __global__ __launch_bounds__(256) void k_embed_sum(const T* __restrict__ g_y, co
   if (cur >= vocab) return;
   bool open_left = cur == left;
   for (int j0 = 0; j0 < m; j0 += U) {
-    typename Cols<T, VEC>::Raw f[U];
+    typename Cols<T, V>::Raw f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {                                   // (padding pairs of a short chunk read a row that exists: position 0)
       const int32_t p = __builtin_amdgcn_readlane(mypos, (j0 + u) & 63);
@@ -283,7 +293,7 @@ __global__ __launch_bounds__(256) void k_embed_sum(const T* __restrict__ g_y, co
 // adds up to kAlone heads by itself; a frequent token has hundreds, which the workgroup's waves share, consecutive equal parts each,
 // added in order.
 constexpr int kJoinWaves = 16, kAlone = 8;
-template <typename T, bool VEC>
+template <typename T, int V>
 __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* key, int64_t n, int64_t vocab, int wd, int colblocks, float scale,
                                                                 T* g_table, const float* part) {
   constexpr int N = Vec16<T>::N;
@@ -291,7 +301,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* k
   __shared__ int32_t sh_long[kJoinWaves], sh_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t chunks = (n + kChunk - 1) / kChunk, first = (int64_t)(blockIdx.x / colblocks) * kJoinWaves, mine = first + wave;
-  const Cols<T, VEC> cols((int)(blockIdx.x % colblocks), wd, lane);
+  const Cols<T, V> cols((int)(blockIdx.x % colblocks), wd, lane);
   // heads of the token that starts in chunk c and leaves it, up to 64; 0: there is none
   const auto heads_of = [&](int64_t c) {
     const int64_t b = (c + 1) * kChunk;                             // c + 1 is a chunk: b < n
@@ -356,7 +366,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* k
 // workgroup's waves, consecutive equal parts each, added in order.
 constexpr int kSmall = 4096, kSmallWaves = 16, kSmallThreads = 64 * kSmallWaves, kSmallRows = 256, kAloneRow = 16, kSmallGroups = 512;
 
-template <typename T, bool VEC>
+template <typename T, int V>
 __global__ __launch_bounds__(kSmallThreads) void k_embed_small(const T* __restrict__ g_y, const int64_t* __restrict__ tokens, int n, int64_t vocab, int wd,
                                                                int colblocks, float scale, int64_t padding, T* __restrict__ g_table) {
   constexpr int N = Vec16<T>::N, U = 4;
@@ -394,14 +404,14 @@ __global__ __launch_bounds__(kSmallThreads) void k_embed_small(const T* __restri
   for (int r = wave; r < rows; r += kSmallWaves) {
     if (cnt[r] > kAloneRow) continue;
     for (int cb = 0; cb < colblocks; ++cb) {
-      const Cols<T, VEC> cols(cb, wd, lane);
+      const Cols<T, V> cols(cb, wd, lane);
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
       for (int j0 = 0, left = cnt[r]; left; j0 += 64) {             // ends: the list holds cnt[r] of row r
         unsigned long long b = __ballot(j0 + lane < m && row[(j0 + lane) & (kSmall - 1)] == r);
         left -= __popcll(b);
         while (b) {
-          typename Cols<T, VEC>::Raw f[U];
+          typename Cols<T, V>::Raw f[U];
           int have = 0;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -430,11 +440,11 @@ __global__ __launch_bounds__(kSmallThreads) void k_embed_small(const T* __restri
     }
     const int share = (k + kSmallWaves - 1) / kSmallWaves, a = wave * share, b = a + share < k ? a + share : k;
     for (int cb = 0; cb < colblocks; ++cb) {
-      const Cols<T, VEC> cols(cb, wd, lane);
+      const Cols<T, V> cols(cb, wd, lane);
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
       for (int j = a; j < b; j += U) {
-        typename Cols<T, VEC>::Raw f[U];
+        typename Cols<T, V>::Raw f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) f[u] = cols.load(g_y + (int64_t)sel[j + u < b ? j + u : j] * wd);
 #pragma unroll
@@ -491,33 +501,43 @@ int embed_check(int64_t n, int64_t vocab, int wd, int elem) {
   return 0;
 }
 
+// f(V as a type): the widest pieces that rows of `wd` elements at both addresses allow
+template <typename T, typename F> int by_piece(int wd, const void* a, const void* b, F f) {
+  constexpr int N = Vec16<T>::N;
+  const uintptr_t at = (uintptr_t)a | (uintptr_t)b;
+  if (wd % N == 0 && at % 16 == 0) return f(std::integral_constant<int, N>());
+  if (wd % 2 == 0 && at % (2 * sizeof(T)) == 0) return f(std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, 1>());
+}
+
 template <typename T>
 int embed_forward(const T* table, int64_t vocab, int wd, const int64_t* tokens, int64_t n, float scale, T* y, int32_t* bad, hipStream_t st) {
-  const bool vec = wd % Vec16<T>::N == 0 && ptr16(table) && ptr16(y);
   const dim3 grid((unsigned)((n + 3) / 4));
-  if (vec) DVGR_LAUNCH((k_embed_fwd<T, true>), grid, dim3(256), 0, st, table, vocab, wd, tokens, n, scale, y, bad);
-  else DVGR_LAUNCH((k_embed_fwd<T, false>), grid, dim3(256), 0, st, table, vocab, wd, tokens, n, scale, y, bad);
+  by_piece<T>(wd, table, y, [&](auto v) {
+    DVGR_LAUNCH((k_embed_fwd<T, decltype(v)::value>), grid, dim3(256), 0, st, table, vocab, wd, tokens, n, scale, y, bad);
+    return 0;
+  });
   return (int)hipGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T, int V>
 int embed_sum(const T* g_y, const int32_t* key, const int32_t* pos, int64_t n, int64_t vocab, int wd, const EmbedPlan& p, float scale,
               T* g_table, float* part, hipStream_t st) {
   const int64_t row_bytes = (int64_t)wd * sizeof(T), sum_blocks = (p.chunks * p.colblocks + 3) / 4;
   const int zero_per = row_bytes >= 32768 ? 1 : row_bytes <= 128 ? 256 : (int)(32768 / row_bytes);
-  DVGR_LAUNCH((k_embed_sum<T, VEC>), dim3((unsigned)(sum_blocks + (vocab + zero_per - 1) / zero_per)), dim3(256), 0, st, g_y, key, pos, n, vocab, wd,
+  DVGR_LAUNCH((k_embed_sum<T, V>), dim3((unsigned)(sum_blocks + (vocab + zero_per - 1) / zero_per)), dim3(256), 0, st, g_y, key, pos, n, vocab, wd,
               p.colblocks, scale, g_table, part, (int)sum_blocks, zero_per);
   int e = (int)hipGetLastError();
   if (e || p.chunks < 2) return e;
-  DVGR_LAUNCH((k_embed_join<T, VEC>), dim3((unsigned)((p.chunks - 1 + kJoinWaves - 1) / kJoinWaves * p.colblocks)), dim3(64 * kJoinWaves), 0, st, key, n,
+  DVGR_LAUNCH((k_embed_join<T, V>), dim3((unsigned)((p.chunks - 1 + kJoinWaves - 1) / kJoinWaves * p.colblocks)), dim3(64 * kJoinWaves), 0, st, key, n,
               vocab, wd, p.colblocks, scale, g_table, part);
   return (int)hipGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T, int V>
 int embed_small(const T* g_y, const int64_t* tokens, int n, int64_t vocab, int wd, float scale, int64_t padding, T* g_table, hipStream_t st) {
   const int colblocks = (wd + 64 * Vec16<T>::N - 1) / (64 * Vec16<T>::N);
-  DVGR_LAUNCH((k_embed_small<T, VEC>), dim3((unsigned)(vocab < kSmallGroups ? vocab : kSmallGroups)), dim3(kSmallThreads), 0, st, g_y, tokens, n, vocab, wd, colblocks, scale,
+  DVGR_LAUNCH((k_embed_small<T, V>), dim3((unsigned)(vocab < kSmallGroups ? vocab : kSmallGroups)), dim3(kSmallThreads), 0, st, g_y, tokens, n, vocab, wd, colblocks, scale,
               padding, g_table);
   return (int)hipGetLastError();
 }
@@ -525,10 +545,10 @@ int embed_small(const T* g_y, const int64_t* tokens, int n, int64_t vocab, int w
 template <typename T>
 int embed_backward(const T* g_y, const int64_t* tokens, int64_t n, int64_t vocab, int wd, float scale, int64_t padding, T* g_table,
                    char* ws, const EmbedPlan& p, hipStream_t st) {
-  const bool vec = wd % Vec16<T>::N == 0 && ptr16(g_y) && ptr16(g_table);
   if (p.small)
-    return vec ? embed_small<T, true>(g_y, tokens, (int)n, vocab, wd, scale, padding, g_table, st)
-               : embed_small<T, false>(g_y, tokens, (int)n, vocab, wd, scale, padding, g_table, st);
+    return by_piece<T>(wd, g_y, g_table, [&](auto v) {
+      return embed_small<T, decltype(v)::value>(g_y, tokens, (int)n, vocab, wd, scale, padding, g_table, st);
+    });
   SortPass s{};
   s.n = n; s.vocab = vocab; s.padding = padding; s.tile = p.tile; s.blocks = p.blocks;
   s.hist = reinterpret_cast<int32_t*>(ws + p.hist);
@@ -544,8 +564,9 @@ int embed_backward(const T* g_y, const int64_t* tokens, int64_t n, int64_t vocab
   const int32_t* key = reinterpret_cast<const int32_t*>(ws + p.key[at]);
   const int32_t* pos = reinterpret_cast<const int32_t*>(ws + p.pos[at]);
   float* part = reinterpret_cast<float*>(ws + p.part);
-  return vec ? embed_sum<T, true>(g_y, key, pos, n, vocab, wd, p, scale, g_table, part, st)
-             : embed_sum<T, false>(g_y, key, pos, n, vocab, wd, p, scale, g_table, part, st);
+  return by_piece<T>(wd, g_y, g_table, [&](auto v) {
+    return embed_sum<T, decltype(v)::value>(g_y, key, pos, n, vocab, wd, p, scale, g_table, part, st);
+  });
 }
 
 }  // namespace
