@@ -6,6 +6,9 @@
 // gradient brings the positions of a token together, adds their rows in fp32 in an order that the tokens alone decide, and rounds
 // once: no float atomics, so the result does not depend on the schedule.  Two forms: up to kSmall positions one launch in which
 // every workgroup picks the tokens of its own rows of the table; beyond, a stable radix sort of (token, position) pairs.
+//
+// 65536 positions x 1024 bf16 of 50000 words: forward 27 us, sort 27 in four launches, sums 40, join 14.5; 104 us where 474 MB at a large
+// copy's rate take 96.  960 x 300 fp32 of 4000 words: 2.6 and 8.2 us, less than it takes to call them.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -18,7 +21,8 @@ namespace dvgr {
 namespace {
 
 // Rows are handled V elements at a time: 16 bytes where rows start at multiples of 16 bytes, otherwise pairs where an even width allows it
-// (53291 x 806 fp16 of 19164 words, forward and backward: 198 us by single elements, 112 by pairs), otherwise single elements.  Neighbouring lanes take neighbouring pieces.
+// (53291 x 806 fp16 of 19164 words, forward and backward: 198 us by single elements, 112 by pairs), otherwise single elements.  Neighbouring
+// lanes take neighbouring pieces.
 template <typename T, int V> using Piece = T __attribute__((ext_vector_type(V)));
 
 // One wave per token position, a few pieces in flight.
@@ -361,8 +365,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* k
 }
 
 // ---- few positions: one launch ----------------------------------------------------------------------------------------------
-// Workgroup w of kSmallGroups owns the rows w, w + kSmallGroups, ... (the frequent tokens of a vocabulary are neighbours).  It reads all the tokens (they fit the L2 many times over) and keeps the positions of its own
-// in their order.  A wave takes a row and adds its positions one after the other; a row of more than kAloneRow positions is shared by the
+// Workgroup w of kSmallGroups owns the rows w, w + kSmallGroups, ... (the frequent tokens of a vocabulary are neighbours).  It reads all
+// the tokens (they fit the L2 many times over) and keeps the positions of its own in their order.  A wave takes a row and adds its positions one after the other; a row of more than kAloneRow positions is shared by the
 // workgroup's waves, consecutive equal parts each, added in order.
 constexpr int kSmall = 4096, kSmallWaves = 16, kSmallThreads = 64 * kSmallWaves, kSmallRows = 256, kAloneRow = 16, kSmallGroups = 512;
 
