@@ -217,7 +217,8 @@ template <typename T> __device__ __forceinline__ void store4(char* p, float a, f
 
 // An 8-XCD chip hands workgroup i to XCD i % 8: give every XCD a contiguous run of the work, so that the workgroups that read the same
 // keys share an L2.  A head with 8 workgroups or more (`tiles`) has one on every XCD instead: samples of different lengths would leave
-// XCDs without work (captions over long videos of 50 to 100 % of 4096 states: dK and dV 750 us with runs, 620 without; the forward 340, 310).  -1: nothing to do.
+// XCDs without work (captions over long videos of 50 to 100 % of 4096 states: dK and dV 750 us with runs, 620 without; the forward 340,
+// 310).  -1: nothing to do.
 __device__ __forceinline__ int64_t xcd_work(int64_t total, int tiles = 1) {
   if (tiles >= 8) return blockIdx.x < total ? (int64_t)blockIdx.x : -1;
   const int64_t per = (total + 7) / 8, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);

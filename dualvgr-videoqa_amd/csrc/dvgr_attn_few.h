@@ -1,7 +1,7 @@
 // dvgr_attn_few.h -- attention where one 32-row tile holds all packed rows of a key head (a word over a video, a question over its
 // frames), or where larger tiles would leave most of the chip idle: bound by the keys' and values' memory, so the waves of a workgroup go
-// over different keys at their own pace.  A wave reads its 32 keys a row at a time (whole lines; read straight as operands, 32 bytes of 32 rows each, they fell out of the cache
-// between the steps) into LDS of its own; nothing waits for another wave before the end.
+// over different keys at their own pace.  A wave reads its 32 keys a row at a time (whole lines; read straight as operands, 32 bytes of 32
+// rows each, they fell out of the cache between the steps) into LDS of its own; nothing waits for another wave before the end.
 #pragma once
 #include "dvgr_attn.h"
 

@@ -4,8 +4,8 @@
 //   loss_r = T^2 sum_k p_k (log p_k - log q_{i_k})         d loss_r / d z_j = T (q_j - sum_{k : i_k = j} p_k)
 //
 // Bound by memory: the forward reads the logits once (running maximum and sum), the backward reads them once more and writes the
-// gradient; the lists are small.  Everything is fp32; the gradient is rounded to the logits' type where it is stored.  4096 x 32000 bf16: 51 us forward (5.2 TB/s, see kKeep), 96 us backward
-// (5.5 TB/s of reads and writes).
+// gradient; the lists are small.  Everything is fp32; the gradient is rounded to the logits' type where it is stored.  4096 x 32000 bf16:
+// 51 us forward (5.2 TB/s, see kKeep), 96 us backward (5.5 TB/s of reads and writes).
 #include <hip/hip_runtime.h>
 
 #include "../../include/dvgr.h"

@@ -366,8 +366,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const int32_t* k
 
 // ---- few positions: one launch ----------------------------------------------------------------------------------------------
 // Workgroup w of kSmallGroups owns the rows w, w + kSmallGroups, ... (the frequent tokens of a vocabulary are neighbours).  It reads all
-// the tokens (they fit the L2 many times over) and keeps the positions of its own in their order.  A wave takes a row and adds its positions one after the other; a row of more than kAloneRow positions is shared by the
-// workgroup's waves, consecutive equal parts each, added in order.
+// the tokens (they fit the L2 many times over) and keeps the positions of its own in their order.  A wave takes a row and adds its
+// positions one after the other; a row of more than kAloneRow positions is shared by the workgroup's waves, consecutive equal parts each,
+// added in order.
 constexpr int kSmall = 4096, kSmallWaves = 16, kSmallThreads = 64 * kSmallWaves, kSmallRows = 256, kAloneRow = 16, kSmallGroups = 512;
 
 template <typename T, int V>
