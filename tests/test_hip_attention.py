@@ -226,6 +226,17 @@ def test_scores_that_grow_and_fall_from_key_to_key(t):
     check(q[:2].detach().requires_grad_(True), k[:2].detach().requires_grad_(True), v[:2].detach().requires_grad_(True))
 
 
+@pytest.mark.parametrize("shape,lens", [((3, 700, 700, 4, 2, 64), [0, 1, 700]), ((2, 1100, 20, 2, 1, 96), [20, 3]), ((5, 600, 300, 3, 3, 128), [300, 129, 128, 127, 5]),
+                                        ((4, 1000, 513, 2, 2, 32), [0, 0, 0, 0]), ((4, 1000, 513, 2, 2, 40), [0, 0, 0, 1]), ((2, 1500, 32, 1, 1, 128), [0, 32]),
+                                        ((1, 3001, 400, 1, 1, 128), None), ((2, 1024, 30, 3, 1, 16), None)])
+@pytest.mark.parametrize("t", TYPES)
+def test_gradients_of_keys_shared_by_workgroups(t, shape, lens):
+    q, k, v, gen = tensors(*shape, t)
+    n = None if lens is None else torch.tensor(lens, device="cuda")
+    check(q, k, v, n)
+    check(q, k, v, n, torch.rand(shape[0], shape[2], generator=gen, device="cuda") < 0.8)
+
+
 @pytest.mark.parametrize("worst", [float("nan"), float("inf")])
 @pytest.mark.parametrize("Lq,Lk", [(5, 40), (5, 100), (40, 20), (40, 100)])
 @pytest.mark.parametrize("t", TYPES)
