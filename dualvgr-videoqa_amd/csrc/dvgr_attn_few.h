@@ -68,10 +68,21 @@ template <int KW> __device__ __forceinline__ FewWork few_work(const Args& A, int
   return f;
 }
 
-// Work in shares: `units` workgroups of `turns` turns each are split until there are `want` of them, in shares of at least `least` turns.
+// Work in shares: `units` workgroups of `turns` turns each are split until there are `want` of them (as many as run at once), in shares of
+// at least `least` turns.  Where that is no split, up to eight are looked at: 264 workgroups on 256 places are two rounds, 5 x 264 are six
+// of a fifth.  A split costs a launch that joins it, about eight turns.  (One query over 33 x 7731 keys, 8 heads of 32, fp32: 176 -> 108 us;
+// 40 x 2048 keys, 8 heads of 128, bf16, split for two turns less: 64 -> 70.)
 struct Shares { int splits, turns_per_split; };
 inline Shares shares_of(int64_t units, int64_t turns, int64_t want, int least) {
   int64_t s = units ? want / units : 1;
+  if (s == 1 || (s < 1 && units < 4 * want)) {
+    int64_t best = (units + want - 1) / want * turns;
+    s = 1;
+    for (int64_t x = 2; x <= 8; ++x) {
+      const int64_t cost = (units * x + want - 1) / want * ((turns + x - 1) / x) + 8;
+      if (cost < best) { best = cost; s = x; }
+    }
+  }
   if (s > turns / least) s = turns / least;
   if (s < 1) s = 1;
   Shares x{};
