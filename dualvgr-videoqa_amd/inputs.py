@@ -157,6 +157,11 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, dtype_code):
         lib = load()
+        for t, name in ((x, "the input"), (w, "the weight"), (b, "the bias")):         # the kernels take addresses: nothing below looks again
+            if t is not None and (t.dtype != torch.float32 or t.device != x.device):
+                raise RuntimeError(f"HipLinear: input and parameters are fp32 on one device; {name} is {t.dtype} on {t.device}")
+        if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+            raise RuntimeError(f"HipLinear: {w.shape[1]} input features; got {tuple(x.shape)}")
         _need_device(x, "HipLinear")
         K = x.shape[-1]
         x2 = x.reshape(-1, K).contiguous()
@@ -190,7 +195,8 @@ class _Linear(torch.autograd.Function):
 
 class HipLinear(nn.Linear):
     """nn.Linear(in_features, out_features) whose forward / backward run on the unit's contraction engine
-    (dvgr_linear_forward / dvgr_linear_backward).  `dtype`: 'fp32' | 'bf16x3' | 'bf16' as for the unit."""
+    (dvgr_linear_forward / dvgr_linear_backward).  `dtype`: 'fp32' | 'bf16x3' | 'bf16' as for the unit: how the products take their
+    operands.  Input, parameters and output are fp32 tensors (a module cast to another type raises)."""
 
     def __init__(self, in_features, out_features, bias=True, dtype: str = "fp32"):
         super().__init__(in_features, out_features, bias=bias)

@@ -247,3 +247,26 @@ def test_two_streams_at_once():
                 got.append(work())
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_two_byte_embeddings_feed_the_attention_module(t, dtype):
+    torch.manual_seed(9)
+    embed, attend = dv.TokenEmbedding(40, 64, scale=8.0).cuda().to(t), dv.CrossAttention(64, 2, state_dim=48, dtype=dtype).cuda()
+    tokens = torch.randint(0, 40, (3, 5), device="cuda")
+    frames = torch.randn(3, 20, 48, device="cuda").to(t).requires_grad_(True)
+    words = embed(tokens)
+    words.retain_grad()
+    y = attend(words, frames)
+    assert words.dtype == t and y.dtype == torch.float32
+    y.square().sum().backward()
+    wide, states = words.detach().float().requires_grad_(True), frames.detach().float().requires_grad_(True)
+    z = attend(wide, states)                                        # the same numbers in fp32
+    assert torch.equal(y, z)
+    z.square().sum().backward()
+    # nothing differs but the one rounding to the input's type (half a step, and half the smallest number)
+    for got, want in ((words.grad, wide.grad), (frames.grad, states.grad)):
+        assert got.dtype == t
+        assert ((got.double() - want.double()).abs() <= want.double().abs() * torch.finfo(t).eps / 2 + torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2).all()
+    assert embed.weight.grad.dtype == t and torch.isfinite(embed.weight.grad).all()

@@ -128,3 +128,34 @@ def test_constructors_refuse():
             dv.CrossAttention(**kw)
     assert set(dv.TokenEmbedding(4, 8, padding_idx=1).state_dict()) == {"weight"}
     assert {k.split(".")[0] for k in dv.CrossAttention(64, 2).state_dict()} == {"query", "key_value", "out"}
+
+
+def test_projections_refuse_what_their_kernels_cannot_read():
+    lin = dv.HipLinear(64, 32)
+    for t in (torch.bfloat16, torch.float16, torch.float64):
+        with pytest.raises(RuntimeError, match="fp32 on one device; the input"):
+            lin(torch.zeros(3, 64, dtype=t))
+    for shape in ((3, 60), (3, 68), (64, 3), ()):
+        with pytest.raises(RuntimeError, match="64 input features"):
+            lin(torch.zeros(shape))
+    with pytest.raises(RuntimeError, match="fp32 on one device; the weight"):
+        dv.HipLinear(64, 32).to(torch.bfloat16)(torch.zeros(3, 64))
+    cast = dv.HipLinear(64, 32)
+    cast.bias = torch.nn.Parameter(cast.bias.detach().half())
+    with pytest.raises(RuntimeError, match="fp32 on one device; the bias"):
+        cast(torch.zeros(3, 64))
+
+    attend = dv.CrossAttention(64, 2, state_dim=48, dtype="bf16")
+    x, s = torch.zeros(1, 2, 64), torch.zeros(1, 5, 48)
+    for t in (torch.float64, torch.int64):
+        with pytest.raises(RuntimeError, match="in fp32, bf16 or fp16"):
+            attend(x.to(t), s)
+        with pytest.raises(RuntimeError, match="in fp32, bf16 or fp16"):
+            attend(x, s.to(t))
+    with pytest.raises(RuntimeError, match="batch, length, features"):
+        attend.states(s[0])
+    with pytest.raises(RuntimeError, match="48 input features"):
+        attend.states(x)
+    assert attend.half() is attend                                  # nn.Module's own cast, then refused by name
+    with pytest.raises(RuntimeError, match="fp32 on one device; the weight"):
+        attend(x, s)
