@@ -183,6 +183,10 @@ class _Linear(torch.autograd.Function):
         M, K = x2.shape
         N = w.shape[0]
         gy2 = gy.reshape(M, N).contiguous()
+        rows = M
+        if M < 4:                                # a word or three: the weight's gradient sums over four rows at least
+            M = 4
+            x2, gy2 = (torch.cat((t, t.new_zeros(M - rows, t.shape[1]))) for t in (x2, gy2))
         gw = torch.empty_like(w)
         gb = torch.empty(N, device=gy.device, dtype=torch.float32) if has_b else None
         gx = torch.empty_like(x2) if ctx.needs_input_grad[0] else None
@@ -190,7 +194,7 @@ class _Linear(torch.autograd.Function):
         L_.check(lib.dvgr_linear_backward(x2.data_ptr(), w.data_ptr(), gy2.data_ptr(), gx.data_ptr() if gx is not None else None,
                                           gw.data_ptr(), gb.data_ptr() if gb is not None else None, M, N, K, code, stream),
                  "dvgr_linear_backward")
-        return (gx.view(*xshape) if gx is not None else None), gw, gb, None
+        return (gx[:rows].view(*xshape) if gx is not None else None), gw, gb, None
 
 
 class HipLinear(nn.Linear):

@@ -270,3 +270,33 @@ def test_two_byte_embeddings_feed_the_attention_module(t, dtype):
         assert got.dtype == t
         assert ((got.double() - want.double()).abs() <= want.double().abs() * torch.finfo(t).eps / 2 + torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2).all()
     assert embed.weight.grad.dtype == t and torch.isfinite(embed.weight.grad).all()
+
+
+@pytest.mark.parametrize("dtype,tol", [("fp32", 2e-6), ("bf16x3", 2e-5)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+def test_projections_of_a_few_words_have_gradients(dtype, tol, rows):
+    # (the bounds of the same products at other sizes: fp32 sums of up to 64 terms, operands split into two bf16 halves)
+    torch.manual_seed(10)
+    lin = dv.HipLinear(64, 24, dtype=dtype).cuda()
+    x, up = torch.randn(rows, 64, device="cuda", requires_grad=True), torch.randn(rows, 24, device="cuda")
+    grads = torch.autograd.grad(lin(x), [x, lin.weight, lin.bias], up)
+    u, w, z = up.double(), lin.weight.detach().double(), x.detach().double()
+    for got, want in zip(grads, (u @ w, u.t() @ z, u.sum(0))):
+        assert got.shape == want.shape and float((got - want).abs().max()) <= tol * float(want.abs().max())
+
+
+def test_an_answer_of_one_word_is_trained():
+    torch.manual_seed(11)
+    attend = dv.CrossAttention(64, 2, key_heads=1, state_dim=48).cuda()
+    x, s = torch.randn(1, 1, 64, device="cuda", requires_grad=True), torch.randn(1, 2, 48, device="cuda", requires_grad=True)
+    up = torch.randn(1, 1, 64, device="cuda")
+    grads = torch.autograd.grad(attend(x, s), [x, s, *attend.parameters()], up)
+    p = {n: t.detach().cpu().double().requires_grad_(True) for n, t in attend.named_parameters()}
+    y, z = x.detach().cpu().double().requires_grad_(True), s.detach().cpu().double().requires_grad_(True)
+    lin = lambda n, t: t @ p[n + ".weight"].t() + p[n + ".bias"]  # noqa: E731
+    q, kv = lin("query", y).view(2, 32), lin("key_value", z).view(2, 2, 32)
+    o = torch.softmax(q @ kv[:, 0].t() * 32 ** -0.5, 1) @ kv[:, 1]
+    want = torch.autograd.grad(lin("out", o.reshape(1, 1, 64)), [y, z, *p.values()], up.cpu().double())
+    # fp32 throughout: chains of dot products of up to 64 terms, a few 2^-24 of their size each (the keys' bias has no gradient: a sum that cancels)
+    for got, w in zip(grads, want):
+        assert float((got.cpu().double() - w).abs().max()) <= 5e-5 * float(w.abs().max()) + 1e-7
