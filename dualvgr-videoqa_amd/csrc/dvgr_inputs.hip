@@ -72,6 +72,12 @@ __global__ __launch_bounds__(256) void k_fill_bias(float* y, const float* b, int
   reinterpret_cast<float4*>(y)[i] = reinterpret_cast<const float4*>(b)[i % n4];
 }
 
+// (a memset recorded into a captured graph has given wrong sums on replays after the first)
+__global__ __launch_bounds__(256) void k_fill_zero(float* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0.f;
+}
+
 }  // namespace
 }  // namespace dvgr
 
@@ -161,7 +167,8 @@ int dvgr_linear_backward(const float* x, const float* w, const float* gy, float*
     if (e) return e;
   }
   if (gb) {
-    const hipError_t e0 = hipMemsetAsync(gb, 0, (size_t)N * sizeof(float), st);
+    DVGR_LAUNCH(k_fill_zero, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, gb, (int64_t)N);
+    const hipError_t e0 = hipGetLastError();
     if (e0 != hipSuccess) return (int)e0;
     ColsumBatch cb{};
     cb.j[cb.n++] = ColsumJob{gy, nullptr, nullptr, nullptr, M, 0, N, N, gb};

@@ -300,3 +300,33 @@ def test_an_answer_of_one_word_is_trained():
     # fp32 throughout: chains of dot products of up to 64 terms, a few 2^-24 of their size each (the keys' bias has no gradient: a sum that cancels)
     for got, w in zip(grads, want):
         assert float((got.cpu().double() - w).abs().max()) <= 5e-5 * float(w.abs().max()) + 1e-7
+
+
+def test_the_whole_path_captured_and_replayed_between_eager_work():
+    torch.manual_seed(12)
+    m = Reader(50, 40, 64, 48).cuda()
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    B, L, F = 16, 9, 70
+    tokens, frames = torch.randint(0, 50, (B, L), generator=gen, device="cuda"), torch.randn(B, F, 48, generator=gen, device="cuda")
+    lens = torch.randint(1, F + 1, (B,), generator=gen, device="cuda")
+    values, indices = torch.randn(B, 40, generator=gen, device="cuda").topk(5, 1)
+    names = [n for n, _ in m.named_parameters()]
+
+    def step():
+        loss = dv.distillation_loss(m(tokens, frames, lens), values, indices, 2.0)
+        return [loss.detach(), *torch.autograd.grad(loss, list(m.parameters()))]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(5):
+        tokens.copy_(torch.randint(0, 50, (B, L), generator=gen, device="cuda"))
+        frames.copy_(torch.randn(B, F, 48, generator=gen, device="cuda"))
+        lens.copy_(torch.randint(1, F + 1, (B,), generator=gen, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        # what the projections add atomically (their biases' sums over 16 shares of up to B F rows) may differ in its last bits
+        for n, a, b in zip(["loss", *names], held, want):
+            assert float((a - b).abs().max()) <= 2e-5 * float(b.abs().max()) + 1e-7, (i, n)
