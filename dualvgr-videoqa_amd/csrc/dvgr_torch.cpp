@@ -9,8 +9,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -76,48 +78,70 @@ int elem_code(const Tensor& t, const char* what) {
 hipStream_t stream_of(const Tensor& t) { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 Tensor bytes_on(const Tensor& t, size_t n) { return at::empty({(int64_t)n}, t.options().dtype(at::kByte)); }
 
-// ---- living nodes: which leaves they hold, on which stream they were made ----------------------------------------------------------
-// autograd keeps one accumulation node for a leaf, on the stream where the first living graph made it.  A backward that is captured
-// and ends there would draw that stream into the capture, which ends the process: it is refused instead.
-std::mutex live_mutex;
-struct OpNode;
-std::unordered_set<const OpNode*> live;
+// ---- captured backwards ---------------------------------------------------------------------------------------------------------
+// autograd runs a node on the stream where it was made, and keeps one accumulation node for a leaf while any graph of it lives.  A
+// backward that is captured and runs into a node of a stream outside the capture would draw that stream in, which ends the process: it
+// is refused instead.  So the nodes in front of an operator are looked through, down to the leaves, while its backward is captured (and
+// only then), whatever stands between it and them: views, copies, other operators.
+bool outside_capture(Node* n) {
+  const auto s = n->stream();
+  if (!s) return false;                                             // (not a device's)
+  const hipStream_t st = at::hip::HIPStreamMasqueradingAsCUDA(at::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *s).stream();
+  if (st == nullptr) return true;                                   // (the null stream cannot be captured, nor asked while another is)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) == hipSuccess) return status == hipStreamCaptureStatusNone;
+  (void)hipGetLastError();
+  return true;
+}
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+// the nodes that the running backward reaches from `todo`, each once, until `found` says yes to one
+template <typename F> bool reaches(std::vector<Node*> todo, F found) {
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();        // (without entries: all of them)
+  std::unordered_set<Node*> seen;
+  while (!todo.empty()) {
+    Node* n = todo.back();
+    todo.pop_back();
+    if (!n || !seen.insert(n).second) continue;
+    if (wanted && !wanted->empty()) {
+      const auto it = wanted->find(n);
+      if (it == wanted->end() || !it->second.should_execute()) continue;
+    }
+    if (found(n)) return true;
+    for (const auto& e : n->next_edges()) todo.push_back(e.function.get());
+  }
+  return false;
+}
+// `n` is about to run: refuses if its gradients go on into such a node
+void refuse_capture(const char* what, Node* n) {
+  if (!capturing()) return;
+  std::vector<Node*> from;
+  for (size_t i = 0; i < n->num_outputs(); ++i)
+    if (n->task_should_compute_output(i)) from.push_back(n->next_edge(i).function.get());
+  TORCH_CHECK(!reaches(std::move(from), outside_capture), what, ": this backward is being captured while a graph of the same leaves lives that was "
+              "made on another stream: drop that graph's outputs (or detach them) before the capture");
+}
+// the same for the node of a Python autograd function, from inside its backward
+void refuse_capture_here(const std::string& what) {
+  if (const auto n = torch::autograd::get_current_node()) refuse_capture(what.c_str(), n.get());
+}
+// test aids: the leaves that a backward of `t` ends in; would a captured backward of `t` be refused
+std::vector<Tensor> dbg_leaves(const Tensor& t) {
+  std::vector<Tensor> out;
+  reaches({t.grad_fn().get()}, [&](Node* n) {
+    if (const auto* a = dynamic_cast<torch::autograd::AccumulateGrad*>(n)) out.push_back(a->variable);
+    return false;
+  });
+  return out;
+}
+bool dbg_refuses_capture(const Tensor& t) { return reaches({t.grad_fn().get()}, outside_capture); }
 
 struct OpNode : Node {
-  hipStream_t stream = nullptr;
-  std::vector<const void*> leaves;
   const char* what = "";
-
-  void hold(const char* name, hipStream_t st, std::initializer_list<const Tensor*> inputs) {
-    what = name;
-    stream = st;
-    for (const Tensor* t : inputs)
-      if (t->requires_grad() && t->is_leaf()) leaves.push_back(t->unsafeGetTensorImpl());
-    if (leaves.empty()) return;
-    std::lock_guard<std::mutex> lock(live_mutex);
-    live.insert(this);
-  }
-  ~OpNode() override {
-    if (leaves.empty()) return;
-    std::lock_guard<std::mutex> lock(live_mutex);
-    live.erase(this);
-  }
-  void check_capture() const {
-    if (leaves.empty() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    std::lock_guard<std::mutex> lock(live_mutex);
-    for (const OpNode* n : live) {
-      if (n->stream == stream) continue;
-      for (const void* a : n->leaves)
-        for (const void* b : leaves)
-          TORCH_CHECK(a != b, what, ": this backward is being captured while a graph of the same leaves lives that was made on another "
-                      "stream: drop that graph's outputs (or detach them) before the capture");
-    }
-  }
   virtual variable_list gradients(variable_list&& grads) = 0;
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(num_outputs());
-    check_capture();
+    refuse_capture(what, this);
     const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
     at::NoGradGuard no_grad;
     const c10::DeviceGuard guard(grads[0].device());
@@ -188,7 +212,7 @@ Tensor embed_tokens(const Tensor& table, Tensor tokens, double scale, std::optio
   if (at::GradMode::is_enabled() && table.requires_grad()) {
     auto n = make_node<EmbedNode>();
     n->set_next_edges(torch::autograd::collect_next_edges(table));
-    n->hold(what, st, {&table});
+    n->what = what;
     n->tokens_ = SavedVariable(tokens, false);
     n->vocab = vocab; n->wd = wd; n->padding = padding; n->elem = elem; n->scale = (float)scale;
     torch::autograd::set_history(y, n);
@@ -245,7 +269,7 @@ Tensor distillation_loss(Tensor z, Tensor v, Tensor i, double temperature, int64
   if (at::GradMode::is_enabled() && z.requires_grad()) {
     auto n = make_node<DistillNode>();
     n->set_next_edges(torch::autograd::collect_next_edges(z));
-    n->hold(what, st, {&z});
+    n->what = what;
     n->logits_ = SavedVariable(z, false); n->values_ = SavedVariable(v, false); n->indices_ = SavedVariable(i, false);
     n->stats_ = SavedVariable(stats, false);
     n->reduction = (int)reduction; n->temperature = (float)temperature;
@@ -356,7 +380,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
   if (grad) {
     auto n = make_node<AttendNode>();
     n->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
-    n->hold(what, st, {&q, &k, &v});
+    n->what = what;
     n->q_ = SavedVariable(qr, false); n->k_ = SavedVariable(kr, false); n->v_ = SavedVariable(vr, false);
     n->o_lo_ = SavedVariable(o_lo, false); n->lse_ = SavedVariable(lse, false); n->lens_ = SavedVariable(lens, false); n->mask_ = SavedVariable(mask, false);
     n->scale = (float)scale;
@@ -373,4 +397,7 @@ PYBIND11_MODULE(_dvgr_torch, m) {
   m.def("embed_tokens", &embed_tokens);
   m.def("distillation_loss", &distillation_loss);
   m.def("cross_attention", &cross_attention);
+  m.def("refuse_capture", &refuse_capture_here);
+  m.def("dbg_leaves", &dbg_leaves);
+  m.def("dbg_refuses_capture", &dbg_refuses_capture);
 }

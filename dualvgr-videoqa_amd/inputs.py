@@ -178,6 +178,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         lib = load()
+        L_.torch_ops().refuse_capture("HipLinear")
         x2, w = ctx.saved_tensors
         xshape, has_b, code = ctx.meta
         M, K = x2.shape

@@ -330,3 +330,74 @@ def test_the_whole_path_captured_and_replayed_between_eager_work():
         # what the projections add atomically (their biases' sums over 16 shares of up to B F rows) may differ in its last bits
         for n, a, b in zip(["loss", *names], held, want):
             assert float((a - b).abs().max()) <= 2e-5 * float(b.abs().max()) + 1e-7, (i, n)
+
+
+def test_which_graphs_a_captured_backward_may_not_run_into():
+    # nothing is run backward here: the look at the nodes alone, from eager code and from inside a capture
+    refuses = dv._lib.torch_ops().dbg_refuses_capture
+    x, z = torch.randn(2, 6, 1, 16, device="cuda", requires_grad=True), torch.randn(2, 3, 16, device="cuda", requires_grad=True)
+    assert refuses(x.view(2, 96)) and refuses(z.transpose(1, 2).contiguous())              # eager, on the null stream
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert refuses(x.exp())                                     # eager, on a stream that no capture knows
+    graph = torch.cuda.CUDAGraph()
+    alive = x.view(2, 96)
+    with torch.cuda.graph(graph):
+        y, u = x.reshape(-1, 16).float() * 2, z.view(6, 16) * 2
+        seen = refuses(y), refuses(u)
+    assert seen == (True, False)                                    # x has a graph outside, z has none
+    del alive, y, u
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x.reshape(-1, 16).float() * 2
+        seen = refuses(y)
+    assert not seen
+
+
+@pytest.mark.parametrize("which", ["logits of three dimensions", "logits along the other stride", "keys and values of one tensor", "projections"])
+def test_captured_backwards_refuse_a_leaf_behind_views_and_copies(which):
+    v, i = torch.randn(2, 3, 3, device="cuda"), torch.zeros(2, 3, 3, device="cuda", dtype=torch.int64)
+    if which == "projections":
+        m = dv.CrossAttention(32, 2, state_dim=16).cuda()
+        x, s = torch.randn(2, 4, 32, device="cuda"), torch.randn(2, 5, 16, device="cuda")
+        leaf, call = m.query.weight, lambda: m(x, s).sum()
+        alive = m.query(x)
+    elif which == "keys and values of one tensor":
+        leaf = torch.randn(2, 6, 2, 1, 16, device="cuda", requires_grad=True)
+        q, call = torch.randn(2, 3, 1, 16, device="cuda"), lambda: dv.cross_attention(q, leaf[:, :, 0], leaf[:, :, 1]).sum()
+        alive = dv.cross_attention(q, leaf[:, :, 1], leaf[:, :, 0])
+    elif which == "logits of three dimensions":
+        leaf = torch.randn(2, 3, 16, device="cuda", requires_grad=True)
+        call = lambda: dv.distillation_loss(leaf, v, i)  # noqa: E731
+        alive = call()
+    else:
+        leaf = torch.randn(16, 6, device="cuda", requires_grad=True)
+        call = lambda: dv.distillation_loss(leaf.t(), v.view(6, 3), i.view(6, 3))  # noqa: E731
+        alive = call()
+    call().backward()                                               # eager ones run
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+        with pytest.raises(RuntimeError, match="captured while"):
+            torch.autograd.grad(out, leaf)
+        del out
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g, = torch.autograd.grad(call(), leaf)
+    want, = torch.autograd.grad(call(), leaf)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float((g - want).abs().max()) <= 1e-5 * float(want.abs().max())      # (a projection's weight gradient may add atomically)
+
+
+def test_a_captured_projection_refuses_while_an_eager_graph_of_its_weight_lives():
+    lin, x = dv.HipLinear(32, 16).cuda(), torch.randn(5, 32, device="cuda")
+    alive = lin(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lin(x)
+        with pytest.raises(RuntimeError, match="HipLinear: this backward is being captured while"):
+            torch.autograd.grad(out, lin.weight, torch.ones_like(out))
+        del out
+    assert alive.shape == (5, 16)

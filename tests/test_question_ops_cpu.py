@@ -159,3 +159,14 @@ def test_projections_refuse_what_their_kernels_cannot_read():
     assert attend.half() is attend                                  # nn.Module's own cast, then refused by name
     with pytest.raises(RuntimeError, match="fp32 on one device; the weight"):
         attend(x, s)
+
+
+def test_the_look_at_a_captured_backward_finds_leaves_behind_views_and_copies():
+    ops = L.torch_ops()
+    x, w = torch.randn(3, 4, 10, requires_grad=True), torch.randn(10, 8, requires_grad=True)
+    found = lambda t: {id(u) for u in ops.dbg_leaves(t)}  # noqa: E731
+    assert found(x.reshape(-1, 10)) == {id(x)} == found(x.transpose(0, 2).contiguous()) == found(x[:, :, :5])
+    y = x.view(12, 10) @ w
+    assert found(y) == {id(x), id(w)} == found(torch.cat([y[:, :4].float(), y[:, 4:]]).exp())
+    assert found(y.detach()) == set() and found(x) == set()
+    assert not ops.dbg_refuses_capture(y)                           # nothing of a device
