@@ -138,11 +138,13 @@ bool dbg_refuses_capture(const Tensor& t) { return reaches({t.grad_fn().get()}, 
 struct OpNode : Node {
   const char* what = "";
   virtual variable_list gradients(variable_list&& grads) = 0;
+  // do the gradients depend on the upstream gradient alone?  Otherwise on the inputs too, one of which wants a gradient: there is a node.
+  virtual bool linear() const { return false; }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(num_outputs());
     refuse_capture(what, this);
-    const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
+    const bool again = at::GradMode::is_enabled() && (!linear() || grads[0].requires_grad());
     at::NoGradGuard no_grad;
     const c10::DeviceGuard guard(grads[0].device());
     variable_list out = gradients(std::move(grads));
@@ -164,6 +166,7 @@ struct EmbedNode : OpNode {
   int elem;
   float scale;
   std::string name() const override { return "EmbedTokensBackward"; }
+  bool linear() const override { return true; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     tokens_.reset_data();

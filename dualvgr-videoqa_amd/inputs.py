@@ -153,6 +153,19 @@ class TokenEmbedding(nn.Embedding):
             raise IndexError("TokenEmbedding: a token is outside the embedding table")
 
 
+class _Once(torch.autograd.Function):
+    """Gradients that are made outside autograd, in a backward that is itself recorded: differentiating them again raises."""
+
+    @staticmethod
+    def forward(ctx, what, *grads):
+        ctx.what = what
+        return tuple(g.detach() if g is not None else None for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what}: its gradient cannot be differentiated again")
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, dtype_code):
@@ -195,7 +208,10 @@ class _Linear(torch.autograd.Function):
         L_.check(lib.dvgr_linear_backward(x2.data_ptr(), w.data_ptr(), gy2.data_ptr(), gx.data_ptr() if gx is not None else None,
                                           gw.data_ptr(), gb.data_ptr() if gb is not None else None, M, N, K, code, stream),
                  "dvgr_linear_backward")
-        return (gx[:rows].view(*xshape) if gx is not None else None), gw, gb, None
+        grads = (gx[:rows].view(*xshape) if gx is not None else None), gw, gb
+        if torch.is_grad_enabled():
+            grads = _Once.apply("HipLinear", *(g.requires_grad_() if g is not None else None for g in grads))
+        return (*grads, None)
 
 
 class HipLinear(nn.Linear):

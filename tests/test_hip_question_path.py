@@ -401,3 +401,31 @@ def test_a_captured_projection_refuses_while_an_eager_graph_of_its_weight_lives(
             torch.autograd.grad(out, lin.weight, torch.ones_like(out))
         del out
     assert alive.shape == (5, 16)
+
+
+def test_a_gradient_of_a_constant_upstream_says_when_it_is_differentiated_again():
+    # a gradient penalty: the first gradient depends on the inputs, whatever comes from above
+    z, x = torch.randn(2, 9, device="cuda", requires_grad=True), torch.randn(1, 3, 2, 8, device="cuda", requires_grad=True)
+    v, i = torch.randn(2, 3, device="cuda"), torch.zeros(2, 3, device="cuda", dtype=torch.int64)
+    for call, leaf in ((lambda: dv.distillation_loss(z, v, i), z), (lambda: dv.distillation_loss(z.view(2, 1, 9), v[:, None], i[:, None], reduction="sum"), z),
+                       (lambda: dv.cross_attention(x, x.detach(), x.detach()).sum(), x), (lambda: dv.cross_attention(x.detach(), x, x.detach()).sum(), x),
+                       (lambda: dv.cross_attention(x.detach(), x.detach(), x).sum(), x)):
+        g, = torch.autograd.grad(call(), leaf, create_graph=True)
+        assert torch.equal(g.detach(), torch.autograd.grad(call(), leaf)[0])
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.square().sum().backward()
+    table = torch.randn(5, 8, device="cuda", requires_grad=True)    # linear: a constant upstream gives a constant gradient
+    g, = torch.autograd.grad(dv.embed_tokens(table, torch.arange(3, device="cuda")).sum(), table, create_graph=True)
+    assert not g.requires_grad
+
+
+def test_a_gradient_through_projections_says_when_it_is_differentiated_again():
+    torch.manual_seed(14)
+    m, lin = dv.CrossAttention(32, 2, state_dim=16).cuda(), dv.HipLinear(16, 8).cuda()
+    x, s, y = torch.randn(2, 4, 32, device="cuda", requires_grad=True), torch.randn(2, 5, 16, device="cuda"), torch.randn(3, 16, device="cuda", requires_grad=True)
+    for call, leaf in ((lambda: m(x, s).sum(), x), (lambda: lin(y).sum(), y), (lambda: lin(y.detach()).square().sum(), lin.weight)):
+        g, = torch.autograd.grad(call(), leaf, create_graph=True)
+        want, = torch.autograd.grad(call(), leaf)
+        assert float((g.detach() - want).abs().max()) <= 1e-5 * float(want.abs().max())
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (call() + g.square().sum()).backward()                  # a penalty beside a loss
