@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -63,6 +64,14 @@ void check(int code, const char* what) {
   TORCH_CHECK(code > 0 || why, what, " failed: ", code);
   TORCH_CHECK(code > 0, what, " failed: ", why);
   TORCH_CHECK(false, what, " failed: hipError_t ", code);
+}
+
+// What these nodes do not do and would not notice: an output without the tangent of its inputs reads as a constant, a trace would record
+// the output's allocation alone.
+void refuse_modes(const char* what, std::initializer_list<const Tensor*> inputs) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced");
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative; got an input with a tangent");
 }
 
 int elem_code(const Tensor& t, const char* what) {
@@ -185,6 +194,7 @@ struct EmbedNode : OpNode {
 
 Tensor embed_tokens(const Tensor& table, Tensor tokens, double scale, std::optional<int64_t> padding_idx, const OptTensor& bad) {
   const char* what = "embed_tokens";
+  refuse_modes(what, {&table});
   const int elem = elem_code(table, what);
   TORCH_CHECK(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0, what, ": the table is (vocab, wd), not empty; got ", table.sizes());
   const int64_t vocab = table.size(0), wd = table.size(1);
@@ -247,6 +257,7 @@ struct DistillNode : OpNode {
 // logits (R, C) with rows any distance apart, values and indices (R, K)
 Tensor distillation_loss(Tensor z, Tensor v, Tensor i, double temperature, int64_t reduction) {
   const char* what = "distillation_loss";
+  refuse_modes(what, {&z});
   const int elem = elem_code(z, what), elem_v = elem_code(v, what);
   const c10::DeviceGuard guard(z.device());
   const hipStream_t st = stream_of(z);
@@ -340,6 +351,7 @@ struct AttendNode : OpNode {
 
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lens_, const OptTensor& mask_, std::optional<double> scale_) {
   const char* what = "cross_attention";
+  refuse_modes(what, {&q, &k, &v});
   elem_code(q, what);
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(3) == k.size(3), what,
               ": q (B, Lq, H, Dh), k and v (B, Lk, Hk, Dh); got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());

@@ -429,3 +429,23 @@ def test_a_gradient_through_projections_says_when_it_is_differentiated_again():
         assert float((g.detach() - want).abs().max()) <= 1e-5 * float(want.abs().max())
         with pytest.raises(RuntimeError, match="differentiated again"):
             (call() + g.square().sum()).backward()                  # a penalty beside a loss
+
+
+def test_transforms_and_traces_are_refused_on_the_device():
+    import torch.autograd.forward_ad as fwd
+    ids, x = torch.zeros(2, 3, device="cuda", dtype=torch.int64), torch.randn(1, 4, 2, 8, device="cuda")
+    for call, t in ((lambda t: dv.embed_tokens(t, ids[0]), torch.randn(5, 8, device="cuda")),
+                    (lambda z: dv.distillation_loss(z, torch.zeros(2, 3, device="cuda"), ids), torch.randn(2, 9, device="cuda")),
+                    (lambda k: dv.cross_attention(x, k, x), x)):
+        with fwd.dual_level():
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(fwd.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, t, check_trace=False)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(torch.stack([t, t]))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda y: call(y).sum())(t)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (t,))
+        assert torch.isfinite(call(t)).all()

@@ -170,3 +170,22 @@ def test_the_look_at_a_captured_backward_finds_leaves_behind_views_and_copies():
     assert found(y) == {id(x), id(w)} == found(torch.cat([y[:, :4].float(), y[:, 4:]]).exp())
     assert found(y.detach()) == set() and found(x) == set()
     assert not ops.dbg_refuses_capture(y)                           # nothing of a device
+
+
+def _calls():
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    x = torch.randn(1, 4, 2, 8)
+    return [(lambda t: dv.embed_tokens(t, ids[0]), torch.randn(5, 8)), (lambda z: dv.distillation_loss(z, torch.zeros(2, 3), ids), torch.randn(2, 9)),
+            (lambda q: dv.cross_attention(q, x, x), x), (lambda k: dv.cross_attention(x, k, x), x), (lambda v: dv.cross_attention(x, x, v), x)]
+
+
+def test_inputs_with_a_tangent_and_traces_are_refused():
+    import torch.autograd.forward_ad as fwd
+    for call, t in _calls():
+        with fwd.dual_level():
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(fwd.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, t, check_trace=False)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call(t)
