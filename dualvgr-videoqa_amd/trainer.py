@@ -148,7 +148,8 @@ class TrainStep:
                  betas=(0.9, 0.999), eps: float = 1e-8, world: int = 1, unit_reducer=None, param_reducer=None,
                  distill_weight: float = 0.0, distill_temperature: float = 2.0):
         self.model = model
-        self.distill_weight, self.distill_temperature = float(distill_weight), float(distill_temperature)
+        self._distill_weight, self.distill_temperature = float(distill_weight), float(distill_temperature)
+        self._distills = self._distill_weight != 0.0         # or a weight is set later: a schedule may pass through 0
         self.unit = model.visual_input_unit
         self.head = model._head
         self.alpha, self.beta, self.world = float(alpha), float(beta), int(world)
@@ -174,6 +175,14 @@ class TrainStep:
     @property
     def lr(self):
         return self.opt.lr
+
+    @property
+    def distill_weight(self):
+        return self._distill_weight
+
+    @distill_weight.setter
+    def distill_weight(self, w):
+        self._distill_weight, self._distills = float(w), True
 
     def step_decay(self):
         """train.py:341-349: halve the learning rate."""
@@ -260,9 +269,10 @@ class TrainStep:
             self.opt.max_norm = float(sd["max_norm"])
 
     def __call__(self, video_appearance_feat, video_motion_feat, question, question_len, answers, teacher=None):
-        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None."""
-        if (teacher is None) != (self.distill_weight == 0.0):
-            raise ValueError("a teacher's top logits and distill_weight != 0 go together")
+        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None.  While `distill_weight` is 0 in a
+        schedule its loss is still in the result, and has no part in the step."""
+        if teacher is None and self.distill_weight != 0.0 or teacher is not None and not self._distills:
+            raise ValueError("a teacher's top logits and distill_weight go together")
         m, unit, head = self.model, self.unit, self.head
         # optimizer.zero_grad() (train.py:139): the unit's flat buffer is simply overwritten by the next backward
         unit.zero_grad_flat()
@@ -280,9 +290,10 @@ class TrainStep:
         raw = m.last_raw                                                     # (L, B, N, D) list tensors as the kernels wrote them
         roots, ups, kd = [logits, raw[3], raw[4], raw[5], raw[6]], [g_logits, g[3], g[4], g[5], g[6]], None
         if teacher is not None:
-            kd = distillation_loss(logits, *teacher, self.distill_temperature)
-            roots.append(kd)
-            ups.append(torch.full_like(kd, self.distill_weight, requires_grad=False))          # (a schedule may move the weight)
+            kd = distillation_loss(logits if self.distill_weight else logits.detach(), *teacher, self.distill_temperature)
+            if self.distill_weight:
+                roots.append(kd)
+                ups.append(torch.full_like(kd, self.distill_weight, requires_grad=False))      # (a schedule may move the weight)
         torch.autograd.backward(roots, ups)
         if self.unit_reducer is not None and not self._unit_shared:
             self.unit_reducer.finish()
@@ -308,5 +319,6 @@ class TrainStep:
         out = {"loss": loss, "ce": ce[0], "common": terms[1], "dependence": terms[2], "grad_sqnorm": sq[0], "logits": logits}
         if kd is not None:
             out["distill"] = kd.detach()
-            out["loss"] = loss + self.distill_weight * out["distill"]
+            if self.distill_weight:
+                out["loss"] = loss + self.distill_weight * out["distill"]
         return out

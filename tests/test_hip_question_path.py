@@ -449,3 +449,25 @@ def test_transforms_and_traces_are_refused_on_the_device():
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (t,), (t,))
         assert torch.isfinite(call(t)).all()
+
+
+def test_a_schedule_of_the_teachers_weight_passes_through_zero():
+    _, _, _, teacher, step, batch = small_step(0.5, True, keep=True)
+    bias = [n for n, _ in step.other if n.endswith("classifier.5.bias")][0]
+    none, g0, _, _ = small_step(0.0, False)
+    for w in (0.25, 0.0, 0.25):
+        step.distill_weight = w
+        out = step(*batch, teacher=teacher)
+        grad = dict(step.other)[bias].grad.clone()
+        z = out["logits"].detach().requires_grad_(True)
+        kd = dv.distillation_loss(z, *teacher, 2.0)
+        gz, = torch.autograd.grad(kd, z)
+        assert torch.equal(out["distill"], kd.detach())
+        assert abs(float(out["loss"] - none["loss"]) - w * float(kd.detach())) <= 1e-6 * float(none["loss"])
+        # (lr = 0: the logits are those of the first step up to its atomics, 1e-4 of their size)
+        assert float((grad - g0[bias] - w * gz.sum(0)).abs().max()) <= 1e-4 * float(z.detach().abs().max())
+    step.distill_weight = 0.0
+    step(*batch)                                                    # no teacher and no weight
+    step.distill_weight = 0.5
+    with pytest.raises(ValueError):
+        step(*batch)
