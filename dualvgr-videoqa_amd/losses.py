@@ -137,3 +137,8 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     lead, K = logits.shape[:-1], values.shape[-1]
     out = L_.torch_ops().distillation_loss(logits.reshape(-1, logits.shape[-1]), values.reshape(-1, K), indices.reshape(-1, K), temperature, code)
     return out.view(lead) if code == 0 else out
+
+
+def listed_rows(values: torch.Tensor, indices: torch.Tensor, classes: int) -> torch.Tensor:
+    """Number of rows that have an entry, as the mean of `distillation_loss` counts them."""
+    return ((indices >= 0) & (indices < classes) & (values != -torch.inf)).any(-1).sum()

@@ -60,6 +60,17 @@ def _all_reduce_stream_ordered(t: torch.Tensor, op, group) -> None:
         dist.all_reduce(t, op=op, group=group, async_op=True).wait()
 
 
+def sum_over_ranks(t: torch.Tensor, group=None) -> torch.Tensor:
+    """`t` summed over the ranks, in the current stream's order (RCCL; other backends take a copy in host memory)."""
+    if dist.get_backend(group) == "nccl":
+        t = t.clone()
+        _all_reduce_stream_ordered(t, dist.ReduceOp.SUM, group)
+        return t
+    h = t.cpu().clone()
+    dist.all_reduce(h, op=dist.ReduceOp.SUM, group=group)
+    return h.to(t.device)
+
+
 class CollectiveIssuer:
     """The ONE ordered place from which a process enqueues its gradient collectives on a device.
 

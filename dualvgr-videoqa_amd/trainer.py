@@ -15,7 +15,9 @@ flat segments (include/dvgr_optim.h) instead of PyTorch's per-tensor loops.  `st
 
 Data parallel (one process per GPU): pass `world` and the reducers; every rank's losses are means over its shard, the
 batch-SUM HSIC term is multiplied by `world`, and gradients are AVERAGED before the clip, so the
-step equals the single-process step on the concatenated batch.
+step equals the single-process step on the concatenated batch.  (The teacher's term is a mean over the pairs that the teacher lists,
+which differ in number between shards: the ranks add up that number, one small all-reduce of torch.distributed in front of the backward,
+and every rank's term is its sum over the mean number per rank.)
 
 A teacher's top answers can take part: `TrainStep(..., distill_weight=w, distill_temperature=T)` and `step(..., teacher=(values,
 indices))` add w * distillation_loss(logits, values, indices, T) to the loss (losses.distillation_loss).
@@ -28,7 +30,8 @@ from typing import Dict, List, Optional
 import torch
 
 from . import _lib as L_
-from .losses import distillation_loss
+from .losses import distillation_loss, listed_rows
+from .parallel import sum_over_ranks
 
 
 class OptimSeg(C.Structure):
@@ -268,8 +271,20 @@ class TrainStep:
         if "max_norm" in sd:
             self.opt.max_norm = float(sd["max_norm"])
 
+    def _distill(self, logits, values, indices):
+        """(a root, the factor that makes it this rank's term of the loss; None: it is that)"""
+        if self.world == 1:
+            return distillation_loss(logits, values, indices, self.distill_temperature), None
+        import torch.distributed as dist
+        group = getattr(self.param_reducer, "group", None) or getattr(self.unit_reducer, "group", None)
+        if not dist.is_initialized() or dist.get_world_size(group) != self.world:
+            raise RuntimeError(f"a teacher with world = {self.world} needs torch.distributed with as many ranks: they add up their listed pairs")
+        total = distillation_loss(logits, values, indices, self.distill_temperature, "sum")
+        rows = sum_over_ranks(listed_rows(values, indices, logits.shape[-1]), group)
+        return total, self.world / rows.clamp(min=1).float()
+
     def __call__(self, video_appearance_feat, video_motion_feat, question, question_len, answers, teacher=None):
-        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None.  While `distill_weight` is 0 in a
+        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None (the same on all ranks).  While `distill_weight` is 0 in a
         schedule its loss is still in the result, and has no part in the step."""
         if teacher is None and self.distill_weight != 0.0 or teacher is not None and not self._distills:
             raise ValueError("a teacher's top logits and distill_weight go together")
@@ -290,10 +305,11 @@ class TrainStep:
         raw = m.last_raw                                                     # (L, B, N, D) list tensors as the kernels wrote them
         roots, ups, kd = [logits, raw[3], raw[4], raw[5], raw[6]], [g_logits, g[3], g[4], g[5], g[6]], None
         if teacher is not None:
-            kd = distillation_loss(logits if self.distill_weight else logits.detach(), *teacher, self.distill_temperature)
-            if self.distill_weight:
+            kd, share = self._distill(logits if self.distill_weight else logits.detach(), *teacher)
+            if self.distill_weight:                                          # (a schedule may move the weight)
                 roots.append(kd)
-                ups.append(torch.full_like(kd, self.distill_weight, requires_grad=False))      # (a schedule may move the weight)
+                ups.append(torch.full_like(kd, self.distill_weight, requires_grad=False) if share is None else self.distill_weight * share)
+            kd = kd.detach() if share is None else kd.detach() * share
         torch.autograd.backward(roots, ups)
         if self.unit_reducer is not None and not self._unit_shared:
             self.unit_reducer.finish()
@@ -318,7 +334,7 @@ class TrainStep:
         loss = ce[0] + self.alpha * terms[1] + self.beta * terms[2]
         out = {"loss": loss, "ce": ce[0], "common": terms[1], "dependence": terms[2], "grad_sqnorm": sq[0], "logits": logits}
         if kd is not None:
-            out["distill"] = kd.detach()
+            out["distill"] = kd
             if self.distill_weight:
                 out["loss"] = loss + self.distill_weight * out["distill"]
         return out

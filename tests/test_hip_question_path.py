@@ -471,3 +471,72 @@ def test_a_schedule_of_the_teachers_weight_passes_through_zero():
     step.distill_weight = 0.5
     with pytest.raises(ValueError):
         step(*batch)
+
+
+def _teacher_rank(rank, world, rendezvous, q):
+    """A rank of TrainStep on GPU 0, gradients averaged over gloo through host memory; its teacher lists other numbers of pairs."""
+    import torch.distributed as dist
+    torch.cuda.set_device(0)
+    dist.init_process_group("gloo", init_method=rendezvous, rank=rank, world_size=world)
+    try:
+        seen = {}
+        for w in (0.5, 0.0):
+            _, _, _, (values, indices), step, batch = small_step(0.5, True, keep=True)
+            indices[rank + 1:] = -1                                 # rank + 1 pairs; 2 of the batch's are never listed
+            step.world, step.distill_weight = world, w
+            real = step.opt.step
+
+            def averaged(segs):
+                for seg in segs:
+                    h = seg[2].cpu()
+                    dist.all_reduce(h)
+                    seg[2].copy_(h / world)
+                return real(segs)
+
+            step.opt.step = averaged
+            out = step(*batch, teacher=(values, indices))
+            bias = [n for n, _ in step.other if n.endswith("classifier.5.bias")][0]
+            seen[w] = (dict(step.other)[bias].grad.cpu(), float(out["distill"]), out["logits"].detach().cpu(), values.cpu(), indices.cpu(),
+                       float(out["loss"] - out["ce"]))
+        q.put((rank, {w: tuple(x.numpy() if torch.is_tensor(x) else x for x in t) for w, t in seen.items()}))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.timeout(300)
+def test_a_teacher_that_lists_other_numbers_of_pairs_on_the_ranks():
+    import torch.multiprocessing as mp
+    from test_hip_parallel import _rendezvous
+    world = 2
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    rendezvous = _rendezvous()
+    procs = [ctx.Process(target=_teacher_rank, args=(r, world, rendezvous, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=240) for _ in range(world))
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    _, d, z, v, i, _ = zip(*(got[r][0.5] for r in range(world)))
+    z = torch.cat([torch.from_numpy(x) for x in z]).double().requires_grad_(True)
+    v, i = (torch.cat([torch.from_numpy(x) for x in t]) for t in (v, i))
+    listed = (i >= 0).any(1)
+    assert int(listed.sum()) == 3                                   # 1 of rank 0, 2 of rank 1
+    logp, logq = torch.log_softmax(v.double()[listed] / 2, 1), torch.log_softmax(z[listed] / 2, 1).gather(1, i[listed])
+    want = (logp.exp() * (logp - logq)).sum(1).mean() * 4           # the concatenated batch's mean
+    gz, = torch.autograd.grad(want, z)
+    assert abs(sum(d) / world - float(want)) <= 1e-5 * float(want)
+    assert abs((got[0][0.0][1] + got[1][0.0][1]) / world - float(want)) <= 1e-4 * float(want)      # (reported at weight 0 as well)
+    # the last bias's averaged gradient: with and without the term (lr does not matter: first steps of equal models, atomics 1e-4 of the logits)
+    for r in range(world):
+        moved = torch.from_numpy(got[r][0.5][0] - got[r][0.0][0]).double()
+        assert float((moved - 0.5 * gz.sum(0)).abs().max()) <= 1e-4 * float(z.detach().abs().max())
+    assert float(gz.sum(0).abs().max()) > 1e-3 * float(z.detach().abs().max())      # a mean over shards would be off by more than the bound
+
+
+def test_a_teacher_without_ranks_to_ask_is_refused():
+    _, _, _, teacher, step, batch = small_step(0.5, True, keep=True)
+    step.world = 2
+    with pytest.raises(RuntimeError, match="needs torch.distributed"):
+        step(*batch, teacher=teacher)

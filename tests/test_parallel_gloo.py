@@ -207,3 +207,38 @@ def test_shard_batch_partitions():
             assert all(a[1] == b[0] for a, b in zip(spans, spans[1:]))
             sizes = [b - a for a, b in spans]
             assert max(sizes) - min(sizes) <= 1
+
+
+def _worker_teacher(rank, world, port, q):
+    dist.init_process_group("gloo", init_method=port, rank=rank, world_size=world)
+    try:
+        values, indices = torch.zeros(5, 3), torch.zeros(5, 3, dtype=torch.int64)
+        indices[rank + 2:] = -1                                     # rank + 2 pairs are listed
+        indices[0, 1] = 9                                           # outside the classes, beside entries that are there
+        mine = losses.listed_rows(values, indices, 9)
+        q.put((rank, int(mine), int(parallel.sum_over_ranks(mine)), int(mine)))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.timeout(300)
+def test_ranks_add_up_the_pairs_that_their_teacher_lists():
+    world = 2
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    procs = [ctx.Process(target=_worker_teacher, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = sorted(q.get(timeout=240) for _ in range(world))
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    assert got == [(0, 2, 5, 2), (1, 3, 5, 3)]
+
+
+def test_listed_pairs_are_counted_as_the_mean_counts_them():
+    inf, nan = float("inf"), float("nan")
+    values = torch.tensor([[0.0, 1.0], [-inf, 1.0], [-inf, -inf], [nan, -inf], [1.0, 2.0], [-inf, 3.0]])
+    indices = torch.tensor([[0, 1], [0, 7], [0, 1], [2, 1], [-1, 9], [-1, 8]])
+    assert int(losses.listed_rows(values, indices, 9)) == 4         # not: -inf alone, outside the classes alone
