@@ -31,38 +31,38 @@ struct Distill {
   float invT, T;
 };
 
-// Per row, for the backward, in powers of two: {max of z / T, log2 sum of 2^(z / T - max), the same of v}; a row without entries has a
-// maximum of -inf for v and neither loss nor gradient.
+// Per row, for the backward: {max of z, log2 sum of exp((z - max) / T), the same of v}; a row without entries has a maximum of -inf for v
+// and neither loss nor gradient.
 struct RowStats { float zmax, zlog, vmax, vlog; };
 
-// Running maximum (in powers of two: x c) and sum of exp((x - max) / T); a maximum of -inf holds nothing.  Every use of a maximum is the
-// same rounded number, so its rounding cancels, and a term costs one fused multiply-add and one exponential.
+// Running maximum and sum of exp((x - max) / T) = 2^((x - max) c); a maximum of -inf holds nothing.  The maximum is one of the numbers
+// themselves and is taken off before the scaling: x c rounded would be off by more than an exponential bears from |x c| = 2^31 on.
 struct MaxSum {
   float m = -INFINITY, l = 0.f;
-  __device__ __forceinline__ void join(float m2, float l2) {
+  __device__ __forceinline__ void join(float m2, float l2, float c) {
     const float mn = fmaxf(m, m2);
     if (mn == -INFINITY) { l += l2; return; }                       // (l, l2: 0, or NaN)
-    l = l * exp2_fast(m - mn) + l2 * exp2_fast(m2 - mn);
+    l = l * exp2_fast((m - mn) * c) + l2 * exp2_fast((m2 - mn) * c);
     m = mn;
   }
   template <int N> __device__ __forceinline__ void add(const float (&f)[N], float c) {
     float mx = f[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) mx = fmaxf(mx, f[i]);
-    const float mn = fmaxf(m, mx * c), ref = mn == -INFINITY ? 0.f : mn;
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += exp2_fast(fmaf(f[i], c, -ref));
-    l = l * exp2_fast(m - ref) + s;
+    for (int i = 0; i < N; ++i) s += exp2_fast((f[i] - ref) * c);
+    l = l * exp2_fast((m - ref) * c) + s;
     m = mn;
   }
 };
 
-__device__ __forceinline__ MaxSum wave_join(MaxSum a) {
+__device__ __forceinline__ MaxSum wave_join(MaxSum a, float c) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const float m2 = __shfl_xor(a.m, d), l2 = __shfl_xor(a.l, d);
-    a.join(m2, l2);
+    a.join(m2, l2, c);
   }
   return a;
 }
@@ -102,12 +102,12 @@ __device__ __forceinline__ MaxSum row_part(const T* row, int64_t c0, int64_t c1,
             s.add(f, c);
           },
           [&](int64_t at) { float f[1] = {(float)row[at]}; s.add(f, c); });
-  s = wave_join(s);
+  s = wave_join(s, c);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (lane == 0) { sh[2 * wave] = s.m; sh[2 * wave + 1] = s.l; }
   __syncthreads();
   s.m = sh[0]; s.l = sh[1];
-  for (int w = 1; w < kThreads / 64; ++w) s.join(sh[2 * w], sh[2 * w + 1]);
+  for (int w = 1; w < kThreads / 64; ++w) s.join(sh[2 * w], sh[2 * w + 1], c);
   return s;
 }
 
@@ -141,14 +141,14 @@ template <typename T> struct Entries {
       one(d, r, k, x[0], y);
       t.add(x, c);
     }
-    t = wave_join(t);
+    t = wave_join(t, c);
     if (t.l != t.l) t.m = t.l;                                      // a NaN among the values is the row's loss
     float sum = 0.f;
     if (t.m != -INFINITY) {
       const float vlog = __log2f(t.l);
       const auto add = [&](float x, float y) {
         if (x == -INFINITY) return;                                 // p = 0 adds nothing, whatever the student says there
-        const float logp = fmaf(x, c, -t.m) - vlog, logq = fmaf(y, c, -s.m) - zlog, p = exp2_fast(logp);
+        const float logp = fmaf(x - t.m, c, -vlog), logq = fmaf(y - s.m, c, -zlog), p = exp2_fast(logp);
         if (p != 0.f) sum += p * (logp - logq);
       };
 #pragma unroll
@@ -189,8 +189,9 @@ __global__ __launch_bounds__(64) void k_distill_join(Distill d, const float2* pa
   Entries<T> e;
   e.fetch(d, r, threadIdx.x);
   MaxSum s;
-  for (int i = threadIdx.x; i < d.splits; i += 64) s.join(part[r * d.splits + i].x, part[r * d.splits + i].y);
-  e.finish(d, r, wave_join(s), loss, stats, threadIdx.x);
+  const float c = d.invT * kLog2e;
+  for (int i = threadIdx.x; i < d.splits; i += 64) s.join(part[r * d.splits + i].x, part[r * d.splits + i].y, c);
+  e.finish(d, r, wave_join(s, c), loss, stats, threadIdx.x);
 }
 
 // the sum of the rows' losses (/ number of rows that have an entry); behind the rows' statistics, the factor of a row's gradient
@@ -228,12 +229,12 @@ __global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowSt
   const float c = d.invT * kLog2e;
   const bool empty = s.vmax == -INFINITY;
   const float f = empty ? 0.f : (up_stride ? up[r] : *up * stats[d.R].zmax) * d.T;
-  const auto grad = [&](float z) { return empty ? 0.f : f * exp2_fast(fmaf(z, c, -s.zmax) - s.zlog); };
+  const auto grad = [&](float z) { return empty ? 0.f : f * exp2_fast(fmaf(z - s.zmax, c, -s.zlog)); };
   for (int k = tid; k < d.K; k += kThreads) {
     float v = -INFINITY;
     const int i = entry(d, r, k, v);
     sh_i[k] = i;
-    sh_p[k] = i < 0 || empty ? 0.f : exp2_fast(fmaf(v, c, -s.vmax) - s.vlog);
+    sh_p[k] = i < 0 || empty ? 0.f : exp2_fast(fmaf(v - s.vmax, c, -s.vlog));
   }
   if (SAME)
     for_row(row, c0, c1, tid, [&](int64_t at, int64_t e) {

@@ -205,3 +205,29 @@ def test_another_stream_and_a_captured_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+@pytest.mark.parametrize("C", [700, 40000])                         # a row in one workgroup, in shares
+@pytest.mark.parametrize("t,base,T", [(torch.float32, 3e9, 1.0), (torch.float32, 1e10, 1.0), (torch.float32, -1e10, 1.0), (torch.float32, 3e38, 2.0),
+                                      (torch.float32, -3e38, 1.0), (torch.float32, 5000.0, 1e-6), (torch.bfloat16, 1e12, 1.0), (torch.bfloat16, 30000.0, 1e-6),
+                                      (torch.float16, 60000.0, 1e-6), (torch.float16, -4000.0, 1e-6)])
+def test_finite_logits_of_any_size(t, base, T, C):
+    # two classes share the maximum, everything else is thousands of exponents below it: q = 1/2, 1/2, 0, .. to the last bit
+    z = torch.full((3, C), base, device="cuda", dtype=t)
+    step = 2.0 ** -3 * abs(base)
+    z -= torch.linspace(0.5, 1.0, C, device="cuda").to(t) * torch.tensor(step, device="cuda").to(t)
+    assert torch.isfinite(z).all()
+    z[:, 5], z[:, C - 7] = base, base
+    z.requires_grad_(True)
+    idx = torch.tensor([[5, 9], [C - 7, 5], [5, -1]], device="cuda")
+    v = torch.full((3, 2), base, device="cuda", dtype=t)
+    v[0, 1] = torch.tensor(base - step, device="cuda").to(t)        # p = (1, 0); (1/2, 1/2); (1)
+    rows = dv.distillation_loss(z, v, idx, T, "none")
+    ln2 = 0.6931471805599453
+    want = torch.tensor([ln2, 0.0, ln2], device="cuda", dtype=torch.float64) * T * T
+    assert ((rows.double() - want).abs() <= 2.0 ** -20 * T * T).all(), rows
+    up = 1.0 / T                                                    # (the gradient's factor is T: fp16 would lose 1e-6)
+    g, = torch.autograd.grad(rows, z, torch.full_like(rows, up))
+    want = torch.zeros(3, C, device="cuda", dtype=torch.float64)
+    want[0, 5], want[0, C - 7], want[2, 5], want[2, C - 7] = -0.5, 0.5, -0.5, 0.5
+    assert ((g.double() - want).abs() <= 2.0 ** -10).all()
