@@ -21,9 +21,14 @@ namespace {
 // for memory, move it at once.
 constexpr float kSlack = 8.f;
 
+struct Max {
+  float at = -INFINITY, cm = 0.f;   // a score; c times it, rounded, 0 where there is none
+  bool far = false;                 // the same in all lanes
+  float slack;                      // in scores
+};
+
 // KS 32-key tiles of a wave's online softmax: s in, probabilities out, m, l and o brought to the new maximum
-template <int KS, int NT, bool MANY> __device__ __forceinline__ void softmax_tiles(f32x16 (&s)[KS], unsigned long long bits, float c, float& m, float& l, f32x16 (&o)[NT],
-                                                                        int lane) {
+template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (&s)[KS], unsigned long long bits, float c, Max& m, float& l, f32x16 (&o)[NT], int lane) {
   if (bits != (KS == 2 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
@@ -37,28 +42,42 @@ template <int KS, int NT, bool MANY> __device__ __forceinline__ void softmax_til
   for (int i = 0; i < KS; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
-  mx = half_max(mx) * c;
-  if (__any(mx > m + (MANY ? kSlack : 0.f))) {
-    const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);      // nothing summed yet: o and l are 0
+  mx = half_max(mx);
+  if (__any(mx > m.at + m.slack)) {
+    const float mn = fmaxf(m.at, mx), cm = mn == -INFINITY ? 0.f : mn * c;
+    m.far = any_far(cm);
+    const float f = m.at == -INFINITY ? 0.f : exp2_fast(m.far ? (m.at - mn) * c : m.cm - cm);      // nothing summed yet: o and l are 0
     l *= f;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[u][r] *= f;
-    m = mn;
+    m.at = mn;
+    m.cm = cm;
   }
-  const float ref = m == -INFINITY ? 0.f : m;
+  if (m.far) {
+    const float ref = m.at == -INFINITY ? 0.f : m.at;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast((s[i][r] - ref) * c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], c, -m.cm));
+  }
 #pragma unroll
   for (int i = 0; i < KS; ++i) {
     float sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[i][r] = exp2_fast(fmaf(s[i][r], c, -ref));
-      sum += s[i][r];
-    }
+    for (int r = 0; r < 16; ++r) sum += s[i][r];
     l += sum;
   }
 }
+
+// the row's sum as a score: p = 2^(c (s - log_sum)) in the backward; +inf for a row without keys, so that every p is 0
+__device__ __forceinline__ float log_sum(const Args& A, float m, float l) { return l == 0.f ? INFINITY : m + __log2f(l) / A.c; }
 
 // a row's output from o (unnormalised), with what its rounding leaves, and its log-sum
 template <typename T, int NT> __device__ __forceinline__ void write_row(const Args& A, int b, int hk, int row, const f32x16 (&o)[NT], float m, float l,
@@ -78,8 +97,7 @@ template <typename T, int NT> __device__ __forceinline__ void write_row(const Ar
       if (lo) store4<T>(lo + d * sizeof(T), x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
     }
   }
-  // log2 of the row's sum, in units of the scaled scores; +inf for a row without keys: every exp2(s - lse) of the backward is 0
-  if (A.a.lse && lane < 32 && stats) A.a.lse[row_index(A, b, hk, row)] = l == 0.f ? INFINITY : m + __log2f(l);
+  if (A.a.lse && lane < 32 && stats) A.a.lse[row_index(A, b, hk, row)] = log_sum(A, m, l);
 }
 
 // ---- many rows: W x 32 of them, tiles of KS x 32 keys -----------------------------------------------------------------------------
@@ -111,7 +129,9 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(A
   f32x16 o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = zero16();
-  float m = -INFINITY, l = 0.f;
+  Max m;
+  m.slack = kSlack / A.c;
+  float l = 0.f;
 
   Stage<T, DP, KT, 64 * W> sk, sv;
   uint32_t there = 0;                                               // lane j: key j of the next tile
@@ -137,12 +157,12 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_fwd(A
 #pragma unroll
       for (int i = 0; i < KS; ++i) s[i] = mma(Tl::frag(lk + i * 32 * Tl::kStride, st, lane), qf[st], s[i]);
     if (sizeof(T) == 2) reads_ahead<KS * Tl::kSteps>();
-    softmax_tiles<KS, NT, true>(s, bits, A.c, m, l, o, lane);
+    softmax_tiles<KS, NT>(s, bits, A.c, m, l, o, lane);
 #pragma unroll
     for (int i = 0; i < KS; ++i) mma_tr<DP>(o, lv + i * 32 * Tl::kStrideT, s[i], lane, T());
   }
   l = half_sum(l);
-  if (live) write_row<T>(A, b, hk, row, o, m, l, 0, 1, true, lane);
+  if (live) write_row<T>(A, b, hk, row, o, m.at, l, 0, 1, true, lane);
 }
 
 // ---- 32 rows: KW waves over different keys -----------------------------------------------------------------------------------------
@@ -166,7 +186,9 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
   f32x16 o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = zero16();
-  float m = -INFINITY, l = 0.f;
+  Max mt;
+  mt.slack = 0.f;
+  float l = 0.f;
   WaveStage<T, DP> sk, sv;
   uint32_t there = 0;
   const auto fetch = [&](int t) {
@@ -193,10 +215,11 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
     f32x16 s[1] = {zero16()};
 #pragma unroll
     for (int st = 0; st < Tl::kSteps; ++st) s[0] = mma(Tl::frag(lk, st, lane), Tl::frag(lq, st, lane), s[0]);
-    softmax_tiles<1, NT, false>(s, bits, A.c, m, l, o, lane);
+    softmax_tiles<1, NT>(s, bits, A.c, mt, l, o, lane);
     mma_tr<DP>(o, lv, s[0], lane, T());
   }
   l = half_sum(l);
+  float m = mt.at;
 
   if (KW > 1) {                                                     // join the waves
     __syncthreads();
@@ -207,10 +230,10 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 ? 2 : 1)) void k_attn_few_
     float mj = -INFINITY;
 #pragma unroll
     for (int k = 0; k < KW; ++k) mj = fmaxf(mj, ml[k * 64 + col]);
-    const float ref = mj == -INFINITY ? 0.f : mj, fac = exp2_fast(m - ref);
+    const float ref = mj == -INFINITY ? 0.f : mj, fac = exp2_fast((m - ref) * A.c);
     l = 0.f;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) l += ml[k * 64 + 32 + col] * exp2_fast(ml[k * 64 + col] - ref);
+    for (int k = 0; k < KW; ++k) l += ml[k * 64 + 32 + col] * exp2_fast((ml[k * 64 + col] - ref) * A.c);
     m = mj;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -272,11 +295,11 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
     float mn = m;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) mn = fmaxf(mn, ml[i].x);
-    const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_fast(m - ref);
+    const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_fast((m - ref) * A.c);
     l *= f0; x *= f0; y *= f0;
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const float f = exp2_fast(ml[i].x - ref);
+      const float f = exp2_fast((ml[i].x - ref) * A.c);
       l += ml[i].y * f;
       x += o[i].x * f; y += o[i].y * f;
     }
@@ -291,7 +314,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
   x = y = l = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = exp2_fast(sh[w][129] - ref);
+    const float f = exp2_fast((sh[w][129] - ref) * A.c);
     x += sh[w][d] * f; y += sh[w][d + 1] * f; l += sh[w][128] * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -302,7 +325,7 @@ __global__ __launch_bounds__(256) void k_attn_join(Args A) {
     out[d] = (T)x; out[d + 1] = (T)y;
     if (lo) { lo[d] = (T)(x - (float)(T)x); lo[d + 1] = (T)(y - (float)(T)y); }
   }
-  if (A.a.lse && lane == 0) A.a.lse[row_index(A, b, hk, row)] = l == 0.f ? INFINITY : m + __log2f(l);
+  if (A.a.lse && lane == 0) A.a.lse[row_index(A, b, hk, row)] = log_sum(A, m, l);
 }
 
 template <typename T, int DP, int KS, int W> int launch_many(const Args& A, hipStream_t st) {

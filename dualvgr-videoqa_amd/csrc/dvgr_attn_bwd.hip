@@ -1,6 +1,6 @@
 // dvgr_attn_bwd.hip -- include/dvgr_attn.h: attention to an encoder's states, backward.
 //
-//     P = exp2(c q.k - lse)      D = rowsum(dO o O)      dS = P o (dO V^T - D)
+//     P = exp2(c (q.k - lse))     D = rowsum(dO o O)      dS = P o (dO V^T - D)
 //     dV = P^T dO      dK = scale dS^T Q      dQ = scale dS K
 //
 // Many rows: two passes over the scores, neither with atomics: one owns keys and goes over the packed rows (dK, dV; the heads of a
@@ -119,8 +119,8 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   extern __shared__ __align__(16) char lds[];
   char* lq = lds;
   char* lg = lq + Tl::template bytesT<RT>();
-  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [lse, D][RT]
-  char* lval = reinterpret_cast<char*>(lstat + 2 * RT);
+  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [c lse, D, lse][RT]
+  char* lval = reinterpret_cast<char*>(lstat + 3 * RT);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * B.rs.splits * ktiles, ktiles);
@@ -169,7 +169,11 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     __syncthreads();
     sq.template put<Tl::kStrideT>(lq, tid);
     sg.template put<Tl::kStrideT>(lg, tid);
-    if (tid < 2 * RT) lstat[tid] = t * RT + tid % RT < A.rows ? stat : tid < RT ? INFINITY : 0.f;      // (no row: p = 0)
+    if (tid < 2 * RT) {
+      const float x = t * RT + tid % RT < A.rows ? stat : tid < RT ? INFINITY : 0.f;      // (no row: p = 0)
+      lstat[tid] = tid < RT ? x * A.c : x;
+      if (tid < RT) lstat[2 * RT + tid] = x;
+    }
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
 #pragma unroll 1
@@ -185,17 +189,29 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
         else dp = mma(Tl::fragT(tg, st, lane), vf[st], dp);
       }
       const float* ls = lstat + (rw * RS + i) * 32 + (lane >> 5) * 4;
+      if (any_far(lstat[(rw * RS + i) * 32 + (lane & 31)])) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 e = *reinterpret_cast<const float4*>(ls + 2 * RT + 8 * g);
+          const float ee[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * g + j] = exp2_fast((s[4 * g + j] - ee[j]) * A.c);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 e = *reinterpret_cast<const float4*>(ls + 8 * g);
+          const float ee[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * g + j] = exp2_fast(fmaf(s[4 * g + j], A.c, -ee[j]));
+        }
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 e = *reinterpret_cast<const float4*>(ls + 8 * g), d = *reinterpret_cast<const float4*>(ls + RT + 8 * g);
-        const float ee[4] = {e.x, e.y, e.z, e.w}, dd[4] = {d.x, d.y, d.z, d.w};
+        const float4 d = *reinterpret_cast<const float4*>(ls + RT + 8 * g);
+        const float dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * g + j;
-          const float p = exp2_fast(fmaf(s[r], A.c, -ee[j]));       // (a key that is not there: its column alone, cleared at the end)
-          s[r] = p;
-          dp[r] = grad16<T>(p * (dp[r] - dd[j]), sc);
-        }
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] = grad16<T>(s[4 * g + j] * (dp[4 * g + j] - dd[j]), sc);      // (a key that is not there: its column alone, cleared at the end)
       }
       mma_tr<DP>(dv, tg, s, lane, T());
       mma_tr<DP>(dk, tq, dp, lane, T());
@@ -316,7 +332,8 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(Bw
   const int64_t ri = row_index(A, b, hk, live ? row : 0);
   float stats[2] = {live ? A.a.lse[ri] : INFINITY, live ? B.delta[ri] : 0.f};
   settle(stats);
-  const float lse = stats[0], delta = stats[1];
+  const float lse = stats[0], delta = stats[1], lse_c = lse * A.c;
+  const bool far = any_far(lse_c);
   const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
   f32x16 dq[NT];
 #pragma unroll
@@ -347,8 +364,15 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(Bw
       for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tk, st, lane), qf[st], s);
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tv, st, lane), gf[st], dp);
+      if (far) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = grad16<T>(exp2_fast(fmaf(s[r], A.c, -lse)) * (dp[r] - delta), sc);
+        for (int r = 0; r < 16; ++r) s[r] = exp2_fast((s[r] - lse) * A.c);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], A.c, -lse_c));
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = grad16<T>(s[r] * (dp[r] - delta), sc);
       if ((uint32_t)(bits >> (32 * i)) != ~0u) {
         const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
 #pragma unroll
@@ -513,7 +537,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * g + j;
-        const float p = exp2_fast(fmaf(s[r], A.c, -ee[j]));         // (a key that is not there: its column alone, cleared as it leaves)
+        const float p = exp2_fast((s[r] - ee[j]) * A.c);         // (a key that is not there: its column alone, cleared as it leaves)
         s[r] = p;
         dp[r] = here ? grad16<T>(p * (dp[r] - dd[j]), sc) : 0.f;
         scr[(8 * g + h4 + j) * kScr + col] = dp[r];
@@ -605,7 +629,7 @@ template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t w
 template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 2 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
+  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 3 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
   const size_t join = RW > 1 ? (size_t)KW * RW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
   if (bytes < join) bytes = join;
   const int64_t keys = (int64_t)B.f.a.B * B.f.a.Hk * B.f.a.Lk;

@@ -364,3 +364,40 @@ def test_module_against_its_formula_and_word_by_word(dtype):
         o = torch.einsum("bhlj,bjhd->blhd", sc.softmax(3), v.cpu()).reshape(3, 6, 128)
         want = o @ m.out.weight.double().cpu().t() + m.out.bias.double().cpu()
         assert float((y.cpu() - want).abs().max()) <= (1e-5 if dtype == "fp32" else 4e-2)
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H", [(2, 3, 40, 2), (2, 3, 500, 2), (1, 1, 5000, 2), (2, 200, 300, 2), (64, 300, 70, 4), (16, 40, 33, 16), (1, 3000, 20, 2)])
+@pytest.mark.parametrize("t,size,scale", [(torch.float32, 1e5, 1.0), (torch.float32, 1e18, 1.0), (torch.float32, 2.0, 1e30), (torch.bfloat16, 1e6, 1.0),
+                                          (torch.bfloat16, 3.0, 1e28), (torch.float16, 60000.0, 1.0), (torch.float16, 0.5, 1e20)])
+def test_finite_scores_of_any_size(t, size, scale, B, Lq, Lk, H):
+    # one number of each head carries the score: size^2 scale = 4e9 to 1e36 for the best key, at most 7/8 of it for the others
+    Dh, gen = 32, torch.Generator(device="cuda").manual_seed(Lk)
+    q, k = torch.zeros(B, Lq, H, Dh, device="cuda", dtype=t), torch.zeros(B, Lk, H, Dh, device="cuda", dtype=t)
+    v = torch.randn(B, Lk, H, Dh, generator=gen, device="cuda").to(t)
+    up = (torch.randn(B, Lq, H, Dh, generator=gen, device="cuda") * 2.0 ** -6).to(t)
+    q[..., 3] = size
+    k[..., 3] = (torch.linspace(-0.875, 0.875, Lk, device="cuda") * size).to(t)[None, :, None]
+    best, twin = Lk // 3, Lk - 2
+    k[:, best, :, 3] = size
+    q.requires_grad_(True), k.requires_grad_(True), v.requires_grad_(True)
+    o = cross_attention(q, k, v, scale=scale)
+    assert torch.equal(o, v[:, best:best + 1].expand(B, Lq, H, Dh))                      # all of the best key, to the bit
+    gq, gk, gv = torch.autograd.grad(o, [q, k, v], up)
+    want = up.double().sum(1)
+    step = torch.finfo(t).eps / 2
+    assert ((gv[:, best].double() - want).abs() <= want.abs() * step + Lq * 2.0 ** -24 * up.double().abs().sum(1)).all()
+    gv[:, best] = 0
+    assert (gv == 0).all()
+    # p (dP - D) = 0 for the best key up to the rounding of two sums of Dh products, for every row of it; and 0 for the others
+    err = (2 * Dh * 2.0 ** -24) * (up.double().abs() * v[:, best:best + 1].double().abs()).sum(3, keepdim=True)
+    # (a bound beyond the type's largest number allows what such a number rounds to, an infinity: fp16 at scale 1e20, where the bound is
+    # 1e20 x 0.5 x 2^-18 x sum |up v|, at least 1e10 while the sum is over 2^-14, and the largest number 65504)
+    for got, bound in ((gq, scale * size * err * 1.01), (gk[:, best], scale * size * 1.01 * err.sum(1))):
+        assert (got.double().abs() <= torch.where(bound > torch.finfo(t).max, torch.inf, bound)).all()
+    gk[:, best] = 0
+    assert (gk == 0).all()
+    with torch.no_grad():                                           # two keys share the maximum
+        k[:, twin, :, 3] = size
+        o = cross_attention(q, k, v, scale=scale).double()
+        want = (v[:, best:best + 1].double() + v[:, twin:twin + 1].double()) / 2
+        assert ((o - want).abs() <= want.abs() * step + 2.0 ** -22).all()
