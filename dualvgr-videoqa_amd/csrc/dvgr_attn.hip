@@ -391,9 +391,10 @@ int check(const dvgr_attn_problem* a) {
   if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->Hk < 1 || a->H % a->Hk || a->Dh < 8 || a->Dh > 128 || a->Dh % 8) return DVGR_E_DIMS;
   if (!(a->scale >= 1e-30f) || !(a->scale <= 1e30f)) return DVGR_E_DIMS;
   const int64_t rows = (int64_t)a->Lq * (a->H / a->Hk), heads = (int64_t)a->B * a->Hk;
-  // packed rows and keys are 32-bit numbers, a launch holds at most 2^32 threads (256 for 64 rows, 512 for 128 keys)
+  // packed rows and keys are 32-bit numbers, a launch holds fewer than 2^32 threads (256 for 64 rows; 512 for 128 keys, workgroups rounded
+  // up to a multiple of 8)
   if (rows >= (1ll << 30) || a->Lk >= (1 << 30) || heads >= (1ll << 22)) return DVGR_E_DIMS;
-  if (heads * (rows / 64 + 1) >= (1ll << 24) || heads * (a->Lk / 128 + 1) >= (1ll << 23)) return DVGR_E_DIMS;
+  if (heads * (rows / 64 + 1) >= (1ll << 24) || heads * (a->Lk / 128 + 1) > (1ll << 23) - 8) return DVGR_E_DIMS;
   return 0;
 }
 bool empty(const dvgr_attn_problem& a) { return a.B == 0 || a.Lq == 0; }

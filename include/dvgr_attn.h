@@ -29,7 +29,7 @@ typedef struct dvgr_attn_view {
 typedef struct dvgr_attn_problem {
   int32_t B, Lq, Lk;       /* samples, queries and keys of a sample; any may be 0                        */
   int32_t H, Hk;           /* query heads, key heads; H a multiple of Hk                                 */
-  int32_t Dh;              /* head size: a multiple of 8, 8 .. 128.  B Hk (Lq H / Hk / 64 + 1) < 2^24, B Hk (Lk / 128 + 1) < 2^23 */
+  int32_t Dh;              /* head size: a multiple of 8, 8 .. 128.  B Hk (Lq H / Hk / 64 + 1) < 2^24, B Hk (Lk / 128 + 1) <= 2^23 - 8 */
   int32_t elem;            /* DVGR_ELEM_*                                                                */
   float scale;             /* 1e-30 .. 1e30                                                              */
   dvgr_attn_view q, k, v;

@@ -189,3 +189,12 @@ def test_inputs_with_a_tangent_and_traces_are_refused():
             torch.jit.trace(call, t, check_trace=False)
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call(t)
+
+
+def test_attention_stays_under_a_launch_of_2_32_threads():
+    # dK and dV: 512 threads for 128 keys, workgroups rounded up to a multiple of 8; D: 256 threads for 64 rows
+    check = lambda **kw: L.load().dvgr_attn_check(C.byref(problem(B=1, H=1, Hk=1, **kw)))  # noqa: E731
+    for tiles in range((1 << 23) - 16, 1 << 23):
+        grid = (tiles + 7) // 8 * 8
+        assert (check(Lk=128 * tiles - 1) == 0) == (grid * 512 < 1 << 32), tiles
+    assert check(Lq=(1 << 30) - 1) == E_DIMS and check(Lq=(1 << 30) - 128) == 0
