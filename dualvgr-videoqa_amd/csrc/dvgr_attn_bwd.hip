@@ -16,9 +16,35 @@ namespace attn {
 namespace {
 
 // fp16 has 5 bits of exponent: the score gradients are scaled by the power of two that puts the largest |dO| of the sample's head
-// group into [0.5, 1), so that small upstream gradients do not vanish, and held inside the type's range.
+// group into [0.5, 1), so that small upstream gradients do not vanish.  With values near the type's largest they then reach
+// p (1 - p) 2 Dh |v| = 2^22: a wave whose tile holds one beyond the type takes that tile's product kHold times smaller, its sums for the
+// moment too (powers of two: nothing is rounded).
 template <typename T> struct Grad16 { static constexpr bool on = false; };
 template <> struct Grad16<f16_t> { static constexpr bool on = true; };
+constexpr float kHold = 256.f;
+template <typename T> __device__ __forceinline__ bool beyond_type(const f32x16& ds) {          // the same in all lanes
+  if (!Grad16<T>::on) return false;
+  float top = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+  return __any(top > 65504.f);
+}
+template <int NT> __device__ __forceinline__ void scale_tiles(f32x16 (&x)[NT], float f) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[t][r] *= f;
+}
+// acc[t] += M^T ds (mma_tr) with the score gradients of a tile
+template <typename T, int DP> __device__ __forceinline__ void mma_grad(f32x16 (&acc)[DP / 32], const char* at, f32x16& ds, bool beyond, int lane) {
+  if (Grad16<T>::on && beyond) {
+    scale_tiles(acc, 1.f / kHold);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] *= 1.f / kHold;
+  }
+  mma_tr<DP>(acc, at, ds, lane, T());
+  if (Grad16<T>::on && beyond) scale_tiles(acc, kHold);
+}
 __device__ __forceinline__ float grad_scale(uint32_t top) {
   const int e = (int)(top >> 23);                                   // bits of the largest |dO|
   return e == 0 || e >= 255 ? 1.f : ldexpf(1.f, 126 - e);
@@ -82,10 +108,8 @@ __global__ __launch_bounds__(256) void k_attn_delta(BwdArgs B) {
   if (threadIdx.x == 0) atomicMax(&B.top[b * A.a.Hk + hk], __float_as_uint(fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]))));
 }
 
-// score gradient as the matrix unit takes it; infinities and NaN stay what they are (a scaled loss that overflows is found by them)
-template <typename T> __device__ __forceinline__ float grad16(float ds, float sc) {
-  return Grad16<T>::on && fabsf(ds) < INFINITY ? fminf(fmaxf(ds * sc, -65504.f), 65504.f) : ds;
-}
+// score gradient as the matrix unit takes it (infinities and NaN stay what they are: a scaled loss that overflows is found by them)
+template <typename T> __device__ __forceinline__ float grad16(float ds, float sc) { return Grad16<T>::on ? ds * sc : ds; }
 
 // a row of dQ, or of its part from one share of the keys
 template <typename T, int NT> __device__ __forceinline__ void write_dq(const BwdArgs& B, int b, int hk, int split, int row, const f32x16 (&dq)[NT], float f,
@@ -214,7 +238,7 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
         for (int j = 0; j < 4; ++j) dp[4 * g + j] = grad16<T>(s[4 * g + j] * (dp[4 * g + j] - dd[j]), sc);      // (a key that is not there: its column alone, cleared at the end)
       }
       mma_tr<DP>(dv, tg, s, lane, T());
-      mma_tr<DP>(dk, tq, dp, lane, T());
+      mma_grad<T, DP>(dk, tq, dp, beyond_type<T>(dp), lane);
     }
   }
   if (RW > 1) {                                                     // add the waves that went over other rows, dK then dV
@@ -378,7 +402,7 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(Bw
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = reg_bit(hb, r) ? s[r] : 0.f;
       }
-      mma_tr<DP>(dq, tk, s, lane, T());
+      mma_grad<T, DP>(dq, tk, s, beyond_type<T>(s), lane);
     }
   }
   if (live) write_dq<T>(B, b, hk, split, row, dq, A.a.scale / sc, 0, 1, lane);
@@ -544,6 +568,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
       }
     }
     wave_order();
+    const bool beyond = beyond_type<T>(dp);
     if (B.g_q.p) {
       f32x16 x;                                                     // rows = keys, column = this lane's packed row
 #pragma unroll
@@ -551,7 +576,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
         const float4 y = *reinterpret_cast<const float4*>(scr + col * kScr + 8 * g + h4);
         x[4 * g] = y.x; x[4 * g + 1] = y.y; x[4 * g + 2] = y.z; x[4 * g + 3] = y.w;
       }
-      mma_tr<DP>(dq, lk, x, lane, T());
+      mma_grad<T, DP>(dq, lk, x, beyond, lane);
     }
     if (B.g_k.p) {
 #pragma unroll
@@ -560,7 +585,7 @@ __global__ __launch_bounds__(64 * KW, (sizeof(T) == 2 && DP <= 96 ? 2 : 1)) void
       leave(B.g_v, t, 1.f, bits);
 #pragma unroll
       for (int u = 0; u < NT; ++u) acc[u] = zero16();
-      mma_tr<DP>(acc, lq, dp, lane, T());
+      mma_grad<T, DP>(acc, lq, dp, beyond, lane);
       leave(B.g_k, t, fac, bits);
     }
   }

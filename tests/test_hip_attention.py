@@ -401,3 +401,21 @@ def test_finite_scores_of_any_size(t, size, scale, B, Lq, Lk, H):
         o = cross_attention(q, k, v, scale=scale).double()
         want = (v[:, best:best + 1].double() + v[:, twin:twin + 1].double()) / 2
         assert ((o - want).abs() <= want.abs() * step + 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk", [(2, 6, 40, 2, 2), (2, 5, 300, 4, 2), (2, 70, 20, 2, 1), (2, 70, 300, 2, 2), (64, 300, 70, 4, 4)])
+def test_large_values_of_half_precision_do_not_hold_the_gradient_back(B, Lq, Lk, H, Hk):
+    # values near the type's largest, flat upstream gradients: differences of dO V^T of 2^19 largest |dO|, where a scaled score gradient of p = 1/2
+    # is beyond the type; the queries are small, so that the gradients themselves are not
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    q = (torch.randn(B, Lq, H, 128, generator=gen, device="cuda") * 2.0 ** -4).half()
+    k = (torch.randn(B, Lk, Hk, 128, generator=gen, device="cuda") * 2.0 ** -4).half()
+    sign = torch.where(torch.rand(128, generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    v = torch.randn(B, Lk, Hk, 128, generator=gen, device="cuda")
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    for j in (1, Lk - 2):                                           # two keys share each row, with opposite values
+        k[:, j, :, 0] = 16.0
+        v[:, j] = 60000.0 * sign * (1 if j == 1 else -1)
+    up = (torch.ones(B, Lq, H, 128, device="cuda") * sign * 2.0 ** -12).half()
+    up[:, ::2] = -up[:, ::2]
+    check(q.requires_grad_(True), k.requires_grad_(True), v.half().requires_grad_(True), up=up)
