@@ -55,23 +55,22 @@ template <int KS, int NT> __device__ __forceinline__ void softmax_tiles(f32x16 (
     m.at = mn;
     m.cm = cm;
   }
-  if (m.far) {
-    const float ref = m.at == -INFINITY ? 0.f : m.at;
+  if (m.far) {                                                      // (in front of the exponentials, which stay in one block with the products behind)
+    const float at = m.at == -INFINITY ? 0.f : m.at;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast((s[i][r] - ref) * c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[i][r] = exp2_fast(fmaf(s[i][r], c, -m.cm));
+      for (int r = 0; r < 16; ++r) s[i][r] -= at;
   }
+  const float ref = m.far ? 0.f : m.cm;
 #pragma unroll
   for (int i = 0; i < KS; ++i) {
     float sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sum += s[i][r];
+    for (int r = 0; r < 16; ++r) {
+      s[i][r] = exp2_fast(fmaf(s[i][r], c, -ref));
+      sum += s[i][r];
+    }
     l += sum;
   }
 }

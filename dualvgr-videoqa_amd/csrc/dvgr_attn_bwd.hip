@@ -143,8 +143,8 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
   extern __shared__ __align__(16) char lds[];
   char* lq = lds;
   char* lg = lq + Tl::template bytesT<RT>();
-  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [c lse, D, lse][RT]
-  char* lval = reinterpret_cast<char*>(lstat + 3 * RT);
+  float* lstat = reinterpret_cast<float*>(lg + Tl::template bytesT<RT>());       // [c lse, D, lse, 0][RT]
+  char* lval = reinterpret_cast<char*>(lstat + 4 * RT);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave % RW;
   const int ktiles = (A.a.Lk + KT - 1) / KT;
   const int64_t w = xcd_work((int64_t)A.a.B * A.a.Hk * B.rs.splits * ktiles, ktiles);
@@ -188,6 +188,7 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     const int r = t * RT + tid % RT;
     if (tid < 2 * RT) stat = from[row_index(A, b, hk, r < A.rows ? r : A.rows - 1)];
   };
+  if (tid < RT) lstat[3 * RT + tid] = 0.f;
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
@@ -204,6 +205,7 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
     for (int i = 0; i < RS; ++i) {
       const char* tq = lq + (rw * RS + i) * 32 * Tl::kStrideT;
       const char* tg = lg + (rw * RS + i) * 32 * Tl::kStrideT;
+      const bool far = any_far(lstat[(rw * RS + i) * 32 + (lane & 31)]);
       f32x16 s = zero16(), dp = zero16();                             // rows = packed rows, column = this lane's key
 #pragma unroll
       for (int st = 0; st < Tl::kSteps; ++st) s = mma(Tl::fragT(tq, st, lane), kf[st], s);
@@ -213,29 +215,27 @@ __global__ __launch_bounds__(64 * KW * RW, (sizeof(T) == 2 && KW > 1 ? 2 : 1)) v
         else dp = mma(Tl::fragT(tg, st, lane), vf[st], dp);
       }
       const float* ls = lstat + (rw * RS + i) * 32 + (lane >> 5) * 4;
-      if (any_far(lstat[(rw * RS + i) * 32 + (lane & 31)])) {
+      if (far) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 e = *reinterpret_cast<const float4*>(ls + 2 * RT + 8 * g);
           const float ee[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[4 * g + j] = exp2_fast((s[4 * g + j] - ee[j]) * A.c);
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 e = *reinterpret_cast<const float4*>(ls + 8 * g);
-          const float ee[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[4 * g + j] = exp2_fast(fmaf(s[4 * g + j], A.c, -ee[j]));
+          for (int j = 0; j < 4; ++j) s[4 * g + j] -= ee[j];
         }
       }
+      const float* lc = far ? ls + 3 * RT : ls;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 d = *reinterpret_cast<const float4*>(ls + RT + 8 * g);
-        const float dd[4] = {d.x, d.y, d.z, d.w};
+        const float4 e = *reinterpret_cast<const float4*>(lc + 8 * g), d = *reinterpret_cast<const float4*>(ls + RT + 8 * g);
+        const float ee[4] = {e.x, e.y, e.z, e.w}, dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dp[4 * g + j] = grad16<T>(s[4 * g + j] * (dp[4 * g + j] - dd[j]), sc);      // (a key that is not there: its column alone, cleared at the end)
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g + j;
+          const float p = exp2_fast(fmaf(s[r], A.c, -ee[j]));       // (a key that is not there: its column alone, cleared at the end)
+          s[r] = p;
+          dp[r] = grad16<T>(p * (dp[r] - dd[j]), sc);
+        }
       }
       mma_tr<DP>(dv, tg, s, lane, T());
       mma_grad<T, DP>(dk, tq, dp, beyond_type<T>(dp), lane);
@@ -356,8 +356,9 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(Bw
   const int64_t ri = row_index(A, b, hk, live ? row : 0);
   float stats[2] = {live ? A.a.lse[ri] : INFINITY, live ? B.delta[ri] : 0.f};
   settle(stats);
-  const float lse = stats[0], delta = stats[1], lse_c = lse * A.c;
-  const bool far = any_far(lse_c);
+  const float lse = stats[0], delta = stats[1];
+  const bool far = any_far(lse * A.c);
+  const float ref = far ? 0.f : lse * A.c;
   const float sc = Grad16<T>::on ? grad_scale(B.top[b * A.a.Hk + hk]) : 1.f;
   f32x16 dq[NT];
 #pragma unroll
@@ -390,13 +391,10 @@ __global__ __launch_bounds__(64 * W, (sizeof(T) == 2 ? 2 : 1)) void k_attn_dq(Bw
       for (int st = 0; st < Tl::kSteps; ++st) dp = mma(Tl::frag(tv, st, lane), gf[st], dp);
       if (far) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_fast((s[r] - lse) * A.c);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_fast(fmaf(s[r], A.c, -lse_c));
+        for (int r = 0; r < 16; ++r) s[r] -= lse;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = grad16<T>(s[r] * (dp[r] - delta), sc);
+      for (int r = 0; r < 16; ++r) s[r] = grad16<T>(exp2_fast(fmaf(s[r], A.c, -ref)) * (dp[r] - delta), sc);
       if ((uint32_t)(bits >> (32 * i)) != ~0u) {
         const uint32_t hb = half_bits((uint32_t)(bits >> (32 * i)), lane);
 #pragma unroll
@@ -654,7 +652,7 @@ template <typename K> int launch(K kern, std::atomic<uint32_t>& asked, int64_t w
 template <typename T, int DP, int KW, int RW, int RS> int launch_dkv(const BwdArgs& B, hipStream_t st) {
   typedef Tile<T, DP> Tl;
   static std::atomic<uint32_t> asked{0};
-  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 3 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
+  size_t bytes = 2 * Tl::template bytesT<RW * RS * 32>() + 4 * RW * RS * 32 * sizeof(float) + (sizeof(T) == 2 && DP == 128 && KW > 1 ? KW * Tl::template bytes<32>() : 0);
   const size_t join = RW > 1 ? (size_t)KW * RW * Tl::kNT * 16 * 64 * sizeof(float) : 0;
   if (bytes < join) bytes = join;
   const int64_t keys = (int64_t)B.f.a.B * B.f.a.Hk * B.f.a.Lk;
