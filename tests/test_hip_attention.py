@@ -419,3 +419,17 @@ def test_large_values_of_half_precision_do_not_hold_the_gradient_back(B, Lq, Lk,
     up = (torch.ones(B, Lq, H, 128, device="cuda") * sign * 2.0 ** -12).half()
     up[:, ::2] = -up[:, ::2]
     check(q.requires_grad_(True), k.requires_grad_(True), v.half().requires_grad_(True), up=up)
+
+
+@pytest.mark.parametrize("shape", [(2, 20, 60, 4, 2, 64), (2, 15, 500, 4, 4, 96), (1, 1, 3000, 8, 2, 64), (2, 200, 330, 2, 1, 128), (64, 140, 70, 4, 4, 32), (1, 1500, 30, 1, 1, 64)])
+@pytest.mark.parametrize("t", TYPES)
+def test_rows_with_scores_of_very_different_size_side_by_side(t, shape):
+    # some rows of a tile are beyond what is taken off with the scaling, some are not, and keys grow so that a row passes from one to the other
+    q, k, v, gen = tensors(*shape, t, sharp=1.0)
+    size = torch.tensor([1.0, 40.0, 1.0, 3000.0, 200.0], device="cuda")
+    with torch.no_grad():
+        q.mul_(size[torch.arange(shape[1], device="cuda") % 5].to(t)[None, :, None, None])
+        k.mul_(torch.linspace(0.01, 8.0, shape[2], device="cuda").to(t)[None, :, None, None])
+    check(q, k, v)
+    lens = torch.randint(1, shape[2] + 1, (shape[0],), generator=gen, device="cuda")
+    check(q, k, v, lens, torch.rand(shape[0], shape[2], generator=gen, device="cuda") < 0.8)
