@@ -224,8 +224,9 @@ template <typename T> __device__ __forceinline__ void store4(char* p, float a, f
 
 // An 8-XCD chip hands workgroup i to XCD i % 8: give every XCD a contiguous run of the work, so that the workgroups that read the same
 // keys share an L2.  A head with 8 workgroups or more (`tiles`) has one on every XCD instead: samples of different lengths would leave
-// XCDs without work (captions over long videos of 50 to 100 % of 4096 states: dK and dV 750 us with runs, 620 without; the forward 340,
-// 310).  -1: nothing to do.
+// XCDs without work (2 x 4096 queries over 2100 and 4000 keys, 16 / 4 heads of 128, bf16: forward 272 us with runs, 214 without; forward and
+// backward 1275, 1063).  Without lengths there is little between them: full keys 280, 277 and 1294, 1296; 8 x 2048 x 2048, 16 heads of 64,
+// 195, 202 and 827, 855.  -1: nothing to do.
 __device__ __forceinline__ int64_t xcd_work(int64_t total, int tiles = 1) {
   if (tiles >= 8) return blockIdx.x < total ? (int64_t)blockIdx.x : -1;
   const int64_t per = (total + 7) / 8, w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);

@@ -6,8 +6,10 @@
 // keys and are joined at the end (dvgr_attn_few.h); the keys are split over workgroups, joined by a second launch, while there are
 // few of them.
 //
-// 2 x 4096 queries over 2048 to 4096 keys, 16 / 4 heads of 128, bf16: 272 us, 850 TFLOP/s of products (a large matrix product: 1198), its
-// waves issuing arithmetic most of the time.  64 x 15 queries over 1024 masked keys, 8 heads of 96, bf16: 32 us, 4.7 TB/s.  One query over
+// 2 x 4096 queries over 2048 to 4096 keys, 16 / 4 heads of 128, bf16: 250 to 280 us from card to card, 850 TFLOP/s of products (a large matrix
+// product: 1198).  Nothing is full there: matrix units 38 % of the time, LDS 33 % (10 of them conflicts), vector arithmetic about as long as the
+// products, while a wave goes through product, softmax, product and two of a SIMD overlap a part of it.  2 x 1024 x 1024, 16 heads of 64,
+// fp32: 82 us, matrix units 60 %.  64 x 15 queries over 1024 masked keys, 8 heads of 96, bf16: 32 us, 4.7 TB/s.  One query over
 // 65536 keys, 32 / 8 heads of 128, bf16: 47 us, 5.7 TB/s, and 4.7 for the join.
 #include "dvgr_attn_few.h"
 

@@ -7,8 +7,10 @@
 // group are rows of the same reduction), one owns rows and goes over the keys (dQ).  The scores are computed in both: 7 products
 // instead of 5, for results that do not depend on the schedule.  Up to 32 rows: one pass over the keys does it all.
 //
-// 2 x 4096 queries over 2048 to 4096 keys, 16 / 4 heads of 128, bf16: dQ 350 us, 990 TFLOP/s of products; dK and dV 610 us, 775, bound by
-// LDS (five reads of a tile for its four products), a fifth of the compute units without work where samples differ in length.
+// 2 x 4096 queries over 2048 to 4096 keys, 16 / 4 heads of 128, bf16: dQ 325 to 355 us from card to card, 990 TFLOP/s of products, matrix units
+// 49 % of the time, LDS 37; dK and dV 575 to 625 us, 775, matrix units 43 % of the busy compute units' time, LDS 49 (11 of them conflicts; five
+// reads of a tile for its four products), waves waiting 41 %; a quarter of the compute units without work where samples differ in length.
+// 2 x 1024 x 1024, 16 heads of 64, fp32: dQ 110 us, dK and dV 171, matrix units 67 and 70 %.
 #include "dvgr_attn_few.h"
 
 namespace dvgr {

@@ -96,7 +96,10 @@ inline Shares shares_of(int64_t units, int64_t turns, int64_t want, int least) {
 // types while there are fewer than two workgroups for each compute unit (eight fill its registers as two of four do, with half the
 // shares to join).  The keys are split over workgroups while there are fewer than that, in shares of at least two turns.
 // KW = 0: the kernels for many rows, which have no need of it: every compute unit has a workgroup of 128 rows.  (The backward adds up
-// over all rows at once, so it takes at most 32.)
+// over all rows at once, so it takes at most 32.)  Where these rows are many and short of that the split keys are not always worth what
+// every 32 rows pay to fetch them again.  Forward, here and with the kernel for many rows, us: 8 samples of 8 heads of 64, fp16, 120 queries
+// over 512 / 4096 keys 7.6 / 28 and 12.4 / 70, 256 queries 10.4 / 51 and 12.8 / 71; 8 heads of 128, bf16, 1000 queries 11.7 / 45 and 17.3 / 94,
+// 2000 queries 22 / 86 and 18 / 95, 3968 queries 47 / 231 and 20 / 102.
 struct FewPlan { int KW, splits, tiles_per_split; };
 inline FewPlan few_plan(const dvgr_attn_problem& a, bool forward) {
   FewPlan p{};

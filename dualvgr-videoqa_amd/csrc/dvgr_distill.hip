@@ -214,7 +214,8 @@ __global__ __launch_bounds__(1024) void k_distill_total(const float* loss, RowSt
   stats[R].zmax = (float)f;
 }
 
-// SAME: z and its gradient have the same alignment, row by row.  A share is written densely first; the classes the teacher lists
+// SAME: z and its gradient have the same alignment, row by row; otherwise elements are written one by one (4096 rows of 50257 classes, bf16,
+// forward and backward: 399 us as a slice of rows of 50304, 230 us for dense rows of 50304).  A share is written densely first; the classes the teacher lists
 // are then written again with their p, which needs no atomics: entries of the same class all write the same sum.
 template <typename T, bool SAME>
 __global__ __launch_bounds__(kThreads) void k_distill_bwd(Distill d, const RowStats* stats, const float* up, int up_stride, T* __restrict__ gz, int64_t ldg) {

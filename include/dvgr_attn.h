@@ -8,10 +8,11 @@
  * in one projection's output.  H query heads share Hk key heads, query head h reads key head h / (H / Hk).  Key j of sample b is
  * there if j < lens[b] and mask[b][j] != 0; what lies in the others is never used, NaN included.  A query with no key gives zeros.
  * Scores, softmax statistics and sums are fp32; for bf16 / fp16 the probabilities and the score gradients are rounded to the element
- * type as operands of the matrix unit, as q, k and v are.  Finite scores may have any size; the backward knows a row's softmax sum as one
- * fp32 score, so its probabilities are off by up to 2^-22 |scale q.k| relative (keys that share a maximum beyond 2^23 count as 1 each).
- * Conventions as in dvgr.h: nothing is allocated or synchronised, launches
- * go to `stream` of the current device, 0 / DVGR_E_* / hipError_t return codes. */
+ * type as operands of the matrix unit, as q, k and v are (with many rows taken at up to 2^8 times their size: results are off by 0.0024
+ * relative in bf16, rms, where rounding them alone would leave 0.0017).  Finite scores may have any size; the backward knows a row's
+ * softmax sum as one fp32 score, so its probabilities are off by up to 2^-22 |scale q.k| relative (keys that share a maximum beyond 2^23
+ * count as 1 each).  Conventions as in dvgr.h: nothing is allocated or synchronised, launches go to `stream` of the current device,
+ * 0 / DVGR_E_* / hipError_t return codes. */
 #ifndef DVGR_ATTN_H
 #define DVGR_ATTN_H
 #include "dvgr.h"
