@@ -89,18 +89,13 @@ Tensor bytes_on(const Tensor& t, size_t n) { return at::empty({(int64_t)n}, t.op
 
 // ---- captured backwards ---------------------------------------------------------------------------------------------------------
 // autograd runs a node on the stream where it was made, and keeps one accumulation node for a leaf while any graph of it lives.  A
-// backward that is captured and runs into a node of a stream outside the capture would draw that stream in, which ends the process: it
-// is refused instead.  So the nodes in front of an operator are looked through, down to the leaves, while its backward is captured (and
-// only then), whatever stands between it and them: views, copies, other operators.
+// backward that is captured and runs into a node of the default stream would draw that stream into the capture, which it cannot be
+// part of and which ends the process: it is refused instead.  (Other streams join the capture and leave it again; wrappers that keep
+// accumulation nodes make them on one.)  So the nodes in front of an operator are looked through, down to the leaves, while its backward is
+// captured (and only then), whatever stands between it and them: views, copies, other operators.
 bool outside_capture(Node* n) {
-  const auto s = n->stream();
-  if (!s) return false;                                             // (not a device's)
-  const hipStream_t st = at::hip::HIPStreamMasqueradingAsCUDA(at::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *s).stream();
-  if (st == nullptr) return true;                                   // (the null stream cannot be captured, nor asked while another is)
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(st, &status) == hipSuccess) return status == hipStreamCaptureStatusNone;
-  (void)hipGetLastError();
-  return true;
+  const auto s = n->stream();                                       // (none: not a device's)
+  return s && at::hip::HIPStreamMasqueradingAsCUDA(at::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *s).stream() == nullptr;
 }
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 // the nodes that the running backward reaches from `todo`, each once, until `found` says yes to one
@@ -127,7 +122,7 @@ void refuse_capture(const char* what, Node* n) {
   for (size_t i = 0; i < n->num_outputs(); ++i)
     if (n->task_should_compute_output(i)) from.push_back(n->next_edge(i).function.get());
   TORCH_CHECK(!reaches(std::move(from), outside_capture), what, ": this backward is being captured while a graph of the same leaves lives that was "
-              "made on another stream: drop that graph's outputs (or detach them) before the capture");
+              "made on the default stream: drop that graph's outputs (or detach them) before the capture");
 }
 // the same for the node of a Python autograd function, from inside its backward
 void refuse_capture_here(const std::string& what) {

@@ -339,7 +339,8 @@ def test_which_graphs_a_captured_backward_may_not_run_into():
     assert refuses(x.view(2, 96)) and refuses(z.transpose(1, 2).contiguous())              # eager, on the null stream
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        assert refuses(x.exp())                                     # eager, on a stream that no capture knows
+        w = torch.randn(3, device="cuda", requires_grad=True)
+        assert not refuses(w.exp())                                 # eager, on another stream: it joins the capture and leaves it again
     graph = torch.cuda.CUDAGraph()
     alive = x.view(2, 96)
     with torch.cuda.graph(graph):
@@ -540,3 +541,40 @@ def test_a_teacher_without_ranks_to_ask_is_refused():
     step.world = 2
     with pytest.raises(RuntimeError, match="needs torch.distributed"):
         step(*batch, teacher=teacher)
+
+
+def test_a_captured_backward_runs_beside_an_eager_graph_of_another_stream():
+    # a wrapper that keeps accumulation nodes makes them on a side stream, and captures on yet another one
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    x, z = torch.randn(2, 6, 2, 16, generator=gen, device="cuda", requires_grad=True), torch.randn(3, 20, generator=gen, device="cuda", requires_grad=True)
+    table, ids = torch.randn(30, 8, generator=gen, device="cuda", requires_grad=True), torch.randint(0, 30, (3, 4), generator=gen, device="cuda")
+    lin = dv.HipLinear(16, 8).cuda()
+    leaves = [x, z, table, lin.weight]
+
+    def step():
+        loss = dv.cross_attention(x, x, x).square().sum() + dv.distillation_loss(z, table[:3, :4].detach(), ids, 2.0)
+        loss = loss + dv.embed_tokens(table, ids).square().sum() + lin(x.view(24, 16)).square().sum()
+        return torch.autograd.grad(loss, leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = [t.view_as(t) for t in leaves]
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_(torch.randn(t.shape, generator=gen, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(held, want):
+            assert float((a - b).abs().max()) <= 1e-5 * float(b.abs().max())
+    assert len(alive) == 4
