@@ -116,7 +116,8 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     data and gets no gradient.  An index outside [0, C) (-1, say) marks an entry that is not there, so rows may list fewer than K;
     entries of the same class add up.  A row without entries has loss 0 and gradient 0.  reduction: "mean" over the rows that
     have an entry (0 if none has), "sum", or "none" (the rows, shaped logits.shape[:-1]).  The loss is fp32, the gradient has the
-    logits' type; 1e-6 <= temperature <= 1e6."""
+    logits' type; 1e-6 <= temperature <= 1e6.  A row's loss is off by about T^2 2^-21 (1 + log C), its logarithms being fp32: from
+    temperatures of 100 on that shows where the lists hold nearly all of the distribution."""
     code = REDUCTIONS.get(reduction)
     if code is None:
         raise RuntimeError(f"distillation_loss: reduction is one of {sorted(REDUCTIONS)}; got {reduction!r}")

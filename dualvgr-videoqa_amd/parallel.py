@@ -295,6 +295,7 @@ class NativeUnitReducer:
             raise RuntimeError("NativeUnitReducer needs a ROCm device (RCCL); CPU jobs use LayerBucketReducer over gloo")
         self.lib = _comm_lib()
         self.device = device
+        self.group = group
         if dist.is_initialized():
             self.rank, self.world = dist.get_rank(group), dist.get_world_size(group)
         elif force_single:

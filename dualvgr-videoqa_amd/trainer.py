@@ -284,8 +284,8 @@ class TrainStep:
         return total, self.world / rows.clamp(min=1).float()
 
     def __call__(self, video_appearance_feat, video_motion_feat, question, question_len, answers, teacher=None):
-        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None (the same on all ranks).  While `distill_weight` is 0 in a
-        schedule its loss is still in the result, and has no part in the step."""
+        """`teacher`: (values (B, K), indices (B, K)) of a teacher's top logits for this batch, or None (the same on all ranks).  While
+        `distill_weight` is 0 in a schedule its loss is still in the result, and has no part in the step."""
         if teacher is None and self.distill_weight != 0.0 or teacher is not None and not self._distills:
             raise ValueError("a teacher's top logits and distill_weight go together")
         m, unit, head = self.model, self.unit, self.head

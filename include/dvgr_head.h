@@ -88,7 +88,9 @@ int dvgr_head_cross_entropy(const dvgr_head_dims *d, int C_valid, const float *l
  * an entry of value -inf has p = 0; entries of the same class add up.  A row without entries has loss 0 and gradient 0.
  * loss_rows: (R) fp32.  total: one float, the sum of the rows (DVGR_DISTILL_SUM) or the mean over the rows that have an entry, 0 if
  * none has (DVGR_DISTILL_MEAN); unused for DVGR_DISTILL_NONE (nullable).
- * stats: (R + 1, 4) fp32, 16-byte aligned, filled for the backward.  1e-6 <= temperature <= 1e6. */
+ * stats: (R + 1, 4) fp32, 16-byte aligned, filled for the backward.  1e-6 <= temperature <= 1e6.  Finite logits may have any size.  The
+ * logarithms are fp32: a row's loss is off by about temperature^2 2^-21 (1 + log C), which matters from temperatures of 100 on where the
+ * lists hold nearly all of the distribution and the loss itself is of the size of 1. */
 #define DVGR_DISTILL_MAX_K 1024
 #define DVGR_DISTILL_NONE 0
 #define DVGR_DISTILL_SUM 1
